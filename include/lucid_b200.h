@@ -427,6 +427,93 @@ int lucid_cp_solve_bwd(int B, int H, int N, int D, float scale, int blk_lo, int 
                        void* dv, int64_t dv_sb, int64_t dv_sh, int64_t dv_sn, int* status, void* stream);
 
 /*
+ * Paged cache of raw keys and solved values.  A pool is [P, Hkv, ps, D] bf16 (P pages of
+ * ps tokens) given by its base address and the element strides (sp, sh, sn), the D
+ * stride being 1; D is a multiple of 4 up to 128, base addresses and strides multiples of
+ * 8 bytes (16 for the wide loads).  block_table is int32 [B][M] with row stride t_sb: the
+ * token t of sequence b lies in row t % ps of page block_table[b][t / ps].  lengths is
+ * int32 [B]: the tokens cached before the call; a negative length marks an unused place
+ * of the batch, which gives zeros and writes nothing.  Tables and lengths are device
+ * memory; what only the device can see is checked there: a page outside [0, P), a
+ * length above M ps, a row past the table or a token outside the vocabulary is not
+ * followed but recorded in `status` (one int32, device memory or mapped host memory, NULL:
+ * not recorded; code 4 page, 5 length, 6 token, | kernel tag << 20), and the results of
+ * that call are not valid.
+ *
+ * lucid_paged_decode_step: LucidAttention's decoding step (modeling_lucid.py:467-481,
+ *   then :505-549) for one new token per sequence:
+ *     x_new = v_new - sum_{t < n} exp(s k^_new . k^_t - 1/s) x_t      (rounded to bf16)
+ *     o     = softmax over the n cached tokens and the new one of s q . k, times x
+ *   q, o [B, Hq, D], k_new, v_new, x_new [B, Hkv, D] with strides (sb, sh).  append != 0
+ *   also writes k_new and x_new into row n of the sequence's pages.
+ * lucid_paged_decode_attn: the attention alone, over the n cached tokens (none: zeros).
+ * Both split the cached tokens of the whole batch evenly over the GPU whatever the
+ * lengths; sums are fp32, results are the same from run to run.
+ */
+size_t lucid_paged_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int step);
+int lucid_paged_decode_step(int B, int Hq, int Hkv, int D, int P, int ps, int M, float scale, float eps,
+                            const void* q, int64_t q_sb, int64_t q_sh,
+                            const void* k_new, int64_t kn_sb, int64_t kn_sh,
+                            const void* v_new, int64_t vn_sb, int64_t vn_sh,
+                            void* k_pages, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn,
+                            void* x_pages, int64_t xp_sp, int64_t xp_sh, int64_t xp_sn,
+                            const int* block_table, int64_t t_sb, const int* lengths,
+                            void* x_new, int64_t xn_sb, int64_t xn_sh,
+                            void* o, int64_t o_sb, int64_t o_sh, int append, int* status,
+                            void* workspace, size_t workspace_bytes, void* stream);
+int lucid_paged_decode_attn(int B, int Hq, int Hkv, int D, int P, int ps, int M, float scale,
+                            const void* q, int64_t q_sb, int64_t q_sh,
+                            const void* k_pages, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn,
+                            const void* x_pages, int64_t xp_sp, int64_t xp_sh, int64_t xp_sn,
+                            const int* block_table, int64_t t_sb, const int* lengths,
+                            void* o, int64_t o_sb, int64_t o_sh, int* status,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Page movement.
+ * lucid_paged_append: rows i < counts[b] (counts NULL: all N) of k and x [B, Hkv, N, D]
+ *   into the rows lengths[b] + i of the sequences' pages; B at most 65535.
+ * lucid_copy_pages: page dst[i] = page src[i] in every layer of both pools, i < pairs.
+ *   src / dst are host arrays, read before the call returns; every dst is named once and
+ *   is no src (LUCID_ERR_SHAPE otherwise).  Pools are [layers, P, ...] with byte strides
+ *   (layer, page), a page being page_bytes (a multiple of 8) dense bytes.
+ */
+int lucid_paged_append(int B, int Hkv, int N, int D, int P, int ps, int M,
+                       const void* k, int64_t k_sb, int64_t k_sh, int64_t k_sn,
+                       const void* x, int64_t x_sb, int64_t x_sh, int64_t x_sn,
+                       void* k_pages, int64_t kp_sp, int64_t kp_sh, int64_t kp_sn,
+                       void* x_pages, int64_t xp_sp, int64_t xp_sh, int64_t xp_sn,
+                       const int* block_table, int64_t t_sb, const int* lengths, const int* counts,
+                       int* status, void* stream);
+int lucid_copy_pages(int layers, int P, int64_t page_bytes, void* k_pages, int64_t k_layer, int64_t k_page,
+                     void* x_pages, int64_t x_layer, int64_t x_page, const int* src, const int* dst, int pairs,
+                     void* stream);
+
+/*
+ * Token log probabilities of rows of logits, and their gradient.  Row r0 * R1 + r1 of
+ * the R0 x R1 rows starts at element r0 s0 + r1 s1; V logits a row, contiguous; dtype
+ * 0 bf16, 1 fp16, 2 fp32.
+ *   logprobs[r] = log softmax(x)[tokens[r]]   (tokens NULL: not computed; token -100:
+ *                 0 and no gradient)
+ *   entropy[r]  = -sum p log p
+ *   top_tokens / top_logprobs [R][top]: the most likely tokens, likeliest first, ties to
+ *                 the lowest index; top at most LUCID_MAX_TOP and V
+ *   stats [R][2]: for the backward
+ * Entries of -inf have probability 0.  A row without a distribution (all -inf, a NaN or
+ * +inf) gives NaN, top tokens -1.
+ * lucid_token_logprobs_bwd: dlogits [R][V] (contiguous, the logits' dtype) =
+ *   g_logprobs (1[token] - p) - g_entropy p (log p + H); either factor may be NULL (zero).
+ *   Rows with both factors zero are written as zeros without being read.
+ */
+#define LUCID_MAX_TOP 64
+int lucid_token_logprobs(int64_t R0, int64_t R1, int V, int dtype, const void* logits, int64_t s0, int64_t s1,
+                         const int64_t* tokens, int top, float* logprobs, float* entropy, float* stats,
+                         float* top_logprobs, int64_t* top_tokens, int* status, void* stream);
+int lucid_token_logprobs_bwd(int64_t R0, int64_t R1, int V, int dtype, const void* logits, int64_t s0, int64_t s1,
+                             const int64_t* tokens, const float* stats, const float* entropy, const float* g_logprobs,
+                             const float* g_entropy, void* dlogits, void* stream);
+
+/*
  * Kernel timing hook (benchmarks).  While enabled for one kernel family,
  * every launch of that family's main kernel is bracketed by a pair of CUDA
  * events recorded on the launch stream; lucid_profile_read waits for the
@@ -450,6 +537,9 @@ int lucid_cp_solve_bwd(int B, int H, int N, int D, float scale, int blk_lo, int 
 #define LUCID_KERNEL_PATH_ATTN 14     /* PaTH softmax attention forward */
 #define LUCID_KERNEL_DECODE 15        /* LUCID decode step (get_new_v_prime) */
 #define LUCID_KERNEL_FWD_FUSED 16     /* chain-schedule solve + attention forward in one launch */
+#define LUCID_KERNEL_PAGED_DECODE 17  /* paged decode step / attention (tile pass and join) */
+#define LUCID_KERNEL_PAGES 18         /* paged append, page copies */
+#define LUCID_KERNEL_LOGPROBS 19      /* token log probabilities, forward and backward */
 int lucid_profile_enable(int kernel);
 int lucid_profile_read(float* total_ms, int* launches);
 

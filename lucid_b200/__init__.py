@@ -21,5 +21,15 @@ from .ops import (  # noqa: F401
     solve_bwd,
     solve_fwd,
 )
+from ._lib import check_status  # noqa: F401
+from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401
+from .paged import (  # noqa: F401
+    PagedBatch,
+    PagedCache,
+    copy_pages,
+    paged_append,
+    paged_decode_attention,
+    paged_decode_step,
+)
 
 __version__ = "0.1.0"

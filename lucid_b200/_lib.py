@@ -15,7 +15,8 @@ LIB_PATH = os.path.join(_HERE, "liblucid_b200.so")
 LUCID_OK = 0
 KERNEL_IDS = {"prep": 1, "solve_fwd": 2, "attn_fwd": 3, "attn_bwd": 4, "solve_bwd": 5, "attn_bwd_row": 6,
               "solve_bwd_row": 7, "path_block": 8, "path_scores": 9, "path_solve": 10, "path_solve_t": 11,
-              "path_row": 12, "path_col": 13, "path_attn": 14, "decode": 15, "fwd_fused": 16}
+              "path_row": 12, "path_col": 13, "path_attn": 14, "decode": 15, "fwd_fused": 16,
+              "paged_decode": 17, "pages": 18, "logprobs": 19}
 ERRORS = {
     1: "unsupported shape (head_dim at most 128, Hq a multiple of Hkv)",
     2: "pointer or stride not 16-byte aligned",
@@ -30,6 +31,7 @@ c_int, c_float, c_size_t, c_void_p, c_int64 = (
 c_float_p = ctypes.POINTER(ctypes.c_float)
 
 S3 = [c_int64] * 3  # (sb, sh, sn) element strides
+S2 = [c_int64] * 2  # (sb, sh) element strides
 
 # name -> (restype, argtypes); every symbol declared in include/lucid_b200.h
 SIGNATURES = {
@@ -91,6 +93,20 @@ SIGNATURES = {
                           + [c_void_p] + [c_void_p] + S3 + [c_void_p] * 2 + [c_void_p] + S3 + [c_void_p] * 4),
     "lucid_cp_solve_bwd": (c_int, [c_int] * 4 + [c_float] + [c_int] * 4 + [c_void_p] + S3 + [c_void_p] * 11
                            + [c_void_p] + S3 + [c_void_p] + S3 + [c_void_p] * 2),
+    "lucid_paged_decode_workspace_bytes": (c_size_t, [c_int] * 5),
+    "lucid_paged_decode_step": (c_int, [c_int] * 7 + [c_float, c_float] + ([c_void_p] + S2) * 3 + ([c_void_p] + S3) * 2
+                                + [c_void_p, c_int64, c_void_p] + ([c_void_p] + S2) * 2 + [c_int, c_void_p]
+                                + [c_void_p, c_size_t, c_void_p]),
+    "lucid_paged_decode_attn": (c_int, [c_int] * 7 + [c_float] + [c_void_p] + S2 + ([c_void_p] + S3) * 2
+                                + [c_void_p, c_int64, c_void_p] + [c_void_p] + S2 + [c_void_p]
+                                + [c_void_p, c_size_t, c_void_p]),
+    "lucid_paged_append": (c_int, [c_int] * 7 + ([c_void_p] + S3) * 4 + [c_void_p, c_int64, c_void_p, c_void_p]
+                           + [c_void_p, c_void_p]),
+    "lucid_copy_pages": (c_int, [c_int, c_int, c_int64] + [c_void_p, c_int64, c_int64] * 2 + [c_void_p, c_void_p, c_int]
+                         + [c_void_p]),
+    "lucid_token_logprobs": (c_int, [c_int64, c_int64, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int]
+                             + [c_void_p] * 7),
+    "lucid_token_logprobs_bwd": (c_int, [c_int64, c_int64, c_int, c_int, c_void_p, c_int64, c_int64] + [c_void_p] * 7),
     "lucid_selftest_umma": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "lucid_profile_enable": (c_int, [c_int]),
     "lucid_profile_read": (c_int, [c_float_p, ctypes.POINTER(c_int)]),
@@ -136,13 +152,16 @@ def check(rc: int, what: str) -> None:
 #   code | barrier << 8 | kernel << 20
 # in the int32 status word at lucid_workspace_status_offset() of the call's workspace.
 STATUS_CODES = {1: "an mbarrier wait timed out", 2: "a cross-CTA dependency flag never arrived",
-                3: "the shared-memory window was not 1024-byte aligned"}
+                3: "the shared-memory window was not 1024-byte aligned",
+                4: "a page of the block table lies outside the pool",
+                5: "a length or a new row lies past the block table",
+                6: "a token lies outside the vocabulary"}
 KERNEL_TAGS = {1: "solve forward", 2: "attention forward", 3: "attention backward column pass",
                4: "transposed-solve column pass", 5: "attention backward row pass",
                6: "solve backward row pass", 7: "tensor-core self test", 8: "LUCID-Path block GEMM",
                9: "LUCID-Path score chain", 10: "LUCID-Path solve", 11: "LUCID-Path transposed solve",
                12: "LUCID-Path row pass", 13: "LUCID-Path column pass", 14: "PaTH attention",
-               15: "stored-tile row pass"}
+               15: "stored-tile row pass", 16: "paged decoding", 17: "paged append", 18: "token log probabilities"}
 
 
 def decode_status(word: int) -> str:
@@ -167,6 +186,7 @@ class _StatusWatch:
 
     def __init__(self):
         self.pending = []
+        self.words = {}   # device index -> (pinned int32 word, its ctypes view, its address)
         self.lock = threading.Lock()
         self.sync = os.environ.get("LUCID_B200_SYNC_STATUS", "0") not in ("", "0")
 
@@ -184,6 +204,29 @@ class _StatusWatch:
         if self.sync:
             self.wait_all()
 
+    def device_word(self, index: int) -> int:
+        """Address of a device's status word in mapped host memory, for kernels that write
+        it only on a failure: nothing is copied or queued on a call that goes well, and
+        a captured graph's replays report through it too."""
+        got = self.words.get(index)
+        if got is None:
+            import torch
+            with self.lock:
+                if index not in self.words:
+                    host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+                    self.words[index] = (host, ctypes.c_int32.from_address(host.data_ptr()), host.data_ptr())
+            got = self.words[index]
+        return got[2]
+
+    def _take_words(self):
+        bad = []
+        for index, (_, word, _) in list(self.words.items()):
+            if word.value:
+                bad.append((f"cuda:{index}", word.value))
+                word.value = 0
+        if bad:
+            raise LucidError("; ".join(f"{what}: {decode_status(w)}" for what, w in bad))
+
     def _take(self, block: bool):
         with self.lock:
             done, keep = [], []
@@ -199,9 +242,17 @@ class _StatusWatch:
     def poll(self) -> None:
         if self.pending:
             self._take(False)
+        for _, word, _ in self.words.values():
+            if word.value:
+                self._take_words()
 
     def wait_all(self) -> None:
+        if self.words:
+            import torch
+            for index in list(self.words):
+                torch.cuda.synchronize(index)
         self._take(True)
+        self._take_words()
 
 
 STATUS = _StatusWatch()

@@ -26,6 +26,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .layer import LucidAttention
+from .logprobs import TokenLogprobs, token_logprobs
+from .paged import PagedBatch
 
 __all__ = ["LUCID_CONFIG", "lucid_config", "LucidRMSNorm", "LucidMLP", "LucidDecoderLayer", "LucidForCausalLM"]
 
@@ -137,16 +139,64 @@ class LucidForCausalLM(nn.Module):
             sd[k[len("model."):] if k.startswith("model.") else k] = v
         return self.load_state_dict(sd, strict=strict)
 
-    def forward(self, input_ids, past_key_values=None, logits_to_keep: int = 0, attn_events=None):
+    def forward(self, input_ids, past_key_values=None, logits_to_keep: int = 0, attn_events=None,
+                prompt_lengths=None):
         """Logits of the last ``logits_to_keep`` positions (0: all).  With a
         transformers Cache, the prefill fills it (raw keys, solved values) as
         the reference does.  attn_events: optional per-layer pairs of CUDA
-        events recorded around each attention call."""
+        events recorded around each attention call.
+
+        With a PagedBatch, a call is the prefill of its (empty) sequences or one new token
+        of each.  ``prompt_lengths`` (one per sequence) are the prompts' lengths in a
+        right-padded prefill: only those rows enter the cache, and ``logits_to_keep=1``
+        takes each prompt's own last position."""
+        paged = isinstance(past_key_values, PagedBatch)
+        if prompt_lengths is not None:
+            prompt_lengths = [int(n) for n in prompt_lengths]
+            if not paged:
+                raise ValueError("prompt_lengths come with a PagedBatch")
+            if len(prompt_lengths) != input_ids.shape[0] or not all(1 <= n <= input_ids.shape[1] for n in prompt_lengths):
+                raise ValueError(f"prompt_lengths {prompt_lengths} do not fit ids of shape {tuple(input_ids.shape)}")
+            if logits_to_keep not in (0, 1):
+                raise ValueError("with prompt_lengths, logits_to_keep is 0 (all) or 1 (each prompt's last)")
+        if paged:
+            if len(past_key_values) != input_ids.shape[0]:
+                raise ValueError(f"{input_ids.shape[0]} rows of ids for {len(past_key_values)} cached sequences")
+            past_key_values.reserve(prompt_lengths if prompt_lengths is not None else input_ids.shape[1])
         x = self.embed_tokens(input_ids)
         for i, layer in enumerate(self.layers):
             x = layer(x, past_key_value=past_key_values,
                       attn_events=None if attn_events is None else attn_events[i])
+        if paged:
+            past_key_values.advance()
         x = self.norm(x)
-        if logits_to_keep:
+        if prompt_lengths is not None and logits_to_keep:
+            last = torch.tensor(prompt_lengths, device=x.device) - 1
+            x = x[torch.arange(x.shape[0], device=x.device), last][:, None]
+        elif logits_to_keep:
             x = x[:, -logits_to_keep:]
         return self.lm_head(x)
+
+    @torch.no_grad()
+    def score(self, input_ids, top: int = 0) -> TokenLogprobs:
+        """Log probabilities of input_ids[:, 1:] given the tokens before them, with each
+        position's entropy and ``top`` most likely tokens: [B, N - 1] and [B, N - 1, top]."""
+        if input_ids.shape[1] < 2:
+            raise ValueError("score needs at least two tokens")
+        return token_logprobs(self(input_ids)[:, :-1], input_ids[:, 1:], top=top)
+
+    @torch.no_grad()
+    def generate(self, input_ids, batch: PagedBatch, max_new_tokens: int, prompt_lengths=None, top: int = 0):
+        """Greedy decoding of empty cached sequences from (right-padded) prompts.  Returns
+        (tokens [B, max_new_tokens], TokenLogprobs of them); ``batch`` then caches the
+        prompts and all but the last new token, so it can be forked or continued."""
+        if max_new_tokens < 1:
+            raise ValueError("max_new_tokens must be positive")
+        logits = self(input_ids, batch, logits_to_keep=1, prompt_lengths=prompt_lengths)
+        tokens, said = [], []
+        while True:
+            tokens.append(logits.argmax(-1))
+            said.append(token_logprobs(logits, tokens[-1], top=top))
+            if len(tokens) == max_new_tokens:
+                return torch.cat(tokens, 1), TokenLogprobs(*(torch.cat(parts, 1) for parts in zip(*said)))
+            logits = self(tokens[-1], batch)

@@ -16,7 +16,9 @@ the cache keeps raw keys and solved values like the reference (:479-481).
 Where a single-pass kernel covers the step's shape (ops.decode_step_fused),
 ``LucidAttention.forward`` computes get_new_v_prime and the attention in one
 pass over the cache and then appends to it; the three methods above keep the
-reference's separate calls for code that calls or patches them.
+reference's separate calls for code that calls or patches them.  With a PagedBatch as the
+cache (paged.py), the prefill appends to its pages and every decoding step is one
+paged_decode_step, for any number of query heads per kv head.
 """
 from __future__ import annotations
 
@@ -25,6 +27,7 @@ from torch import nn
 
 from .ops import (LucidAttentionFunction, LucidAttnFunction, LucidSolveFunction, decode_attention, decode_step,
                   decode_step_fused, decode_update)
+from .paged import PagedBatch
 
 __all__ = ["LucidAttention", "patch_reference", "get_v_prime", "get_new_v_prime", "eager_lucid_attention_forward"]
 
@@ -133,7 +136,9 @@ class LucidAttention(nn.Module):
         q = self.q_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         k = self.k_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         v = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
-        if past_key_value is None or self.training:
+        if isinstance(past_key_value, PagedBatch):
+            o = self._paged_forward(q, k, v, past_key_value)
+        elif past_key_value is None or self.training:
             o = LucidAttentionFunction.apply(q, k, v, float(self.scaling), float(self.k_norm.eps or 1e-5))
         else:
             past = past_key_value.get_seq_length(self.layer_idx)
@@ -152,6 +157,22 @@ class LucidAttention(nn.Module):
                 o, _ = self.eager_lucid_attention_forward(q, k_all, x_all, self.scaling, None)
         o = o.reshape(*input_shape, -1).contiguous()
         return self.o_proj(o), None
+
+    def _paged_forward(self, q, k, v, batch: PagedBatch):
+        """Attention against a paged cache whose next tokens are reserved: the prefill of
+        sequences that are all empty (rows past a prompt's length come last and are
+        ignored by causality), or one new token of sequences that are all begun."""
+        if self.training:
+            raise RuntimeError("a paged cache is for inference: call eval() first")
+        begun = [n > 0 for n in batch.host_lengths]
+        if not any(begun):
+            x = self.get_v_prime(k, v, self.scaling, None)
+            batch.append(self.layer_idx, k, x)
+            return self.eager_lucid_attention_forward(q, k, x, self.scaling, None)[0]
+        if not all(begun) or q.shape[2] != 1:
+            raise NotImplementedError("a paged cache takes the prefill of empty sequences or one new token of begun "
+                                      f"ones; got {q.shape[2]} tokens for lengths {batch.host_lengths}")
+        return batch.step(self.layer_idx, q, k, v, float(self.scaling), _k_norm_eps(self))[0]
 
 
 def patch_reference(module) -> None:

@@ -1,0 +1,470 @@
+"""Paged cache of raw keys and solved values, and the operators that read and move it.
+
+  paged_decode_step       one new token per sequence: get_new_v_prime (modeling_lucid.py:576-598),
+                          the attention over the cache and the new token (:505-549), the append
+  paged_decode_attention  the attention alone, over the cached tokens
+  paged_append            rows of new keys / solved values into the sequences' pages
+  copy_pages              whole pages copied in every layer
+  PagedCache, PagedBatch  the bookkeeping: sequences, forking, freeing, compacting
+
+A pool is [P, Hkv, page_size, D] bf16 (any strides with a unit innermost one); the block
+table [B, M] int32 names the pages of each sequence in order and ``lengths`` [B] int32 the
+tokens cached so far; both live on the pool's device.  A negative length marks an unused
+place of the batch: zeros come out and nothing is written.  Only the rows below a
+sequence's length are ever read, so pages need no clearing.  What only the device can
+see (a page outside the pool, a length past the block table) is not followed but
+reported: the next call of this package or ``check_status()`` raises LucidError.
+
+These operators are inference only; their outputs carry no gradient.  They can be captured
+into CUDA graphs; the workspace of a captured call belongs to its graph.
+"""
+from __future__ import annotations
+
+import array
+import contextlib
+import heapq
+
+import torch
+
+from . import _lib
+from ._lib import LucidError
+
+__all__ = ["paged_decode_step", "paged_decode_attention", "paged_append", "copy_pages", "PagedCache", "PagedBatch"]
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Context in which ``device`` is the current one."""
+    return _NO_GUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _rows(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
+    """A bf16 CUDA operand of the given shape, copied if its rows are not 8-byte aligned."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name}: LUCID B200 kernels need CUDA tensors (no CPU fallback)")
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: expected bfloat16, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the pool on {device}")
+    s = t.stride()
+    ok = s[3] == 1 and (s[0] | s[1] | s[2]) % 4 == 0 and t.data_ptr() % 8 == 0
+    return t if ok else t.clone(memory_format=torch.contiguous_format)  # contiguous() keeps an odd start
+
+
+def _pools(key_pages: torch.Tensor, x_pages: torch.Tensor, dims: int = 4):
+    """The pools as they are: never copied, so what the kernels cannot address is refused."""
+    for t, name in ((key_pages, "key_pages"), (x_pages, "x_pages")):
+        if not t.is_cuda:
+            raise RuntimeError(f"{name}: LUCID B200 kernels need CUDA tensors (no CPU fallback)")
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name}: expected bfloat16, got {t.dtype}")
+        if t.dim() != dims:
+            raise ValueError(f"{name}: expected a {dims}-D pool, got shape {tuple(t.shape)}")
+        s = t.stride()
+        if s[-1] != 1 or t.data_ptr() % 8 or any(st % 4 or st == 0 and n > 1 for st, n in zip(s[:-1], t.shape[:-1])):
+            raise ValueError(f"{name}: needs a unit innermost stride, the others nonzero multiples of 4 elements, "
+                             f"and an 8-byte aligned base; got strides {s}")
+    if x_pages.shape != key_pages.shape or x_pages.device != key_pages.device:
+        raise ValueError(f"key_pages {tuple(key_pages.shape)} on {key_pages.device} and x_pages "
+                         f"{tuple(x_pages.shape)} on {x_pages.device} must match")
+
+
+def _index(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name}: expected int32, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the pool on {device}")
+    if t.dim() != len(shape) or any(want is not None and n != want for n, want in zip(t.shape, shape)):
+        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: needs a unit innermost stride")
+    return t
+
+
+def _table(block_table, lengths, B, device):
+    _index(block_table, "block_table", (B, None), device)
+    _index(lengths, "lengths", (B,), device)
+    return block_table.data_ptr(), block_table.stride(0), lengths.data_ptr()
+
+
+def paged_decode_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
+                      x_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scale: float,
+                      eps: float = 1e-5, append: bool = True):
+    """One decoding step of LucidAttention.forward (modeling_lucid.py:467-481, then :505-549)
+    for one new token per sequence, in one pass over the paged cache, for any number of
+    query heads per kv head.  query [B,Hq,1,D], key / value [B,Hkv,1,D], D a multiple of 4
+    up to 128.  ``lengths`` counts the tokens before the step.  With ``append`` the new key
+    and its solved value are also written into row lengths[b] of sequence b, whose page the
+    caller has assigned (and shares with no other sequence); ``lengths`` stays as it is.
+    Returns (O [B,1,Hq,D], x_new [B,Hkv,1,D])."""
+    lib = _lib.load()
+    _lib.STATUS.poll()
+    _pools(key_pages, x_pages)
+    P, Hkv, ps, D = key_pages.shape
+    dev = key_pages.device
+    if query.dim() != 4 or query.shape[2] != 1:
+        raise ValueError(f"query: expected [B, Hq, 1, D] (one new token), got {tuple(query.shape)}")
+    B, Hq = query.shape[0], query.shape[1]
+    query = _rows(query, "query", (B, Hq, 1, D), dev)
+    key = _rows(key, "key", (B, Hkv, 1, D), dev)
+    value = _rows(value, "value", (B, Hkv, 1, D), dev)
+    tab, t_sb, lens = _table(block_table, lengths, B, dev)
+    with _on(dev):
+        x_new = torch.empty(B, Hkv, 1, D, dtype=torch.bfloat16, device=dev)
+        o = torch.empty(B, 1, Hq, D, dtype=torch.bfloat16, device=dev)
+        ws = torch.empty(lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 1), dtype=torch.uint8, device=dev)
+        rc = lib.lucid_paged_decode_step(
+            B, Hq, Hkv, D, P, ps, block_table.shape[1], scale, eps, query.data_ptr(), query.stride(0), query.stride(1),
+            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
+            key_pages.data_ptr(), *key_pages.stride()[:3], x_pages.data_ptr(), *x_pages.stride()[:3], tab, t_sb, lens,
+            x_new.data_ptr(), Hkv * D, D, o.data_ptr(), Hq * D, D, 1 if append else 0,
+            _lib.STATUS.device_word(dev.index), ws.data_ptr(), ws.numel(), _stream())
+    _lib.check(rc, "lucid_paged_decode_step")
+    return o, x_new
+
+
+def paged_decode_attention(query: torch.Tensor, key_pages: torch.Tensor, x_pages: torch.Tensor,
+                           block_table: torch.Tensor, lengths: torch.Tensor, scale: float) -> torch.Tensor:
+    """softmax(s q K^T) X of one new query per sequence over its ``lengths`` cached tokens
+    (eager_lucid_attention_forward during decoding, the new token's row already in the
+    cache).  query [B,Hq,1,D]; a sequence without tokens gives zeros.  Returns O [B,1,Hq,D]."""
+    lib = _lib.load()
+    _lib.STATUS.poll()
+    _pools(key_pages, x_pages)
+    P, Hkv, ps, D = key_pages.shape
+    dev = key_pages.device
+    if query.dim() != 4 or query.shape[2] != 1:
+        raise ValueError(f"query: expected [B, Hq, 1, D] (one new token), got {tuple(query.shape)}")
+    B, Hq = query.shape[0], query.shape[1]
+    query = _rows(query, "query", (B, Hq, 1, D), dev)
+    tab, t_sb, lens = _table(block_table, lengths, B, dev)
+    with _on(dev):
+        o = torch.empty(B, 1, Hq, D, dtype=torch.bfloat16, device=dev)
+        ws = torch.empty(lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 0), dtype=torch.uint8, device=dev)
+        rc = lib.lucid_paged_decode_attn(
+            B, Hq, Hkv, D, P, ps, block_table.shape[1], scale, query.data_ptr(), query.stride(0), query.stride(1),
+            key_pages.data_ptr(), *key_pages.stride()[:3], x_pages.data_ptr(), *x_pages.stride()[:3], tab, t_sb, lens,
+            o.data_ptr(), Hq * D, D, _lib.STATUS.device_word(dev.index), ws.data_ptr(), ws.numel(), _stream())
+    _lib.check(rc, "lucid_paged_decode_attn")
+    return o
+
+
+def paged_append(key: torch.Tensor, x: torch.Tensor, key_pages: torch.Tensor, x_pages: torch.Tensor,
+                 block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None = None) -> None:
+    """Writes rows i < counts[b] (None: all N) of key and x [B,Hkv,N,D] into the rows
+    lengths[b] + i of sequence b's pages, in place; rows past the counts (a padded batch)
+    are not touched, nor are ``lengths``.  The caller has assigned the pages, and no two
+    sequences of the call write the same one."""
+    lib = _lib.load()
+    _lib.STATUS.poll()
+    _pools(key_pages, x_pages)
+    P, Hkv, ps, D = key_pages.shape
+    dev = key_pages.device
+    if key.dim() != 4:
+        raise ValueError(f"key: expected [B, Hkv, N, D], got {tuple(key.shape)}")
+    B, N = key.shape[0], key.shape[2]
+    key = _rows(key.detach(), "key", (B, Hkv, N, D), dev)
+    x = _rows(x.detach(), "x", (B, Hkv, N, D), dev)
+    tab, t_sb, lens = _table(block_table, lengths, B, dev)
+    if counts is not None:
+        _index(counts, "counts", (B,), dev)
+    with _on(dev):
+        rc = lib.lucid_paged_append(
+            B, Hkv, N, D, P, ps, block_table.shape[1], key.data_ptr(), *key.stride()[:3], x.data_ptr(), *x.stride()[:3],
+            key_pages.data_ptr(), *key_pages.stride()[:3], x_pages.data_ptr(), *x_pages.stride()[:3], tab, t_sb, lens,
+            None if counts is None else counts.data_ptr(), _lib.STATUS.device_word(dev.index), _stream())
+    _lib.check(rc, "lucid_paged_append")
+
+
+def _ids(v, name: str) -> array.array:
+    """Page numbers as a C int array; sequences of ints or a CPU tensor."""
+    if isinstance(v, torch.Tensor):
+        if v.is_cuda or v.dim() != 1 or v.is_floating_point() or v.is_complex() or v.dtype == torch.bool:
+            raise TypeError(f"{name}: expected a 1-D integer CPU tensor or a sequence of page numbers")
+        v = v.tolist()
+    try:
+        return array.array("i", v)
+    except (TypeError, OverflowError) as e:
+        raise TypeError(f"{name}: expected page numbers ({e})") from None
+
+
+def copy_pages(key_pages: torch.Tensor, x_pages: torch.Tensor, src, dst) -> None:
+    """Page dst[i] becomes a copy of page src[i], in place, in both pools: [P,Hkv,ps,D], or
+    [layers,P,Hkv,ps,D] for all layers at once.  src and dst are host sequences (or CPU
+    tensors) of page numbers; each dst is named once and is no src, so the order of the
+    copies is free.  A page's [Hkv,ps,D] block must be dense."""
+    lib = _lib.load()
+    _lib.STATUS.poll()
+    _pools(key_pages, x_pages, 5 if key_pages.dim() == 5 else 4)
+    shape = key_pages.shape
+    layers, P = (shape[0], shape[1]) if len(shape) == 5 else (1, shape[0])
+    src, dst = _ids(src, "src"), _ids(dst, "dst")
+    if len(src) != len(dst):
+        raise ValueError(f"src names {len(src)} pages, dst {len(dst)}")
+    n = shape[-3] * shape[-2] * shape[-1]
+    strides = []
+    for t, name in ((key_pages, "key_pages"), (x_pages, "x_pages")):
+        s = t.stride()
+        inner = sorted((st, size) for st, size in zip(s[-3:], shape[-3:]) if size > 1)
+        span = 1
+        for st, size in inner:
+            if st != span:
+                raise ValueError(f"{name}: the pages' [Hkv, page_size, D] blocks must be dense, got strides {s}")
+            span *= size
+        strides.append((2 * s[0] if len(shape) == 5 else 0, 2 * s[-4]))
+    if len(src) == 0 or layers == 0 or n == 0:
+        return
+    if n % 4:
+        raise ValueError(f"a page of {n} elements is not a multiple of 8 bytes")
+    with _on(key_pages.device):
+        rc = lib.lucid_copy_pages(layers, P, 2 * n, key_pages.data_ptr(), *strides[0], x_pages.data_ptr(), *strides[1],
+                                  src.buffer_info()[0], dst.buffer_info()[0], len(src), _stream())
+    if rc == 1:
+        raise ValueError(f"copy_pages: pages must lie in [0, {P}), each dst named once and none of them a src")
+    _lib.check(rc, "lucid_copy_pages")
+
+
+class _Sequence:
+    __slots__ = ("pages", "length")
+
+    def __init__(self):
+        self.pages: list[int] = []
+        self.length = 0
+
+
+class PagedCache:
+    """Key / solved-value cache of every layer in pages of ``page_size`` tokens, shared by
+    any number of sequences: ``key_pages`` / ``x_pages`` are [layers, P, Hkv, page_size, D]
+    and page p holds the same tokens in every layer.  The page lists live on the host, so
+    running out of pages is an exception before anything changes; copies are queued on
+    the current stream.
+
+        cache = PagedCache(layers, kv_heads, head_dim, num_pages=4096)
+        batch = cache.batch(cache.new(8))
+        logits = model(ids, past_key_values=batch, prompt_lengths=lens)     # prefill
+        logits = model(next_ids, past_key_values=batch)                     # one token each
+        other = cache.fork(batch.sequences[0]); cache.free(batch.sequences[1]); cache.compact()
+    """
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int, page_size: int = 64,
+                 device="cuda"):
+        if min(num_layers, num_kv_heads, num_pages, page_size) < 1 or not 4 <= head_dim <= 128 or head_dim % 4:
+            raise ValueError("PagedCache: sizes must be positive and head_dim a multiple of 4 up to 128")
+        self.page_size = page_size
+        shape = (num_layers, num_pages, num_kv_heads, page_size, head_dim)
+        self.key_pages = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        self.x_pages = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        self._refs = [0] * num_pages
+        self._free = list(range(num_pages))   # a heap: the lowest page first
+        self._sequences: dict[int, _Sequence] = {}
+        self._next = 0
+        self._version = 0                     # grows when page lists change under a batch
+
+    @classmethod
+    def for_config(cls, config, num_pages: int, page_size: int = 64, device="cuda") -> "PagedCache":
+        """A cache for a decoder configuration (decoder.lucid_config)."""
+        head_dim = getattr(config, "head_dim", None) or config.hidden_size // config.num_attention_heads
+        return cls(config.num_hidden_layers, config.num_key_value_heads, head_dim, num_pages, page_size, device)
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def new(self, count: int = 1) -> list[int]:
+        """``count`` empty sequences; a sequence is known by its number."""
+        made = list(range(self._next, self._next + count))
+        self._next += count
+        for i in made:
+            self._sequences[i] = _Sequence()
+        return made
+
+    def _get(self, sequence: int) -> _Sequence:
+        try:
+            return self._sequences[sequence]
+        except KeyError:
+            raise LucidError(f"sequence {sequence} is not in the cache") from None
+
+    def length(self, sequence: int) -> int:
+        return self._get(sequence).length
+
+    def pages(self, sequence: int) -> list[int]:
+        """The pages of the sequence's tokens, in order."""
+        s = self._get(sequence)
+        return s.pages[:-(-s.length // self.page_size)]
+
+    def _drop(self, pages) -> None:
+        for p in pages:
+            self._refs[p] -= 1
+            if self._refs[p] == 0:
+                heapq.heappush(self._free, p)
+
+    def _take(self) -> int:
+        p = heapq.heappop(self._free)
+        self._refs[p] = 1
+        return p
+
+    def fork(self, sequence: int) -> int:
+        """A new sequence with the same tokens, sharing the pages; a shared page that one of
+        them goes on to fill is copied first (``PagedBatch.reserve``)."""
+        pages = self.pages(sequence)
+        child, = self.new()
+        self._sequences[child].pages = pages
+        self._sequences[child].length = self._sequences[sequence].length
+        for p in pages:
+            self._refs[p] += 1
+        self._version += 1
+        return child
+
+    def free(self, sequence: int) -> None:
+        """Ends a sequence; pages that no other one shares become free."""
+        self._drop(self._get(sequence).pages)
+        del self._sequences[sequence]
+        self._version += 1
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of the pool (every page at or past the number
+        in use goes to a free one before it) and returns how many moved."""
+        used = len(self._refs) - len(self._free)
+        src = [p for p in range(used, len(self._refs)) if self._refs[p]]
+        dst = [p for p in range(used) if not self._refs[p]]
+        if not src:
+            return 0
+        copy_pages(self.key_pages, self.x_pages, src, dst)
+        to = dict(zip(src, dst))
+        for s in self._sequences.values():
+            s.pages = [to.get(p, p) for p in s.pages]
+        for a, b in to.items():
+            self._refs[b], self._refs[a] = self._refs[a], 0
+        self._free = list(range(used, len(self._refs)))
+        self._version += 1
+        return len(src)
+
+    def batch(self, sequences) -> "PagedBatch":
+        return PagedBatch(self, sequences)
+
+
+class PagedBatch:
+    """Sequences of a PagedCache that run together: the model's ``past_key_values``.
+
+    One model step is ``reserve(counts)``, then ``append`` or ``step`` in every layer, then
+    ``advance()``; LucidForCausalLM.forward does all three.  ``block_table``, ``lengths``
+    and ``counts`` are the device tensors the operators read."""
+
+    def __init__(self, cache: PagedCache, sequences):
+        self.cache = cache
+        self.sequences = list(sequences)
+        if not self.sequences or len(set(self.sequences)) != len(self.sequences):
+            raise ValueError("a batch is one or more different sequences")
+        for s in self.sequences:
+            cache._get(s)
+        self._counts: list[int] | None = None   # reserved and not advanced yet
+        self._version = -1
+        self._on_device: list[list[int]] = []
+        self._host_lengths: list[int] = []
+        self._host_counts: list[int] = []
+        self.block_table = self.lengths = self.counts = None
+
+    def __len__(self) -> int:
+        return len(self.sequences)
+
+    @property
+    def host_lengths(self) -> list[int]:
+        return [self.cache.length(s) for s in self.sequences]
+
+    def get_seq_length(self, layer_idx: int = 0) -> int:
+        """The longest sequence's cached tokens."""
+        return max(self.host_lengths)
+
+    def reserve(self, counts) -> None:
+        """Assigns the pages for ``counts`` more tokens of each sequence (one number for
+        all, or one each) and copies shared pages that would be written.  Raises LucidError,
+        with nothing changed, when the pool has too few free pages."""
+        if torch.cuda.is_current_stream_capturing():
+            raise LucidError("PagedBatch.reserve works on the host: call it before the capture")
+        c = self.cache
+        seqs = [c._get(s) for s in self.sequences]
+        counts = [counts] * len(seqs) if isinstance(counts, int) else [int(n) for n in counts]
+        if len(counts) != len(seqs) or min(counts) < 0:
+            raise ValueError(f"reserve: {len(seqs)} sequences need as many counts, none negative; got {counts}")
+        ps, dropped, shared, need = c.page_size, {}, [], 0
+        for s, n in zip(seqs, counts):
+            if n and s.length % ps:
+                p = s.pages[s.length // ps]
+                if c._refs[p] - dropped.get(p, 0) > 1:
+                    dropped[p] = dropped.get(p, 0) + 1
+                    shared.append(s)
+                    need += 1
+            need += max(0, -(-(s.length + n) // ps) - len(s.pages))
+        if need > len(c._free):
+            raise LucidError(f"the paged cache is full: {need} pages needed, {len(c._free)} of {len(c._refs)} free")
+        src, dst = [], []
+        for s in shared:
+            at = s.length // ps
+            src.append(s.pages[at])
+            dst.append(c._take())
+            c._refs[src[-1]] -= 1
+            s.pages = s.pages[:at] + [dst[-1]] + s.pages[at + 1:]
+        for s, n in zip(seqs, counts):
+            while len(s.pages) * ps < s.length + n:
+                s.pages.append(c._take())
+        if src:
+            copy_pages(c.key_pages, c.x_pages, src, dst)
+        self._counts, self._version = counts, c._version
+        self._upload(seqs, counts)
+
+    def _upload(self, seqs, counts) -> None:
+        """Brings the device tensors up to date, touching those that changed."""
+        dev = self.cache.key_pages.device
+        pages = [list(s.pages) for s in seqs]
+        if pages != self._on_device or self.block_table is None:
+            width = max(1, max(map(len, pages)))
+            table = torch.full((len(pages), width), -1, dtype=torch.int32)
+            for i, row in enumerate(pages):
+                table[i, :len(row)] = torch.tensor(row, dtype=torch.int32)
+            self.block_table, self._on_device = table.to(dev), pages
+        lengths = [s.length for s in seqs]
+        if lengths != self._host_lengths or self.lengths is None:
+            self.lengths = torch.tensor(lengths, dtype=torch.int32).to(dev)
+            self._host_lengths = lengths
+        if counts != self._host_counts or self.counts is None:
+            self.counts = torch.tensor(counts, dtype=torch.int32).to(dev)
+            self._host_counts = counts
+
+    def _check(self) -> None:
+        if self._counts is None:
+            raise LucidError("reserve() the step's tokens first")
+        if self._version != self.cache._version:
+            raise LucidError("the cache's pages changed since reserve(): reserve again")
+
+    def append(self, layer: int, key: torch.Tensor, x: torch.Tensor) -> None:
+        """The reserved tokens' rows of one layer, key / x [B,Hkv,N,D] with N at least the
+        largest count; rows past a sequence's count are padding."""
+        self._check()
+        if key.shape[2] < max(self._counts):
+            raise ValueError(f"append: {max(self._counts)} tokens were reserved, {key.shape[2]} rows given")
+        paged_append(key, x, self.cache.key_pages[layer], self.cache.x_pages[layer], self.block_table, self.lengths,
+                     self.counts)
+
+    def step(self, layer: int, query, key, value, scale: float, eps: float = 1e-5):
+        """paged_decode_step of one layer, appending; one token of every sequence reserved."""
+        self._check()
+        if any(n != 1 for n in self._counts):
+            raise ValueError("step: reserve one token of every sequence")
+        return paged_decode_step(query, key, value, self.cache.key_pages[layer], self.cache.x_pages[layer],
+                                 self.block_table, self.lengths, scale, eps)
+
+    def advance(self) -> None:
+        """Counts the reserved tokens as cached."""
+        self._check()
+        for s, n in zip(self.sequences, self._counts):
+            self.cache._sequences[s].length += n
+        self.lengths = self.lengths + self.counts
+        self._host_lengths = [a + n for a, n in zip(self._host_lengths, self._counts)]
+        self._counts = None
