@@ -28,6 +28,7 @@ namespace lb {
 
 constexpr int kPdWarps = 4, kPdThreads = 32 * kPdWarps;
 constexpr int kPdTile = 16 * kPdWarps;  // tokens per tile, 16 per warp
+constexpr int kPdStages = 3;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -44,6 +45,25 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ float2 unpack_bf16(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
+
+// 2^v; results below 2^-126 flush to zero, which nothing here can tell from a weight of 0
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// CB bytes from global to shared memory, the bytes at and past `bytes` zero and unread
+template <int CB>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int bytes) {
+  if constexpr (CB == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // cached tokens of sequence b; negative lengths mark unused places of the batch
 __device__ __forceinline__ int pd_len(const PagedDecodeArgs& a, int b) {
@@ -114,6 +134,27 @@ __device__ __forceinline__ void pd_next_item(const PagedDecodeArgs& a, PdCursor&
   }
 }
 
+template <int KR>
+__device__ __forceinline__ void load_chunk(const unsigned char* p, uint32_t (&r)[KR]) {
+  if constexpr (KR == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    r[0] = v.x; r[1] = v.y;
+  }
+}
+
+// bytes of one stage of one warp: 16 tokens' chunks of both pools
+template <int CE, int NK, int NX>
+constexpr int pd_stage_bytes() { return 32 * (2 * NK + 4 * NX) * CE * 2; }
+
+// The rows stream through a ring of kPdStages stages per warp, filled by cp.async two
+// tiles ahead across item borders.  Each lane copies exactly the chunks that it later
+// multiplies, so a stage needs no barrier, only the lane's own wait; one copy instruction
+// of the warp covers 64 (keys) or 128 (values) contiguous bytes of each of its rows.  Page
+// numbers are looked up one tile before their copies are issued.
+//
 // STEP: an update row behind the query rows.  R8: at most 8 rows, so rows 8-15 of the
 // P operand carry the low halves of P and one mma does both.  A row's elements are cut
 // into chunks of CE (16 bytes where every row is 16-byte aligned, else 8): lane j of a
@@ -125,15 +166,74 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
   constexpr int NT = NX * CE;      // 8-column output tiles
   constexpr int KR = CE / 2;       // 32-bit registers per chunk
   constexpr int KS = NK * CE / 4;  // 16-element k steps
-  __shared__ float red[2][16][132];  // a warp pair's accumulator rows
+  constexpr int CB = CE * 2, STAGE = pd_stage_bytes<CE, NK, NX>();
+  extern __shared__ __align__(16) unsigned char ring[];  // [warp][stage][chunk][lane][CB]
+  __shared__ float red[2][R8 ? 8 : 16][132];  // a warp pair's accumulator rows
   __shared__ float red_ml[kPdWarps][16][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const long long T = pd_total(a, lane);
   const long long G = pd_ctas(a, T);
   if (blockIdx.x >= G) return;
   const long long t0 = blockIdx.x * T / G, t1 = (blockIdx.x + 1) * T / G;
   PdCursor c = pd_seek(a, t0, lane);
   const float c1 = a.s * kLog2e, c2 = kLog2e / a.s, inv_d = 1.f / (float)a.D;
+  const unsigned char* own = ring + warp * (kPdStages * STAGE) + lane * CB;
+  const uint32_t own_s = (uint32_t)__cvta_generic_to_shared(own);
+
+  // ---- the producer's side: cursor `pc` runs ahead of `c` ----
+  PdCursor pc = c;
+  long long pt = t0;             // tile whose page numbers are in (page, row)
+  int page = -1, row = 0, ph = 0;
+  auto look_up = [&]() {         // token 16 warp + (lane & 15) of tile pt
+    const int tok = pc.tile * kPdTile + 16 * warp + (lane & 15);
+    page = -1;
+    ph = pc.hb / a.nblk;
+    if (pt < t1 && tok < pc.n) {
+      const int pi = tok / a.ps;
+      row = tok - pi * a.ps;
+      page = a.table[(long long)pc.b * a.t_sb + pi];
+    }
+  };
+  auto issue = [&](int st) {     // copies of tile pt, then the look-up of the next
+    if (pt < t1) {
+      if (page >= a.P || (page < 0 && pc.tile * kPdTile + 16 * warp + (lane & 15) < pc.n)) {
+        report(a.status, kStatusPage, kTagPagedDecode);
+        page = -1;
+      }
+      const bf16* kh = a.k.p + (long long)ph * a.k.sh;
+      const bf16* xh = a.x.p + (long long)ph * a.x.sh;
+      const uint32_t dst = own_s + st * STAGE;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const int pg = __shfl_sync(0xffffffffu, page, g + 8 * kt), rw = __shfl_sync(0xffffffffu, row, g + 8 * kt);
+        const bf16* p = kh + (long long)max(pg, 0) * a.k.sp + (long long)rw * a.k.sn + j * CE;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          const int bytes = pg >= 0 ? max(0, min(CB, (a.D - (4 * i + j) * CE) * 2)) : 0;
+          copy_async<CB>(dst + (kt * NK + i) * 32 * CB, bytes ? p + 4 * i * CE : a.k.p, bytes);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int kq = 8 * (q >> 1) + 2 * j + (q & 1);
+        const int pg = __shfl_sync(0xffffffffu, page, kq), rw = __shfl_sync(0xffffffffu, row, kq);
+        const bf16* p = xh + (long long)max(pg, 0) * a.x.sp + (long long)rw * a.x.sn + g * CE;
+#pragma unroll
+        for (int cx = 0; cx < NX; ++cx) {
+          const int bytes = pg >= 0 ? max(0, min(CB, (a.D - (8 * cx + g) * CE) * 2)) : 0;
+          copy_async<CB>(dst + (2 * NK + cx * 4 + q) * 32 * CB, bytes ? p + 8 * cx * CE : a.x.p, bytes);
+        }
+      }
+      if (++pt < t1 && ++pc.tile == pc.nt) pd_next_item(a, pc);
+      look_up();
+    }
+    copy_commit();
+  };
+  look_up();
+#pragma unroll
+  for (int s = 0; s < kPdStages - 1; ++s) issue(s);
+  int st = 0;                    // stage of the consumer's tile
 
   for (long long t = t0; t < t1;) {
     // ---- one segment: the run's tiles of one item ----
@@ -148,16 +248,16 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
 #pragma unroll
     for (int hf = 0; hf < (R8 ? 1 : 2); ++hf) {
       const int r = g + 8 * hf;
-      const bf16* row = nullptr;
-      if (r < nq) row = a.q + (long long)c.b * a.q_sb + (long long)(h * a.gq + r_first + r) * a.q_sh;
-      else if (r == upd) row = a.kn + (long long)c.b * a.kn_sb + (long long)h * a.kn_sh;
+      const bf16* row_q = nullptr;
+      if (r < nq) row_q = a.q + (long long)c.b * a.q_sb + (long long)(h * a.gq + r_first + r) * a.q_sh;
+      else if (r == upd) row_q = a.kn + (long long)c.b * a.kn_sb + (long long)h * a.kn_sh;
 #pragma unroll
       for (int i = 0; i < NK; ++i)
 #pragma unroll
         for (int u = 0; u < CE / 4; ++u) {
           const int e = (4 * i + j) * CE + 4 * u;
           uint2 v = make_uint2(0u, 0u);
-          if (row != nullptr && e < a.D) v = *reinterpret_cast<const uint2*>(row + e);
+          if (row_q != nullptr && e < a.D) v = *reinterpret_cast<const uint2*>(row_q + e);
           qa[i * (CE / 4) + u][hf] = v.x;
           qa[i * (CE / 4) + u][(R8 ? 1 : 2) + hf] = v.y;
           if (STEP && r == upd) {
@@ -181,39 +281,19 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
     m[0] = STEP && g == upd ? 0.f : -INFINITY;
     m[1] = STEP && g + 8 == upd ? 0.f : -INFINITY;
 
-    const bf16* kh = a.k.p + (long long)h * a.k.sh;
-    const bf16* xh = a.x.p + (long long)h * a.x.sh;
     for (int it = 0; it < tiles; ++it) {
+      issue(st == 0 ? kPdStages - 1 : st - 1);
+      copy_wait<kPdStages - 1>();            // this lane's copies of tile t + it have landed
+      const unsigned char* in = own + st * STAGE;
+      st = st + 1 == kPdStages ? 0 : st + 1;
       const int base = (c.tile + it) * kPdTile + 16 * warp;
       if (base >= c.n) continue;             // uniform in the warp
-      // page and row of token base + (lane & 15)
-      const int tok = base + (lane & 15);
-      int page = -1, row = 0;
-      if (tok < c.n) {
-        page = a.table[(long long)c.b * a.t_sb + tok / a.ps];
-        row = tok % a.ps;
-        if (page < 0 || page >= a.P) {
-          report(a.status, kStatusPage, kTagPagedDecode);
-          page = -1;
-        }
-      }
       // keys: operand B of both 8-key tiles
       uint32_t kr[2][NK][KR];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        const int pg = __shfl_sync(0xffffffffu, page, g + 8 * kt), rw = __shfl_sync(0xffffffffu, row, g + 8 * kt);
-        const bf16* p = kh + (long long)max(pg, 0) * a.k.sp + (long long)rw * a.k.sn;
+      for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
-#pragma unroll
-          for (int u = 0; u < CE / 4; ++u) {
-            const int e = (4 * i + j) * CE + 4 * u;
-            uint2 v = make_uint2(0u, 0u);
-            if (pg >= 0 && e < a.D) v = *reinterpret_cast<const uint2*>(p + e);
-            kr[kt][i][2 * u] = v.x;
-            kr[kt][i][2 * u + 1] = v.y;
-          }
-      }
+        for (int i = 0; i < NK; ++i) load_chunk<KR>(in + (kt * NK + i) * 32 * CB, kr[kt][i]);
       float S[2][4] = {};
       float dg[2][4] = {};
 #pragma unroll
@@ -258,10 +338,10 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float mn = is_upd ? 0.f : fmaxf(m[hf], mx);
         const float ms = mn == -INFINITY ? 0.f : mn;
-        al[hf] = exp2f(m[hf] - ms);          // 0 while nothing has been seen
+        al[hf] = ex2(m[hf] - ms);            // 0 while nothing has been seen
         float p[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) p[q] = exp2f(z[q] - ms);
+        for (int q = 0; q < 4; ++q) p[q] = ex2(z[q] - ms);
         l[hf] = l[hf] * al[hf] + ((p[0] + p[1]) + (p[2] + p[3]));
         m[hf] = mn;
         phi[2 * hf] = pack_bf16(p[0], p[1]);
@@ -285,19 +365,7 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
       for (int cx = 0; cx < NX; ++cx) {
         uint32_t xr[4][KR];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int kq = 8 * (q >> 1) + 2 * j + (q & 1);
-          const int pg = __shfl_sync(0xffffffffu, page, kq), rw = __shfl_sync(0xffffffffu, row, kq);
-          const bf16* p = xh + (long long)max(pg, 0) * a.x.sp + (long long)rw * a.x.sn;
-#pragma unroll
-          for (int u = 0; u < CE / 4; ++u) {
-            const int e = (8 * cx + g) * CE + 4 * u;
-            uint2 v = make_uint2(0u, 0u);
-            if (pg >= 0 && e < a.D) v = *reinterpret_cast<const uint2*>(p + e);
-            xr[q][2 * u] = v.x;
-            xr[q][2 * u + 1] = v.y;
-          }
-        }
+        for (int q = 0; q < 4; ++q) load_chunk<KR>(in + (2 * NK + cx * 4 + q) * 32 * CB, xr[q]);
 #pragma unroll
         for (int e = 0; e < CE; ++e) {
           const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
@@ -344,8 +412,8 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
       const float Ms = M[hf] == -INFINITY ? 0.f : M[hf];
       L[hf] = 0.f;
 #pragma unroll
-      for (int w = 0; w < kPdWarps; ++w) L[hf] += exp2f(red_ml[w][g + 8 * hf][0] - Ms) * red_ml[w][g + 8 * hf][1];
-      f[hf] = exp2f(m[hf] - Ms);
+      for (int w = 0; w < kPdWarps; ++w) L[hf] += ex2(red_ml[w][g + 8 * hf][0] - Ms) * red_ml[w][g + 8 * hf][1];
+      f[hf] = ex2(m[hf] - Ms);
     }
     // (0 + 1) + (2 + 3): warps 1 and 3 store, 0 and 2 add; 2 stores, 0 adds
 #pragma unroll
@@ -400,16 +468,18 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
     c.tile += tiles;
     if (c.tile == c.nt && t < t1) pd_next_item(a, c);
   }
+  copy_wait<0>();
 }
 
-// One block of 128 threads per (sequence, kv head) and query row: merges the item's
-// segments, and in the step adds the new token.
-constexpr int kPdMaxCtas = 1184;
+// One block per (sequence, kv head) and query row merges the item's segments and, in the
+// step, adds the new token.  Warp w takes the segments w, w + 8, ... (a row of 128 floats
+// is one 16-byte load per lane, all of them independent), then the warps join in order.
+constexpr int kPdMaxCtas = 1184, kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
 
 template <bool STEP>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedDecodeArgs a) {
-  __shared__ float fs[kPdMaxCtas];
-  __shared__ float wred[4];
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedDecodeArgs a) {
+  __shared__ __align__(16) float sum_a[kJoinWarps][128], sum_u[kJoinWarps][128];
+  __shared__ float wm[kJoinWarps], wl[kJoinWarps], wz[kJoinWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / a.H, h = blockIdx.x % a.H;
   const int raw = a.lengths[b];
@@ -417,7 +487,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   const bool used = raw >= 0 && !over;
   if (over && tid == 0) report(a.status, kStatusLength, kTagPagedDecode);
   const int n = used ? raw : 0, nt = pd_tiles(n);
-  const int pr = a.D + 4, slot_rows = a.rows + (STEP ? 1 : 0);
+  const int pr = a.D + 4;
+  const long long slot = (long long)(a.rows + (STEP ? 1 : 0)) * pr;
   // first tile of the sequence and the batch's tiles
   long long before = 0, T = 0;
   for (int i = lane; i < a.B; i += 32) {
@@ -434,104 +505,134 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   T *= per;
   before *= per;
   const long long G = pd_ctas(a, T);
-  auto bsum = [&](float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if (lane == 0) wred[warp] = v;
-    __syncthreads();
-    return (wred[0] + wred[1]) + (wred[2] + wred[3]);
-  };
-  auto bmax = [&](float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if (lane == 0) wred[warp] = v;
-    __syncthreads();
-    return fmaxf(fmaxf(wred[0], wred[1]), fmaxf(wred[2], wred[3]));
-  };
-  // segments of the item (h, blk): ctas [i0, i1], slots i + item
-  auto range = [&](int blk, int& i0, int& cnt, const float*& p) {
-    const long long item = (long long)blockIdx.x * a.nblk + blk;
+  // segments of the item (h, blk): ctas [i0, i0 + cnt), slots cta + item
+  auto range = [&](int blk, int& cnt) -> const float* {
+    cnt = 0;
+    if (nt == 0) return a.part;
     const long long first = before + ((long long)h * a.nblk + blk) * nt, last = first + nt - 1;
-    i0 = (int)(((first + 1) * G - 1) / T);
+    const int i0 = (int)(((first + 1) * G - 1) / T);
     cnt = (int)(((last + 1) * G - 1) / T) - i0 + 1;
-    p = a.part + (i0 + item) * (long long)slot_rows * pr;
+    return a.part + (i0 + (long long)blockIdx.x * a.nblk + blk) * slot;
   };
-  const int d = tid;
-  float xv = 0.f, knv = 0.f;
+  const bool col = 4 * lane < a.D;
+  const float c1 = a.s * kLog2e;
+  // the new key and value are nothing that the tile pass writes
+  bf16 kb = __float2bfloat16(0.f);
+  float vv = 0.f;
+  if (STEP && used && tid < a.D) {
+    kb = a.kn[(long long)b * a.kn_sb + (long long)h * a.kn_sh + tid];
+    vv = __bfloat162float(a.vn[(long long)b * a.vn_sb + (long long)h * a.vn_sh + tid]);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the tile pass has ended and its stores are seen
+
+  float xv = 0.f;
   if constexpr (STEP) {
-    float u = 0.f;
-    if (nt > 0) {
-      int i0, cnt;
-      const float* p;
-      range(0, i0, cnt, p);
-      const int upd = min(a.gq, a.rows);
-      if (d < a.D) {
-#pragma unroll 4
-        for (int i = 0; i < cnt; ++i) u += p[((long long)i * slot_rows + upd) * pr + d];
+    int cnt;
+    const float* p = range(0, cnt) + (long long)min(a.gq, a.rows) * pr + 4 * lane;
+    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (col) {
+#pragma unroll 8
+      for (int i = warp; i < cnt; i += kJoinWarps) {
+        const float4 v = *reinterpret_cast<const float4*>(p + i * slot);
+        u.x += v.x; u.y += v.y; u.z += v.z; u.w += v.w;
       }
     }
-    bf16 xb = __float2bfloat16(0.f), kb = xb;
-    if (d < a.D && used) {
-      kb = a.kn[(long long)b * a.kn_sb + (long long)h * a.kn_sh + d];
-      xb = __float2bfloat16(__bfloat162float(a.vn[(long long)b * a.vn_sb + (long long)h * a.vn_sh + d]) - u);
-    }
-    xv = __bfloat162float(xb);
-    knv = __bfloat162float(kb);
-    if (blockIdx.y == 0 && d < a.D) {
-      a.xo[(long long)b * a.xo_sb + (long long)h * a.xo_sh + d] = xb;
-      if (a.append && used) {
-        const int pi = n / a.ps;
-        const int page = pi < a.M ? a.table[(long long)b * a.t_sb + pi] : -1;
-        if (page < 0 || page >= a.P) {
-          if (d == 0) report(a.status, pi < a.M ? kStatusPage : kStatusLength, kTagPagedDecode);
-        } else {
-          const long long row = n % a.ps;
-          a.k.p[(long long)page * a.k.sp + (long long)h * a.k.sh + row * a.k.sn + d] = kb;
-          a.x.p[(long long)page * a.x.sp + (long long)h * a.x.sh + row * a.x.sn + d] = xb;
+    *reinterpret_cast<float4*>(&sum_u[warp][4 * lane]) = u;
+  }
+  for (int r = blockIdx.y; r < a.gq; r += gridDim.y) {
+    int cnt;
+    const float* p = range(r / a.rows, cnt) + (long long)(r % a.rows) * pr;
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = warp; i0 < cnt; i0 += 32 * kJoinWarps) {  // at most 32 segments of this warp at a time
+      const int mine = i0 + lane * kJoinWarps;
+      float mi = -INFINITY, li = 0.f;
+      if (mine < cnt) {
+        mi = p[mine * slot + a.D];
+        li = p[mine * slot + a.D + 1];
+      }
+      float mx = mi;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float mn = fmaxf(M, mx), ms = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2(mi - ms), fo = ex2(M - ms);
+      float ls = f * li;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
+      L = L * fo + ls;
+      acc.x *= fo; acc.y *= fo; acc.z *= fo; acc.w *= fo;
+      M = mn;
+      const int k = min(32, (cnt - i0 + kJoinWarps - 1) / kJoinWarps);
+#pragma unroll 8
+      for (int q = 0; q < k; ++q) {
+        const float fq = __shfl_sync(0xffffffffu, f, q);
+        if (col) {
+          const float4 v = *reinterpret_cast<const float4*>(p + (long long)(i0 + q * kJoinWarps) * slot + 4 * lane);
+          acc.x = fmaf(fq, v.x, acc.x);
+          acc.y = fmaf(fq, v.y, acc.y);
+          acc.z = fmaf(fq, v.z, acc.z);
+          acc.w = fmaf(fq, v.w, acc.w);
         }
       }
     }
-  }
-  for (int r = blockIdx.y; r < a.gq; r += gridDim.y) {
-    const long long orow = (long long)b * a.o_sb + (long long)(h * a.gq + r) * a.o_sh;
-    if (!used || (!STEP && nt == 0)) {   // no token to attend to
-      if (d < a.D) a.o[orow + d] = __float2bfloat16(0.f);
-      continue;
+    float z = 0.f;
+    if constexpr (STEP) {  // the new token's score: thread d < 128 has element d
+      if (tid < a.D)
+        z = __bfloat162float(a.q[(long long)b * a.q_sb + (long long)(h * a.gq + r) * a.q_sh + tid]) * __bfloat162float(kb);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
     }
-    int i0 = 0, cnt = 0;
-    const float* p = nullptr;
-    if (nt > 0) range(r / a.rows, i0, cnt, p);
-    const int rr = r % a.rows;
-    float z = -INFINITY;
-    if constexpr (STEP) {
-      const float qv = d < a.D ? __bfloat162float(a.q[(long long)b * a.q_sb + (long long)(h * a.gq + r) * a.q_sh + d]) : 0.f;
-      z = bsum(qv * knv) * a.s * kLog2e;
+    *reinterpret_cast<float4*>(&sum_a[warp][4 * lane]) = acc;
+    if (lane == 0) {
+      wm[warp] = M;
+      wl[warp] = L;
+      wz[warp] = z;
     }
-    float mx = z;
-    for (int i = tid; i < cnt; i += 128) mx = fmaxf(mx, p[((long long)i * slot_rows + rr) * pr + a.D]);
-    const float M = bmax(mx), Ms = M == -INFINITY ? 0.f : M;
-    float ls = 0.f;
-    for (int i = tid; i < cnt; i += 128) {
-      const float* e = p + ((long long)i * slot_rows + rr) * pr + a.D;
-      const float f = exp2f(e[0] - Ms);
-      fs[i] = f;
-      ls += f * e[1];
+    __syncthreads();
+    if (tid < a.D) {
+      if (STEP && r == (int)blockIdx.y) {  // x_new, as the cache holds it
+        float u = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) u += sum_u[w][tid];
+        const bf16 xb = __float2bfloat16(vv - u);
+        xv = __bfloat162float(xb);
+        if (blockIdx.y == 0) {
+          a.xo[(long long)b * a.xo_sb + (long long)h * a.xo_sh + tid] = xb;
+          if (a.append && used) {
+            const int pi = n / a.ps;
+            const int page = pi < a.M ? a.table[(long long)b * a.t_sb + pi] : -1;
+            if (page < 0 || page >= a.P) {
+              if (tid == 0) report(a.status, pi < a.M ? kStatusPage : kStatusLength, kTagPagedDecode);
+            } else {
+              const long long row = n % a.ps;
+              a.k.p[(long long)page * a.k.sp + (long long)h * a.k.sh + row * a.k.sn + tid] = kb;
+              a.x.p[(long long)page * a.x.sp + (long long)h * a.x.sh + row * a.x.sn + tid] = xb;
+            }
+          }
+        }
+      }
+      float mx = -INFINITY, zn = -INFINITY;
+      if constexpr (STEP) zn = ((wz[0] + wz[1]) + (wz[2] + wz[3])) * c1;
+      mx = zn;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) mx = fmaxf(mx, wm[w]);
+      const float ms = mx == -INFINITY ? 0.f : mx;
+      float Ls = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float f = ex2(wm[w] - ms);
+        Ls = fmaf(f, wl[w], Ls);
+        o = fmaf(f, sum_a[w][tid], o);
+      }
+      if constexpr (STEP) {
+        const float pn = ex2(zn - ms);
+        Ls += pn;
+        o = fmaf(pn, xv, o);
+      }
+      const bool none = !used || (!STEP && nt == 0);  // no token to attend to
+      a.o[(long long)b * a.o_sb + (long long)(h * a.gq + r) * a.o_sh + tid] = __float2bfloat16(none ? 0.f : o / Ls);
     }
-    float L = bsum(ls);  // its barriers also order fs
-    float acc = 0.f;
-    if (d < a.D) {
-#pragma unroll 4
-      for (int i = 0; i < cnt; ++i) acc = fmaf(fs[i], p[((long long)i * slot_rows + rr) * pr + d], acc);
-    }
-    if constexpr (STEP) {
-      const float pn = exp2f(z - Ms);
-      L += pn;
-      acc = fmaf(pn, xv, acc);
-    }
-    if (d < a.D) a.o[orow + d] = __float2bfloat16(acc / L);
-    __syncthreads();  // fs is free again
+    __syncthreads();  // the sums are free again
   }
 }
 
@@ -546,7 +647,11 @@ int paged_decode_ctas() {
 
 template <bool STEP, bool R8, int CE, int NK, int NX>
 static cudaError_t launch_pd(const PagedDecodeArgs& a, cudaStream_t st) {
-  paged_decode_kernel<STEP, R8, CE, NK, NX><<<a.nctas, kPdThreads, 0, st>>>(a);
+  constexpr int smem = kPdWarps * kPdStages * pd_stage_bytes<CE, NK, NX>();
+  const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<STEP, R8, CE, NK, NX>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  paged_decode_kernel<STEP, R8, CE, NK, NX><<<a.nctas, kPdThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -568,11 +673,19 @@ cudaError_t launch_paged_decode(const PagedDecodeArgs& a, bool step, cudaStream_
   cudaError_t e = step ? (rows <= 8 ? launch_pd_d<true, true>(a, st) : launch_pd_d<true, false>(a, st))
                        : (rows <= 8 ? launch_pd_d<false, true>(a, st) : launch_pd_d<false, false>(a, st));
   if (e != cudaSuccess) return e;
-  // one block per query row while that still fills the GPU only a few times over
-  const int bh = a.B * a.H, gy = bh >= 4096 ? 1 : a.gq;
-  if (step) paged_join_kernel<true><<<dim3(bh, gy), 128, 0, st>>>(a);
-  else paged_join_kernel<false><<<dim3(bh, gy), 128, 0, st>>>(a);
-  return cudaGetLastError();
+  // one block per query row while that fills the GPU only a few times over.  The join's
+  // blocks may start while the tile pass ends (they wait before reading its results).
+  const int bh = a.B * a.H;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(bh, bh >= 4096 ? 1 : a.gq);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return step ? cudaLaunchKernelEx(&cfg, paged_join_kernel<true>, a) : cudaLaunchKernelEx(&cfg, paged_join_kernel<false>, a);
 }
 
 }  // namespace lb
