@@ -29,6 +29,7 @@ namespace lb {
 constexpr int kPdWarps = 4, kPdThreads = 32 * kPdWarps;
 constexpr int kPdTile = 16 * kPdWarps;  // tokens per tile, 16 per warp
 constexpr int kPdStages = 3;
+constexpr float kPdSlack = 8.f;         // log2 units
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -87,6 +88,13 @@ __device__ __forceinline__ long long pd_ctas(const PagedDecodeArgs& a, long long
   return T < a.nctas ? T : a.nctas;
 }
 
+// a / b for nonnegative a and positive b; nearly always both fit 32 bits, where the
+// division is several times shorter
+__device__ __forceinline__ long long pd_div(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return (unsigned)a / (unsigned)b;
+  return a / b;
+}
+
 // position in the sequence of tiles
 struct PdCursor {
   int b, hb, tile, nt, n;  // sequence, h * nblk + blk, tile of the item, the item's tiles, tokens
@@ -112,8 +120,8 @@ __device__ __forceinline__ PdCursor pd_seek(const PagedDecodeArgs& a, long long 
       c.n = __shfl_sync(0xffffffffu, n, f);
       c.nt = pd_tiles(c.n);
       const long long rem = t0 - acc - __shfl_sync(0xffffffffu, incl - own, f);
-      c.hb = (int)(rem / c.nt);
-      c.tile = (int)(rem % c.nt);
+      c.hb = (int)pd_div(rem, c.nt);
+      c.tile = (int)(rem - (long long)c.hb * c.nt);
       return c;
     }
     acc += __shfl_sync(0xffffffffu, incl, 31);
@@ -145,15 +153,20 @@ __device__ __forceinline__ void load_chunk(const unsigned char* p, uint32_t (&r)
   }
 }
 
-// bytes of one stage of one warp: 16 tokens' chunks of both pools
-template <int CE, int NK, int NX>
-constexpr int pd_stage_bytes() { return 32 * (2 * NK + 4 * NX) * CE * 2; }
+// Shared-memory rows: 16 tokens of each pool per warp and stage, RB bytes each (128 up to
+// D = 64, else 256), a chunk's place in its row swizzled so that the fragment reads below
+// are free of bank conflicts (8 lanes read 16-byte, 16 lanes 8-byte chunks at a time: key
+// reads take chunks 4 i + j of rows g, value reads chunks 8 c + g of rows 2 j + const).
+template <int CE>
+__device__ __forceinline__ int pd_kswz(int row) { return CE == 8 ? (row & 1) * 4 : (row & 3) * 4; }
+template <int CE>
+__device__ __forceinline__ int pd_xswz(int row) { return ((row >> 1) & 3) * (CE == 8 ? 2 : 4); }
+template <int CE, int NX>
+constexpr int pd_row_bytes() { return NX * 16 * CE <= 128 ? 128 : 256; }
 
-// The rows stream through a ring of kPdStages stages per warp, filled by cp.async two
-// tiles ahead across item borders.  Each lane copies exactly the chunks that it later
-// multiplies, so a stage needs no barrier, only the lane's own wait; one copy instruction
-// of the warp covers 64 (keys) or 128 (values) contiguous bytes of each of its rows.  Page
-// numbers are looked up one tile before their copies are issued.
+// The rows stream through a ring of kPdStages stages per warp, filled by cp.async across
+// item borders: consecutive lanes copy consecutive chunks, so whole rows are requested at
+// once.  Page numbers are looked up one tile before their copies are issued.
 //
 // STEP: an update row behind the query rows.  R8: at most 8 rows, so rows 8-15 of the
 // P operand carry the low halves of P and one mma does both.  A row's elements are cut
@@ -161,13 +174,14 @@ constexpr int pd_stage_bytes() { return 32 * (2 * NK + 4 * NX) * CE * 2; }
 // quad holds the key chunks 4 i + j (i < NK), lane group g the value chunks
 // 8 c + g (c < NX); the same permutation of the inner index on both operands, and of
 // the output columns, leaves the products unchanged.
-template <bool STEP, bool R8, int CE, int NK, int NX>
+template <bool STEP, bool R8, int CE, int NK, int NX, bool FULL>
 __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __grid_constant__ PagedDecodeArgs a) {
   constexpr int NT = NX * CE;      // 8-column output tiles
   constexpr int KR = CE / 2;       // 32-bit registers per chunk
   constexpr int KS = NK * CE / 4;  // 16-element k steps
-  constexpr int CB = CE * 2, STAGE = pd_stage_bytes<CE, NK, NX>();
-  extern __shared__ __align__(16) unsigned char ring[];  // [warp][stage][chunk][lane][CB]
+  constexpr int CB = CE * 2, RB = pd_row_bytes<CE, NX>(), STAGE = 32 * RB;
+  constexpr int NU = FULL ? RB / CB / 2 : (NK * 4 + 1) / 2;  // copies per lane and pool, at most
+  extern __shared__ __align__(16) unsigned char ring[];  // [warp][stage][pool][16 tokens][RB]
   __shared__ float red[2][R8 ? 8 : 16][132];  // a warp pair's accumulator rows
   __shared__ float red_ml[kPdWarps][16][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
@@ -175,57 +189,72 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
   const long long T = pd_total(a, lane);
   const long long G = pd_ctas(a, T);
   if (blockIdx.x >= G) return;
-  const long long t0 = blockIdx.x * T / G, t1 = (blockIdx.x + 1) * T / G;
+  const long long t0 = pd_div(blockIdx.x * T, G);
+  int left = (int)(pd_div((blockIdx.x + 1) * T, G) - t0);  // tiles of this CTA
   PdCursor c = pd_seek(a, t0, lane);
   const float c1 = a.s * kLog2e, c2 = kLog2e / a.s, inv_d = 1.f / (float)a.D;
-  const unsigned char* own = ring + warp * (kPdStages * STAGE) + lane * CB;
+  unsigned char* own = ring + warp * (kPdStages * STAGE);
   const uint32_t own_s = (uint32_t)__cvta_generic_to_shared(own);
 
   // ---- the producer's side: cursor `pc` runs ahead of `c` ----
   PdCursor pc = c;
-  long long pt = t0;             // tile whose page numbers are in (page, row)
-  int page = -1, row = 0, ph = 0;
-  auto look_up = [&]() {         // token 16 warp + (lane & 15) of tile pt
+  int ahead = left;              // tiles from the one whose offsets are in (koff, xoff)
+  long long koff = 0, xoff = 0;  // element offsets of the row of token 16 warp + (lane & 15)
+  auto look_up = [&]() {
     const int tok = pc.tile * kPdTile + 16 * warp + (lane & 15);
-    page = -1;
-    ph = pc.hb / a.nblk;
-    if (pt < t1 && tok < pc.n) {
-      const int pi = tok / a.ps;
-      row = tok - pi * a.ps;
-      page = a.table[(long long)pc.b * a.t_sb + pi];
+    if (ahead > 0 && tok < pc.n) {
+      const int pi = tok / a.ps, row = tok - pi * a.ps, h = pc.hb / a.nblk;
+      int page = a.table[(long long)pc.b * a.t_sb + pi];
+      if (page < 0 || page >= a.P) {
+        report(a.status, kStatusPage, kTagPagedDecode);
+        page = 0;
+      }
+      koff = page * a.k.sp + h * a.k.sh + row * a.k.sn;
+      xoff = page * a.x.sp + h * a.x.sh + row * a.x.sn;
     }
   };
-  auto issue = [&](int st) {     // copies of tile pt, then the look-up of the next
-    if (pt < t1) {
-      if (page >= a.P || (page < 0 && pc.tile * kPdTile + 16 * warp + (lane & 15) < pc.n)) {
-        report(a.status, kStatusPage, kTagPagedDecode);
-        page = -1;
-      }
-      const bf16* kh = a.k.p + (long long)ph * a.k.sh;
-      const bf16* xh = a.x.p + (long long)ph * a.x.sh;
+  // this lane's copies: element e = 32 u + lane of the 16 x nc chunks; packed as row,
+  // element offset in the row, place of a key and of a value chunk in the stage
+  const int nc = a.D / CE, inv_nc = (65535 + nc) / nc;   // e / nc = e inv_nc >> 16 for e < 2048
+  uint32_t todo[NU], place[NU];
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    const int e = 32 * u + lane, r = FULL ? e / (RB / CB) : (e * inv_nc) >> 16, ch = FULL ? e % (RB / CB) : e - r * nc;
+    todo[u] = FULL || r < 16 ? r | (ch * CE) << 8 : 0xffu;
+    place[u] = (r * RB + (ch ^ pd_kswz<CE>(r)) * CB) | (16 * RB + r * RB + (ch ^ pd_xswz<CE>(r)) * CB) << 16;
+  }
+  if constexpr (!FULL) {         // the chunks between D and the fragments' width stay zero
+    for (int i = lane; i < kPdStages * STAGE / 16; i += 32) *reinterpret_cast<uint4*>(own + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+    __syncwarp();
+  }
+  const bool one_page = (a.ps & 15) == 0;  // a warp's 16 tokens never span two pages
+  auto issue = [&](int st) {     // copies of the producer's tile, then the look-up of the next
+    if (ahead > 0) {
       const uint32_t dst = own_s + st * STAGE;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        const int pg = __shfl_sync(0xffffffffu, page, g + 8 * kt), rw = __shfl_sync(0xffffffffu, row, g + 8 * kt);
-        const bf16* p = kh + (long long)max(pg, 0) * a.k.sp + (long long)rw * a.k.sn + j * CE;
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          const int bytes = pg >= 0 ? max(0, min(CB, (a.D - (4 * i + j) * CE) * 2)) : 0;
-          copy_async<CB>(dst + (kt * NK + i) * 32 * CB, bytes ? p + 4 * i * CE : a.k.p, bytes);
-        }
+      const int lim = pc.n - (pc.tile * kPdTile + 16 * warp);  // tokens of this warp's 16
+      long long k0 = 0, x0 = 0;
+      if (one_page && lim > 0) {
+        k0 = __shfl_sync(0xffffffffu, koff, 0);
+        x0 = __shfl_sync(0xffffffffu, xoff, 0);
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int kq = 8 * (q >> 1) + 2 * j + (q & 1);
-        const int pg = __shfl_sync(0xffffffffu, page, kq), rw = __shfl_sync(0xffffffffu, row, kq);
-        const bf16* p = xh + (long long)max(pg, 0) * a.x.sp + (long long)rw * a.x.sn + g * CE;
-#pragma unroll
-        for (int cx = 0; cx < NX; ++cx) {
-          const int bytes = pg >= 0 ? max(0, min(CB, (a.D - (8 * cx + g) * CE) * 2)) : 0;
-          copy_async<CB>(dst + (2 * NK + cx * 4 + q) * 32 * CB, bytes ? p + 8 * cx * CE : a.x.p, bytes);
+      for (int u = 0; u < NU; ++u) {
+        const int r = todo[u] & 0xff, e = todo[u] >> 8;
+        const bool in = r < lim;
+        long long ko, xo;
+        if (one_page) {
+          ko = k0 + r * a.k.sn;
+          xo = x0 + r * a.x.sn;
+        } else {
+          ko = __shfl_sync(0xffffffffu, koff, r & 15);
+          xo = __shfl_sync(0xffffffffu, xoff, r & 15);
+        }
+        if (FULL || r < 16) {
+          copy_async<CB>(dst + (place[u] & 0xffff), a.k.p + (in ? ko + e : 0), in ? CB : 0);
+          copy_async<CB>(dst + (place[u] >> 16), a.x.p + (in ? xo + e : 0), in ? CB : 0);
         }
       }
-      if (++pt < t1 && ++pc.tile == pc.nt) pd_next_item(a, pc);
+      if (--ahead > 0 && ++pc.tile == pc.nt) pd_next_item(a, pc);
       look_up();
     }
     copy_commit();
@@ -235,13 +264,13 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
   for (int s = 0; s < kPdStages - 1; ++s) issue(s);
   int st = 0;                    // stage of the consumer's tile
 
-  for (long long t = t0; t < t1;) {
+  while (left > 0) {
     // ---- one segment: the run's tiles of one item ----
     const int h = c.hb / a.nblk, blk = c.hb % a.nblk;
     const int r_first = blk * a.rows;                      // first query row of the block
     const int nq = min(a.gq - r_first, a.rows);            // query rows of the block
     const int upd = STEP && blk == 0 ? nq : -1;            // the update row
-    const int tiles = (int)min((long long)(c.nt - c.tile), t1 - t);
+    const int tiles = min(c.nt - c.tile, left);
     // operand A: rows g and g + 8
     uint32_t qa[KS][R8 ? 2 : 4];
     float ss = 0.f;
@@ -282,8 +311,10 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
     m[1] = STEP && g + 8 == upd ? 0.f : -INFINITY;
 
     for (int it = 0; it < tiles; ++it) {
+      __syncwarp();                          // every lane has read the stage that is filled next
       issue(st == 0 ? kPdStages - 1 : st - 1);
-      copy_wait<kPdStages - 1>();            // this lane's copies of tile t + it have landed
+      copy_wait<kPdStages - 1>();            // this lane's copies of the tile have landed,
+      __syncwarp();                          // and the other lanes'
       const unsigned char* in = own + st * STAGE;
       st = st + 1 == kPdStages ? 0 : st + 1;
       const int base = (c.tile + it) * kPdTile + 16 * warp;
@@ -293,7 +324,7 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < NK; ++i) load_chunk<KR>(in + (kt * NK + i) * 32 * CB, kr[kt][i]);
+        for (int i = 0; i < NK; ++i) load_chunk<KR>(in + (g + 8 * kt) * RB + ((4 * i + j) ^ pd_kswz<CE>(g)) * CB, kr[kt][i]);
       float S[2][4] = {};
       float dg[2][4] = {};
 #pragma unroll
@@ -331,19 +362,26 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
         for (int q = 0; q < 4; ++q) {
           const float sc = S[q >> 1][2 * hf + (q & 1)];
           z[q] = is_upd ? fmaf(sc * rs_new * rk[q], c1, -c2) : sc * c1;
-          if (base + 8 * (q >> 1) + 2 * j + (q & 1) >= c.n) z[q] = -INFINITY;
+        }
+        if (base + 16 > c.n) {               // uniform: the sequence's last tokens
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (base + 8 * (q >> 1) + 2 * j + (q & 1) >= c.n) z[q] = -INFINITY;
         }
         float mx = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = is_upd ? 0.f : fmaxf(m[hf], mx);
-        const float ms = mn == -INFINITY ? 0.f : mn;
-        al[hf] = ex2(m[hf] - ms);            // 0 while nothing has been seen
+        // the reference point moves only when a score passes it by kPdSlack: until then
+        // the weights stay below 2^kPdSlack, whose digits fp32 and bf16 pairs hold alike
+        if (!is_upd && mx > m[hf] + kPdSlack) {
+          al[hf] = ex2(m[hf] - mx);          // 0 while nothing has been seen
+          m[hf] = mx;
+        }
+        const float ms = m[hf] == -INFINITY ? 0.f : m[hf];
         float p[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) p[q] = ex2(z[q] - ms);
         l[hf] = l[hf] * al[hf] + ((p[0] + p[1]) + (p[2] + p[3]));
-        m[hf] = mn;
         phi[2 * hf] = pack_bf16(p[0], p[1]);
         phi[2 * hf + 1] = pack_bf16(p[2], p[3]);
         const float2 h0 = unpack_bf16(phi[2 * hf]), h1 = unpack_bf16(phi[2 * hf + 1]);
@@ -365,7 +403,8 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
       for (int cx = 0; cx < NX; ++cx) {
         uint32_t xr[4][KR];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) load_chunk<KR>(in + (2 * NK + cx * 4 + q) * 32 * CB, xr[q]);
+        for (int q = 0; q < 4; ++q)
+          load_chunk<KR>(in + (16 + 8 * (q >> 1) + 2 * j + (q & 1)) * RB + ((8 * cx + g) ^ pd_xswz<CE>(2 * j)) * CB, xr[q]);
 #pragma unroll
         for (int e = 0; e < CE; ++e) {
           const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
@@ -464,9 +503,9 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
       }
     }
     // ---- on to the next item ----
-    t += tiles;
+    left -= tiles;
     c.tile += tiles;
-    if (c.tile == c.nt && t < t1) pd_next_item(a, c);
+    if (c.tile == c.nt && left > 0) pd_next_item(a, c);
   }
   copy_wait<0>();
 }
@@ -510,8 +549,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     cnt = 0;
     if (nt == 0) return a.part;
     const long long first = before + ((long long)h * a.nblk + blk) * nt, last = first + nt - 1;
-    const int i0 = (int)(((first + 1) * G - 1) / T);
-    cnt = (int)(((last + 1) * G - 1) / T) - i0 + 1;
+    const int i0 = (int)pd_div((first + 1) * G - 1, T);
+    cnt = (int)pd_div((last + 1) * G - 1, T) - i0 + 1;
     return a.part + (i0 + (long long)blockIdx.x * a.nblk + blk) * slot;
   };
   const bool col = 4 * lane < a.D;
@@ -645,13 +684,13 @@ int paged_decode_ctas() {
   return std::min(2 * sms, kPdMaxCtas);
 }
 
-template <bool STEP, bool R8, int CE, int NK, int NX>
+template <bool STEP, bool R8, int CE, int NK, int NX, bool FULL>
 static cudaError_t launch_pd(const PagedDecodeArgs& a, cudaStream_t st) {
-  constexpr int smem = kPdWarps * kPdStages * pd_stage_bytes<CE, NK, NX>();
-  const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<STEP, R8, CE, NK, NX>,
+  constexpr int smem = kPdWarps * kPdStages * 32 * pd_row_bytes<CE, NX>();
+  const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<STEP, R8, CE, NK, NX, FULL>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  paged_decode_kernel<STEP, R8, CE, NK, NX><<<a.nctas, kPdThreads, smem, st>>>(a);
+  paged_decode_kernel<STEP, R8, CE, NK, NX, FULL><<<a.nctas, kPdThreads, smem, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -660,12 +699,14 @@ static cudaError_t launch_pd_d(const PagedDecodeArgs& a, cudaStream_t st) {
   const bool al16 = ((reinterpret_cast<uintptr_t>(a.k.p) | reinterpret_cast<uintptr_t>(a.x.p)) & 15u) == 0 &&
                     ((a.k.sp | a.k.sh | a.k.sn | a.x.sp | a.x.sh | a.x.sn) & 7) == 0;
   if (al16 && a.D % 8 == 0) {
-    if (a.D <= 64) return launch_pd<STEP, R8, 8, 2, 1>(a, st);
-    return launch_pd<STEP, R8, 8, 4, 2>(a, st);
+    if (a.D == 64) return launch_pd<STEP, R8, 8, 2, 1, true>(a, st);
+    if (a.D == 128) return launch_pd<STEP, R8, 8, 4, 2, true>(a, st);
+    if (a.D < 64) return launch_pd<STEP, R8, 8, 2, 1, false>(a, st);
+    return launch_pd<STEP, R8, 8, 4, 2, false>(a, st);
   }
-  if (a.D <= 64) return launch_pd<STEP, R8, 4, 4, 2>(a, st);
-  if (a.D <= 80) return launch_pd<STEP, R8, 4, 5, 3>(a, st);
-  return launch_pd<STEP, R8, 4, 8, 4>(a, st);
+  if (a.D <= 64) return launch_pd<STEP, R8, 4, 4, 2, false>(a, st);
+  if (a.D <= 80) return launch_pd<STEP, R8, 4, 5, 3, false>(a, st);
+  return launch_pd<STEP, R8, 4, 8, 4, false>(a, st);
 }
 
 cudaError_t launch_paged_decode(const PagedDecodeArgs& a, bool step, cudaStream_t st) {
