@@ -28,7 +28,6 @@ namespace lb {
 
 constexpr int kPdWarps = 4, kPdThreads = 32 * kPdWarps;
 constexpr int kPdTile = 16 * kPdWarps;  // tokens per tile, 16 per warp
-constexpr int kPdStages = 3;
 constexpr float kPdSlack = 8.f;         // log2 units
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -161,10 +160,30 @@ template <int CE>
 __device__ __forceinline__ int pd_kswz(int row) { return CE == 8 ? (row & 1) * 4 : (row & 3) * 4; }
 template <int CE>
 __device__ __forceinline__ int pd_xswz(int row) { return ((row >> 1) & 3) * (CE == 8 ? 2 : 4); }
-template <int CE, int NX>
-constexpr int pd_row_bytes() { return NX * 16 * CE <= 128 ? 128 : 256; }
 
-// The rows stream through a ring of kPdStages stages per warp, filled by cp.async across
+// How rows reach shared memory.  kRows: any strides, row by row.  kFull: rows of exactly
+// the fragments' width, the same with constant places.  kFlat: rows that follow one another
+// in pages of a multiple of 16 tokens but start on 8-byte boundaries only (an odd multiple
+// of 4 elements): the 16 tokens are one run of bytes, copied 16 at a time as it is (5
+// copies per lane and pool at D = 68 instead of 9), whose reads conflict up to 4-way.
+enum : int { kRows = 0, kFull = 1, kFlat = 2 };
+
+// Three CTAs of four warps per SM where the registers allow (at most 168 a thread): the
+// tile loop is a chain of short dependent steps, and D = 128 over 4 x 32K tokens took
+// 388 us with two CTAs and three stages, 336 us with three and two.  16 rows at D > 96,
+// and the addresses of odd rows at D > 64, need more registers.
+template <bool R8, int CE, int NK, int NX, int MODE>
+struct PdShape {
+  static constexpr int kCols = NX * 8 * CE;                 // columns covered
+  static constexpr int kRowBytes = MODE == kFlat ? 0 : kCols <= 64 ? 128 : 256;
+  static constexpr int kPool = MODE == kFlat ? 16 * 2 * ((NK * 16 < kCols ? NK * 16 : kCols) - 4) : 16 * kRowBytes;  // bytes of a pool in a stage, at most
+  static constexpr int kCtas = kCols <= 64 || MODE != kRows && (R8 || kCols <= 96) ? 3 : 2;
+  static constexpr int kStages = kCtas == 2 || kPool <= 3072 ? 3 : 2;
+  // reads of the columns past D may run up to 192 bytes past a flat run
+  static constexpr int kSmem = kPdWarps * kStages * 2 * kPool + (MODE == kFlat ? 256 : 0);
+};
+
+// The rows stream through a ring of stages per warp, filled by cp.async across
 // item borders: consecutive lanes copy consecutive chunks, so whole rows are requested at
 // once.  Page numbers are looked up one tile before their copies are issued.
 //
@@ -174,14 +193,15 @@ constexpr int pd_row_bytes() { return NX * 16 * CE <= 128 ? 128 : 256; }
 // quad holds the key chunks 4 i + j (i < NK), lane group g the value chunks
 // 8 c + g (c < NX); the same permutation of the inner index on both operands, and of
 // the output columns, leaves the products unchanged.
-template <bool STEP, bool R8, int CE, int NK, int NX, bool FULL>
-__global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __grid_constant__ PagedDecodeArgs a) {
+template <bool STEP, bool R8, int CE, int NK, int NX, int MODE>
+__global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCtas) paged_decode_kernel(const __grid_constant__ PagedDecodeArgs a) {
   constexpr int NT = NX * CE;      // 8-column output tiles
   constexpr int KR = CE / 2;       // 32-bit registers per chunk
   constexpr int KS = NK * CE / 4;  // 16-element k steps
-  constexpr int CB = CE * 2, RB = pd_row_bytes<CE, NX>(), STAGE = 32 * RB;
-  constexpr int NU = FULL ? RB / CB / 2 : (NK * 4 + 1) / 2;  // copies per lane and pool, at most
-  extern __shared__ __align__(16) unsigned char ring[];  // [warp][stage][pool][16 tokens][RB]
+  using Shape = PdShape<R8, CE, NK, NX, MODE>;
+  constexpr int CB = CE * 2, RB = Shape::kRowBytes, POOL = Shape::kPool, STAGE = 2 * POOL, STAGES = Shape::kStages;
+  constexpr int NU = MODE == kFull ? RB / CB / 2 : MODE == kRows ? (NK * 4 + 1) / 2 : (POOL / 16 + 31) / 32;  // copies per lane and pool
+  extern __shared__ __align__(16) unsigned char ring[];  // [warp][stage][pool]: 16 tokens
   __shared__ float red[2][R8 ? 8 : 16][132];  // a warp pair's accumulator rows
   __shared__ float red_ml[kPdWarps][16][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
@@ -193,7 +213,7 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
   int left = (int)(pd_div((blockIdx.x + 1) * T, G) - t0);  // tiles of this CTA
   PdCursor c = pd_seek(a, t0, lane);
   const float c1 = a.s * kLog2e, c2 = kLog2e / a.s, inv_d = 1.f / (float)a.D;
-  unsigned char* own = ring + warp * (kPdStages * STAGE);
+  unsigned char* own = ring + warp * (STAGES * STAGE);
   const uint32_t own_s = (uint32_t)__cvta_generic_to_shared(own);
 
   // ---- the producer's side: cursor `pc` runs ahead of `c` ----
@@ -213,21 +233,24 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
       xoff = page * a.x.sp + h * a.x.sh + row * a.x.sn;
     }
   };
-  // this lane's copies: element e = 32 u + lane of the 16 x nc chunks; packed as row,
+  // this lane's copies by rows: element 32 u + lane of the 16 x nc chunks; packed as row,
   // element offset in the row, place of a key and of a value chunk in the stage
   const int nc = a.D / CE, inv_nc = (65535 + nc) / nc;   // e / nc = e inv_nc >> 16 for e < 2048
-  uint32_t todo[NU], place[NU];
+  uint32_t todo[MODE == kFlat ? 1 : NU], place[MODE == kFlat ? 1 : NU];
+  if constexpr (MODE != kFlat) {
 #pragma unroll
-  for (int u = 0; u < NU; ++u) {
-    const int e = 32 * u + lane, r = FULL ? e / (RB / CB) : (e * inv_nc) >> 16, ch = FULL ? e % (RB / CB) : e - r * nc;
-    todo[u] = FULL || r < 16 ? r | (ch * CE) << 8 : 0xffu;
-    place[u] = (r * RB + (ch ^ pd_kswz<CE>(r)) * CB) | (16 * RB + r * RB + (ch ^ pd_xswz<CE>(r)) * CB) << 16;
+    for (int u = 0; u < NU; ++u) {
+      const int e = 32 * u + lane, r = MODE == kFull ? e / (RB / CB) : (e * inv_nc) >> 16;
+      const int ch = MODE == kFull ? e % (RB / CB) : e - r * nc;
+      todo[u] = MODE == kFull || r < 16 ? r | (ch * CE) << 8 : 0xffu;
+      place[u] = (r * RB + (ch ^ pd_kswz<CE>(r)) * CB) | (POOL + r * RB + (ch ^ pd_xswz<CE>(r)) * CB) << 16;
+    }
   }
-  if constexpr (!FULL) {         // the chunks between D and the fragments' width stay zero
-    for (int i = lane; i < kPdStages * STAGE / 16; i += 32) *reinterpret_cast<uint4*>(own + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+  if constexpr (MODE == kRows) {  // the chunks between D and the fragments' width stay zero
+    for (int i = lane; i < STAGES * STAGE / 16; i += 32) *reinterpret_cast<uint4*>(own + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
     __syncwarp();
   }
-  const bool one_page = (a.ps & 15) == 0;  // a warp's 16 tokens never span two pages
+  const bool one_page = MODE == kFlat || (a.ps & 15) == 0;  // a warp's 16 tokens never span two pages
   auto issue = [&](int st) {     // copies of the producer's tile, then the look-up of the next
     if (ahead > 0) {
       const uint32_t dst = own_s + st * STAGE;
@@ -237,21 +260,35 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
         k0 = __shfl_sync(0xffffffffu, koff, 0);
         x0 = __shfl_sync(0xffffffffu, xoff, 0);
       }
+      if constexpr (MODE == kFlat) {
+        const int most = max(0, min(lim, 16)) * a.D * 2;   // bytes of the run that are tokens
+        const bf16* kp = a.k.p + k0;
+        const bf16* xp = a.x.p + x0;
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        const int r = todo[u] & 0xff, e = todo[u] >> 8;
-        const bool in = r < lim;
-        long long ko, xo;
-        if (one_page) {
-          ko = k0 + r * a.k.sn;
-          xo = x0 + r * a.x.sn;
-        } else {
-          ko = __shfl_sync(0xffffffffu, koff, r & 15);
-          xo = __shfl_sync(0xffffffffu, xoff, r & 15);
+        for (int u = 0; u < NU; ++u) {
+          const int e = 16 * (32 * u + lane), bytes = max(0, min(16, most - e)), from = bytes > 0 ? e / 2 : 0;
+          if (e < 32 * a.D) {
+            copy_async<16>(dst + e, kp + from, bytes);
+            copy_async<16>(dst + POOL + e, xp + from, bytes);
+          }
         }
-        if (FULL || r < 16) {
-          copy_async<CB>(dst + (place[u] & 0xffff), a.k.p + (in ? ko + e : 0), in ? CB : 0);
-          copy_async<CB>(dst + (place[u] >> 16), a.x.p + (in ? xo + e : 0), in ? CB : 0);
+      } else {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          const int r = todo[u] & 0xff, e = todo[u] >> 8;
+          const bool in = r < lim;
+          long long ko, xo;
+          if (one_page) {
+            ko = k0 + r * a.k.sn;
+            xo = x0 + r * a.x.sn;
+          } else {
+            ko = __shfl_sync(0xffffffffu, koff, r & 15);
+            xo = __shfl_sync(0xffffffffu, xoff, r & 15);
+          }
+          if (MODE == kFull || r < 16) {
+            copy_async<CB>(dst + (place[u] & 0xffff), a.k.p + (in ? ko + e : 0), in ? CB : 0);
+            copy_async<CB>(dst + (place[u] >> 16), a.x.p + (in ? xo + e : 0), in ? CB : 0);
+          }
         }
       }
       if (--ahead > 0 && ++pc.tile == pc.nt) pd_next_item(a, pc);
@@ -261,7 +298,7 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
   };
   look_up();
 #pragma unroll
-  for (int s = 0; s < kPdStages - 1; ++s) issue(s);
+  for (int s = 0; s < STAGES - 1; ++s) issue(s);
   int st = 0;                    // stage of the consumer's tile
 
   while (left > 0) {
@@ -312,11 +349,11 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
 
     for (int it = 0; it < tiles; ++it) {
       __syncwarp();                          // every lane has read the stage that is filled next
-      issue(st == 0 ? kPdStages - 1 : st - 1);
-      copy_wait<kPdStages - 1>();            // this lane's copies of the tile have landed,
+      issue(st == 0 ? STAGES - 1 : st - 1);
+      copy_wait<STAGES - 1>();            // this lane's copies of the tile have landed,
       __syncwarp();                          // and the other lanes'
       const unsigned char* in = own + st * STAGE;
-      st = st + 1 == kPdStages ? 0 : st + 1;
+      st = st + 1 == STAGES ? 0 : st + 1;
       const int base = (c.tile + it) * kPdTile + 16 * warp;
       if (base >= c.n) continue;             // uniform in the warp
       // keys: operand B of both 8-key tiles
@@ -324,7 +361,15 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < NK; ++i) load_chunk<KR>(in + (g + 8 * kt) * RB + ((4 * i + j) ^ pd_kswz<CE>(g)) * CB, kr[kt][i]);
+        for (int i = 0; i < NK; ++i) {
+          if constexpr (MODE == kFlat) {
+            // a chunk past D is the next row's: not this key's
+            load_chunk<KR>(in + (g + 8 * kt) * 2 * a.D + (4 * i + j) * CB, kr[kt][i]);
+            if (4 * i + 3 >= (NK == 4 ? 1 : 4 * NK - 11 + (NK == 5 ? 8 : 0)) && 4 * i + j >= nc) kr[kt][i][0] = kr[kt][i][1] = 0u;
+          } else {
+            load_chunk<KR>(in + (g + 8 * kt) * RB + ((4 * i + j) ^ pd_kswz<CE>(g)) * CB, kr[kt][i]);
+          }
+        }
       float S[2][4] = {};
       float dg[2][4] = {};
 #pragma unroll
@@ -403,8 +448,11 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
       for (int cx = 0; cx < NX; ++cx) {
         uint32_t xr[4][KR];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          load_chunk<KR>(in + (16 + 8 * (q >> 1) + 2 * j + (q & 1)) * RB + ((8 * cx + g) ^ pd_xswz<CE>(2 * j)) * CB, xr[q]);
+        for (int q = 0; q < 4; ++q) {
+          const int r = 8 * (q >> 1) + 2 * j + (q & 1);
+          if constexpr (MODE == kFlat) load_chunk<KR>(in + POOL + r * 2 * a.D + (8 * cx + g) * CB, xr[q]);
+          else load_chunk<KR>(in + POOL + r * RB + ((8 * cx + g) ^ pd_xswz<CE>(2 * j)) * CB, xr[q]);
+        }
 #pragma unroll
         for (int e = 0; e < CE; ++e) {
           const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
@@ -513,7 +561,7 @@ __global__ void __launch_bounds__(kPdThreads, 2) paged_decode_kernel(const __gri
 // One block per (sequence, kv head) and query row merges the item's segments and, in the
 // step, adds the new token.  Warp w takes the segments w, w + 8, ... (a row of 128 floats
 // is one 16-byte load per lane, all of them independent), then the warps join in order.
-constexpr int kPdMaxCtas = 1184, kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
 
 template <bool STEP>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedDecodeArgs a) {
@@ -675,41 +723,50 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   }
 }
 
-int paged_decode_ctas() {
+static int pd_sms() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
     cudaGetLastError();
     sms = 148;
   }
-  return std::min(2 * sms, kPdMaxCtas);
+  return sms;
 }
 
-template <bool STEP, bool R8, int CE, int NK, int NX, bool FULL>
-static cudaError_t launch_pd(const PagedDecodeArgs& a, cudaStream_t st) {
-  constexpr int smem = kPdWarps * kPdStages * 32 * pd_row_bytes<CE, NX>();
-  const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<STEP, R8, CE, NK, NX, FULL>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+// the most CTAs a tile pass runs with (workspace size)
+int paged_decode_ctas() { return 3 * pd_sms(); }
+
+template <bool STEP, bool R8, int CE, int NK, int NX, int MODE>
+static cudaError_t launch_pd(PagedDecodeArgs& a, cudaStream_t st) {
+  using Shape = PdShape<R8, CE, NK, NX, MODE>;
+  const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<STEP, R8, CE, NK, NX, MODE>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
   if (e != cudaSuccess) return e;
-  paged_decode_kernel<STEP, R8, CE, NK, NX, FULL><<<a.nctas, kPdThreads, smem, st>>>(a);
+  a.nctas = Shape::kCtas * pd_sms();
+  paged_decode_kernel<STEP, R8, CE, NK, NX, MODE><<<a.nctas, kPdThreads, Shape::kSmem, st>>>(a);
   return cudaGetLastError();
 }
 
 template <bool STEP, bool R8>
-static cudaError_t launch_pd_d(const PagedDecodeArgs& a, cudaStream_t st) {
-  const bool al16 = ((reinterpret_cast<uintptr_t>(a.k.p) | reinterpret_cast<uintptr_t>(a.x.p)) & 15u) == 0 &&
-                    ((a.k.sp | a.k.sh | a.k.sn | a.x.sp | a.x.sh | a.x.sn) & 7) == 0;
-  if (al16 && a.D % 8 == 0) {
-    if (a.D == 64) return launch_pd<STEP, R8, 8, 2, 1, true>(a, st);
-    if (a.D == 128) return launch_pd<STEP, R8, 8, 4, 2, true>(a, st);
-    if (a.D < 64) return launch_pd<STEP, R8, 8, 2, 1, false>(a, st);
-    return launch_pd<STEP, R8, 8, 4, 2, false>(a, st);
+static cudaError_t launch_pd_d(PagedDecodeArgs& a, cudaStream_t st) {
+  const bool base16 = ((reinterpret_cast<uintptr_t>(a.k.p) | reinterpret_cast<uintptr_t>(a.x.p)) & 15u) == 0 &&
+                      ((a.k.sp | a.k.sh | a.x.sp | a.x.sh) & 7) == 0;
+  if (base16 && ((a.k.sn | a.x.sn | a.D) & 7) == 0) {
+    if (a.D == 64) return launch_pd<STEP, R8, 8, 2, 1, kFull>(a, st);
+    if (a.D == 128) return launch_pd<STEP, R8, 8, 4, 2, kFull>(a, st);
+    if (a.D < 64) return launch_pd<STEP, R8, 8, 2, 1, kRows>(a, st);
+    return launch_pd<STEP, R8, 8, 4, 2, kRows>(a, st);
   }
-  if (a.D <= 64) return launch_pd<STEP, R8, 4, 4, 2, false>(a, st);
-  if (a.D <= 80) return launch_pd<STEP, R8, 4, 5, 3, false>(a, st);
-  return launch_pd<STEP, R8, 4, 8, 4, false>(a, st);
+  if (base16 && a.k.sn == a.D && a.x.sn == a.D && a.ps % 16 == 0) {  // D is an odd multiple of 4 here
+    if (a.D < 64) return launch_pd<STEP, R8, 4, 4, 2, kFlat>(a, st);
+    if (a.D < 80) return launch_pd<STEP, R8, 4, 5, 3, kFlat>(a, st);
+    return launch_pd<STEP, R8, 4, 8, 4, kFlat>(a, st);
+  }
+  if (a.D <= 64) return launch_pd<STEP, R8, 4, 4, 2, kRows>(a, st);
+  if (a.D <= 80) return launch_pd<STEP, R8, 4, 5, 3, kRows>(a, st);
+  return launch_pd<STEP, R8, 4, 8, 4, kRows>(a, st);
 }
 
-cudaError_t launch_paged_decode(const PagedDecodeArgs& a, bool step, cudaStream_t st) {
+cudaError_t launch_paged_decode(PagedDecodeArgs a, bool step, cudaStream_t st) {
   const int rows = std::min(a.gq, a.rows) + (step ? 1 : 0);
   cudaError_t e = step ? (rows <= 8 ? launch_pd_d<true, true>(a, st) : launch_pd_d<true, false>(a, st))
                        : (rows <= 8 ? launch_pd_d<false, true>(a, st) : launch_pd_d<false, false>(a, st));

@@ -57,7 +57,6 @@ int decode(bool step, int B, int Hq, int Hkv, int D, int P, int ps, int M, float
   a.B = B; a.H = Hkv; a.Hq = Hq; a.D = D; a.P = P; a.ps = ps; a.M = M;
   a.gq = Hq / Hkv;
   row_blocks(a.gq, step, &a.nblk, &a.rows);
-  a.nctas = paged_decode_ctas();
   a.s = scale; a.eps = eps;
   a.q = static_cast<const bf16*>(q); a.q_sb = q_sb; a.q_sh = q_sh;
   a.kn = static_cast<const bf16*>(kn); a.kn_sb = kn_sb; a.kn_sh = kn_sh;

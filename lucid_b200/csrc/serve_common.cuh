@@ -32,7 +32,7 @@ struct PoolView {
 struct PagedDecodeArgs {
   int B, H, Hq, D;             // sequences, kv heads, query heads, head dimension
   int P, ps, M;                // pool pages, page size, block table width
-  int gq, nblk, rows, nctas;   // query heads per kv head, row blocks of them, rows per block, CTAs
+  int gq, nblk, rows, nctas;   // query heads per kv head, row blocks of them, rows per block, CTAs (set by the launch)
   float s, eps;
   const bf16* q;  long long q_sb, q_sh;
   const bf16* kn; long long kn_sb, kn_sh;   // new keys (step only)
@@ -85,7 +85,7 @@ struct LogprobArgs {
   int* status;
 };
 
-cudaError_t launch_paged_decode(const PagedDecodeArgs& a, bool step, cudaStream_t st);
+cudaError_t launch_paged_decode(PagedDecodeArgs a, bool step, cudaStream_t st);
 cudaError_t launch_paged_append(const PagedAppendArgs& a, cudaStream_t st);
 cudaError_t launch_page_copy(const PageCopyArgs& a, cudaStream_t st);
 cudaError_t launch_logprobs_fwd(const LogprobArgs& a, int dtype, cudaStream_t st);
