@@ -498,7 +498,7 @@ int lucid_copy_pages(int layers, int P, int64_t page_bytes, void* k_pages, int64
  *   entropy[r]  = -sum p log p
  *   top_tokens / top_logprobs [R][top]: the most likely tokens, likeliest first, ties to
  *                 the lowest index; top at most LUCID_MAX_TOP and V
- *   stats [R][2]: for the backward
+ *   stats [R][2]: for the backward (NULL: not written)
  * Entries of -inf have probability 0.  A row without a distribution (all -inf, a NaN or
  * +inf) gives NaN, top tokens -1.
  * lucid_token_logprobs_bwd: dlogits [R][V] (contiguous, the logits' dtype) =

@@ -185,8 +185,10 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_fwd_kernel(const __grid_c
   const float nan = __int_as_float(0x7fc00000);
   if (tid == 0) {
     a.entropy[r] = ok ? kLn2 * (ll - W / L) : nan;
-    a.stats[2 * r] = ok ? M : nan;
-    a.stats[2 * r + 1] = ok ? ll : nan;
+    if (a.stats != nullptr) {
+      a.stats[2 * r] = ok ? M : nan;
+      a.stats[2 * r + 1] = ok ? ll : nan;
+    }
     if (a.tokens != nullptr) {
       const long long tok = a.tokens[r];
       float lp = 0.f;

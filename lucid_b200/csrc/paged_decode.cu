@@ -23,6 +23,7 @@
 #include "serve_common.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace lb {
 
@@ -723,11 +724,28 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   }
 }
 
-static int pd_sms() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+constexpr int kPdDevices = 64;  // devices whose attributes are remembered
+
+static int pd_device() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
-    sms = 148;
+    dev = kPdDevices;
+  }
+  return dev;
+}
+
+static int pd_sms() {
+  static std::atomic<int> known[kPdDevices];
+  const int dev = pd_device();
+  if (dev >= kPdDevices) return 148;
+  int sms = known[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+      cudaGetLastError();
+      return 148;
+    }
+    known[dev].store(sms, std::memory_order_relaxed);
   }
   return sms;
 }
@@ -738,9 +756,14 @@ int paged_decode_ctas() { return 3 * pd_sms(); }
 template <bool STEP, bool R8, int CE, int NK, int NX, int MODE>
 static cudaError_t launch_pd(PagedDecodeArgs& a, cudaStream_t st) {
   using Shape = PdShape<R8, CE, NK, NX, MODE>;
-  const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<STEP, R8, CE, NK, NX, MODE>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
-  if (e != cudaSuccess) return e;
+  static std::atomic<bool> sized[kPdDevices];  // shared memory granted on this device
+  const int dev = pd_device();
+  if (dev >= kPdDevices || !sized[dev].load(std::memory_order_relaxed)) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<STEP, R8, CE, NK, NX, MODE>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < kPdDevices) sized[dev].store(true, std::memory_order_relaxed);
+  }
   a.nctas = Shape::kCtas * pd_sms();
   paged_decode_kernel<STEP, R8, CE, NK, NX, MODE><<<a.nctas, kPdThreads, Shape::kSmem, st>>>(a);
   return cudaGetLastError();

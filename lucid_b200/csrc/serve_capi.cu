@@ -176,7 +176,7 @@ int lucid_token_logprobs(int64_t R0, int64_t R1, int V, int dtype, const void* l
                          float* top_logprobs, int64_t* top_tokens, int* status, void* stream) {
   if (!logprob_shape(R0, R1, V, dtype) || top < 0 || top > LUCID_MAX_TOP || top > V) return LUCID_ERR_SHAPE;
   if (R0 == 0 || R1 == 0) return LUCID_OK;
-  if (!ptr_ok(logits, dtype == 2 ? 4 : 2) || !ptr_ok(entropy, 4) || !ptr_ok(stats, 4) ||
+  if (!ptr_ok(logits, dtype == 2 ? 4 : 2) || !ptr_ok(entropy, 4) || (stats != nullptr && !ptr_ok(stats, 4)) ||
       (tokens != nullptr && (!ptr_ok(tokens, 8) || !ptr_ok(logprobs, 4))) ||
       (top > 0 && (!ptr_ok(top_logprobs, 4) || !ptr_ok(top_tokens, 8))))
     return LUCID_ERR_ALIGN;

@@ -7,7 +7,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .paged import _on, _stream
+from .paged import _on, _raw_stream
 
 __all__ = ["token_logprobs", "TokenLogprobs", "MAX_TOP"]
 
@@ -43,21 +43,22 @@ def _row_view(logits: torch.Tensor):
     return logits, r0, r1, s0, s1
 
 
-def _forward(logits, tokens, top):
+def _forward(logits, tokens, top, keep):
+    """The outputs, and with ``keep`` the rows' statistics for the backward."""
     lib = _lib.load()
-    dev, lead = logits.device, logits.shape[:-1]
+    index, lead = logits.get_device(), logits.shape[:-1]
     view, r0, r1, s0, s1 = _row_view(logits)
-    with _on(dev):
-        logprobs = torch.empty(lead, dtype=torch.float32, device=dev) if tokens is not None else None
-        entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-        stats = torch.empty(*lead, 2, dtype=torch.float32, device=dev)
-        top_lp = torch.empty(*lead, top, dtype=torch.float32, device=dev)
-        top_tok = torch.empty(*lead, top, dtype=torch.int64, device=dev)
+    entropy = logits.new_empty(lead, dtype=torch.float32)
+    logprobs = torch.empty_like(entropy) if tokens is not None else None
+    stats = entropy.new_empty((*lead, 2)) if keep else None
+    top_lp = entropy.new_empty((*lead, top))
+    top_tok = logits.new_empty((*lead, top), dtype=torch.int64)
+    with _on(index):
         rc = lib.lucid_token_logprobs(
             r0, r1, logits.shape[-1], _DTYPES[logits.dtype], view.data_ptr(), s0, s1,
             None if tokens is None else tokens.data_ptr(), top, None if tokens is None else logprobs.data_ptr(),
-            entropy.data_ptr(), stats.data_ptr(), top_lp.data_ptr(), top_tok.data_ptr(),
-            _lib.STATUS.device_word(dev.index), _stream())
+            entropy.data_ptr(), stats.data_ptr() if keep else None, top_lp.data_ptr(), top_tok.data_ptr(),
+            _lib.STATUS.device_word(index), _raw_stream(index))
     _lib.check(rc, "lucid_token_logprobs")
     return logprobs, entropy, top_lp, top_tok, stats
 
@@ -67,7 +68,7 @@ class TokenLogprobsFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, tokens, top: int):
-        logprobs, entropy, top_lp, top_tok, stats = _forward(logits, tokens, top)
+        logprobs, entropy, top_lp, top_tok, stats = _forward(logits, tokens, top, True)
         ctx.save_for_backward(logits, tokens, stats, entropy)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_lp, top_tok)
@@ -80,16 +81,16 @@ class TokenLogprobsFunction(torch.autograd.Function):
             return None, None, None
         lib = _lib.load()
         logits, tokens, stats, entropy = ctx.saved_tensors
-        dev = logits.device
+        index = logits.get_device()
         view, r0, r1, s0, s1 = _row_view(logits)
         gl, ge = (None if g is None else g.float().contiguous() for g in (g_logprobs, g_entropy))
-        with _on(dev):
-            dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        with _on(index):
             rc = lib.lucid_token_logprobs_bwd(
                 r0, r1, logits.shape[-1], _DTYPES[logits.dtype], view.data_ptr(), s0, s1,
                 None if tokens is None else tokens.data_ptr(), stats.data_ptr(), entropy.data_ptr(),
                 None if gl is None else gl.data_ptr(), None if ge is None else ge.data_ptr(), dlogits.data_ptr(),
-                _stream())
+                _raw_stream(index))
         _lib.check(rc, "lucid_token_logprobs_bwd")
         return dlogits, None, None
 
@@ -120,8 +121,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
                              f"{tuple(logits.shape)} on {logits.device}")
         if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
             raise TypeError(f"tokens: expected integers, got {tokens.dtype}")
-        tokens = tokens.to(torch.int64).contiguous()
+        if tokens.dtype != torch.int64 or not tokens.is_contiguous():
+            tokens = tokens.to(torch.int64).contiguous()
     _lib.STATUS.poll()
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*TokenLogprobsFunction.apply(logits, tokens, top))
-    return TokenLogprobs(*_forward(logits, tokens, top)[:4])
+    return TokenLogprobs(*_forward(logits, tokens, top, False)[:4])

@@ -32,43 +32,45 @@ from ._lib import LucidError
 __all__ = ["paged_decode_step", "paged_decode_attention", "paged_append", "copy_pages", "PagedCache", "PagedBatch"]
 
 _NO_GUARD = contextlib.nullcontext()
+_BF16, _INT32 = torch.bfloat16, torch.int32
+_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(i).cuda_stream without building a Stream
 
 
-def _on(device: torch.device):
-    """Context in which ``device`` is the current one."""
-    return _NO_GUARD if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+def _on(index: int):
+    """Context in which device ``index`` is the current one."""
+    return _NO_GUARD if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def _rows(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
     """A bf16 CUDA operand of the given shape, copied if its rows are not 8-byte aligned."""
-    if not t.is_cuda:
-        raise RuntimeError(f"{name}: LUCID B200 kernels need CUDA tensors (no CPU fallback)")
-    if t.dtype != torch.bfloat16:
-        raise TypeError(f"{name}: expected bfloat16, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.device != device:
+    if t.dtype != _BF16 or t.shape != shape or t.device != device:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name}: LUCID B200 kernels need CUDA tensors (no CPU fallback)")
+        if t.dtype != _BF16:
+            raise TypeError(f"{name}: expected bfloat16, got {t.dtype}")
+        if t.shape != shape:
+            raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
         raise ValueError(f"{name} is on {t.device}, the pool on {device}")
-    s = t.stride()
-    ok = s[3] == 1 and (s[0] | s[1] | s[2]) % 4 == 0 and t.data_ptr() % 8 == 0
-    return t if ok else t.clone(memory_format=torch.contiguous_format)  # contiguous() keeps an odd start
+    s0, s1, s2, s3 = t.stride()
+    if s3 == 1 and (s0 | s1 | s2 | t.data_ptr() >> 1) & 3 == 0:
+        return t
+    return t.detach().clone(memory_format=torch.contiguous_format)  # contiguous() keeps an odd start
 
 
-def _pools(key_pages: torch.Tensor, x_pages: torch.Tensor, dims: int = 4):
+def _pools(key_pages: torch.Tensor, x_pages: torch.Tensor, dims: int = 4) -> None:
     """The pools as they are: never copied, so what the kernels cannot address is refused."""
     for t, name in ((key_pages, "key_pages"), (x_pages, "x_pages")):
         if not t.is_cuda:
             raise RuntimeError(f"{name}: LUCID B200 kernels need CUDA tensors (no CPU fallback)")
-        if t.dtype != torch.bfloat16:
+        if t.dtype != _BF16:
             raise TypeError(f"{name}: expected bfloat16, got {t.dtype}")
-        if t.dim() != dims:
-            raise ValueError(f"{name}: expected a {dims}-D pool, got shape {tuple(t.shape)}")
         s = t.stride()
-        if s[-1] != 1 or t.data_ptr() % 8 or any(st % 4 or st == 0 and n > 1 for st, n in zip(s[:-1], t.shape[:-1])):
+        if len(s) != dims:
+            raise ValueError(f"{name}: expected a {dims}-D pool, got shape {tuple(t.shape)}")
+        low = s[0]
+        for st in s[:-1]:
+            low |= st
+        if s[-1] != 1 or (low | t.data_ptr() >> 1) & 3 or (0 in s and any(st == 0 and n > 1 for st, n in zip(s, t.shape))):
             raise ValueError(f"{name}: needs a unit innermost stride, the others nonzero multiples of 4 elements, "
                              f"and an 8-byte aligned base; got strides {s}")
     if x_pages.shape != key_pages.shape or x_pages.device != key_pages.device:
@@ -77,21 +79,24 @@ def _pools(key_pages: torch.Tensor, x_pages: torch.Tensor, dims: int = 4):
 
 
 def _index(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name}: expected int32, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the pool on {device}")
-    if t.dim() != len(shape) or any(want is not None and n != want for n, want in zip(t.shape, shape)):
-        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    """An int32 table or vector on the pool's device; None in ``shape`` is any size."""
+    s = t.shape
+    if t.dtype != _INT32 or t.device != device or len(s) != len(shape) or s[0] != shape[0] or t.stride(-1) != 1 and s[-1] > 1:
+        if t.dtype != _INT32:
+            raise TypeError(f"{name}: expected int32, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the pool on {device}")
+        if len(s) != len(shape) or s[0] != shape[0]:
+            raise ValueError(f"{name}: expected shape {shape}, got {tuple(s)}")
         raise ValueError(f"{name}: needs a unit innermost stride")
     return t
 
 
-def _table(block_table, lengths, B, device):
-    _index(block_table, "block_table", (B, None), device)
-    _index(lengths, "lengths", (B,), device)
-    return block_table.data_ptr(), block_table.stride(0), lengths.data_ptr()
+def _one_token(query: torch.Tensor):
+    s = query.shape
+    if len(s) != 4 or s[2] != 1:
+        raise ValueError(f"query: expected [B, Hq, 1, D] (one new token), got {tuple(s)}")
+    return s[0], s[1]
 
 
 def paged_decode_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor,
@@ -108,24 +113,25 @@ def paged_decode_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     _lib.STATUS.poll()
     _pools(key_pages, x_pages)
     P, Hkv, ps, D = key_pages.shape
-    dev = key_pages.device
-    if query.dim() != 4 or query.shape[2] != 1:
-        raise ValueError(f"query: expected [B, Hq, 1, D] (one new token), got {tuple(query.shape)}")
-    B, Hq = query.shape[0], query.shape[1]
+    dev, index = key_pages.device, key_pages.get_device()
+    B, Hq = _one_token(query)
     query = _rows(query, "query", (B, Hq, 1, D), dev)
     key = _rows(key, "key", (B, Hkv, 1, D), dev)
     value = _rows(value, "value", (B, Hkv, 1, D), dev)
-    tab, t_sb, lens = _table(block_table, lengths, B, dev)
-    with _on(dev):
-        x_new = torch.empty(B, Hkv, 1, D, dtype=torch.bfloat16, device=dev)
-        o = torch.empty(B, 1, Hq, D, dtype=torch.bfloat16, device=dev)
-        ws = torch.empty(lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 1), dtype=torch.uint8, device=dev)
+    _index(block_table, "block_table", (B, None), dev)
+    _index(lengths, "lengths", (B,), dev)
+    (q0, q1, _, _), (k0, k1, _, _), (v0, v1, _, _) = query.stride(), key.stride(), value.stride()
+    (kp0, kp1, kp2, _), (xp0, xp1, xp2, _) = key_pages.stride(), x_pages.stride()
+    x_new = key_pages.new_empty((B, Hkv, 1, D))
+    o = key_pages.new_empty((B, 1, Hq, D))
+    nbytes = lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 1)
+    ws = lengths.new_empty(nbytes + 3 >> 2)
+    with _on(index):
         rc = lib.lucid_paged_decode_step(
-            B, Hq, Hkv, D, P, ps, block_table.shape[1], scale, eps, query.data_ptr(), query.stride(0), query.stride(1),
-            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
-            key_pages.data_ptr(), *key_pages.stride()[:3], x_pages.data_ptr(), *x_pages.stride()[:3], tab, t_sb, lens,
-            x_new.data_ptr(), Hkv * D, D, o.data_ptr(), Hq * D, D, 1 if append else 0,
-            _lib.STATUS.device_word(dev.index), ws.data_ptr(), ws.numel(), _stream())
+            B, Hq, Hkv, D, P, ps, block_table.shape[1], scale, eps, query.data_ptr(), q0, q1, key.data_ptr(), k0, k1,
+            value.data_ptr(), v0, v1, key_pages.data_ptr(), kp0, kp1, kp2, x_pages.data_ptr(), xp0, xp1, xp2,
+            block_table.data_ptr(), block_table.stride(0), lengths.data_ptr(), x_new.data_ptr(), Hkv * D, D,
+            o.data_ptr(), Hq * D, D, append, _lib.STATUS.device_word(index), ws.data_ptr(), nbytes, _raw_stream(index))
     _lib.check(rc, "lucid_paged_decode_step")
     return o, x_new
 
@@ -139,19 +145,21 @@ def paged_decode_attention(query: torch.Tensor, key_pages: torch.Tensor, x_pages
     _lib.STATUS.poll()
     _pools(key_pages, x_pages)
     P, Hkv, ps, D = key_pages.shape
-    dev = key_pages.device
-    if query.dim() != 4 or query.shape[2] != 1:
-        raise ValueError(f"query: expected [B, Hq, 1, D] (one new token), got {tuple(query.shape)}")
-    B, Hq = query.shape[0], query.shape[1]
+    dev, index = key_pages.device, key_pages.get_device()
+    B, Hq = _one_token(query)
     query = _rows(query, "query", (B, Hq, 1, D), dev)
-    tab, t_sb, lens = _table(block_table, lengths, B, dev)
-    with _on(dev):
-        o = torch.empty(B, 1, Hq, D, dtype=torch.bfloat16, device=dev)
-        ws = torch.empty(lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 0), dtype=torch.uint8, device=dev)
+    _index(block_table, "block_table", (B, None), dev)
+    _index(lengths, "lengths", (B,), dev)
+    q0, q1, _, _ = query.stride()
+    (kp0, kp1, kp2, _), (xp0, xp1, xp2, _) = key_pages.stride(), x_pages.stride()
+    o = key_pages.new_empty((B, 1, Hq, D))
+    nbytes = lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 0)
+    ws = lengths.new_empty(nbytes + 3 >> 2)
+    with _on(index):
         rc = lib.lucid_paged_decode_attn(
-            B, Hq, Hkv, D, P, ps, block_table.shape[1], scale, query.data_ptr(), query.stride(0), query.stride(1),
-            key_pages.data_ptr(), *key_pages.stride()[:3], x_pages.data_ptr(), *x_pages.stride()[:3], tab, t_sb, lens,
-            o.data_ptr(), Hq * D, D, _lib.STATUS.device_word(dev.index), ws.data_ptr(), ws.numel(), _stream())
+            B, Hq, Hkv, D, P, ps, block_table.shape[1], scale, query.data_ptr(), q0, q1, key_pages.data_ptr(), kp0, kp1,
+            kp2, x_pages.data_ptr(), xp0, xp1, xp2, block_table.data_ptr(), block_table.stride(0), lengths.data_ptr(),
+            o.data_ptr(), Hq * D, D, _lib.STATUS.device_word(index), ws.data_ptr(), nbytes, _raw_stream(index))
     _lib.check(rc, "lucid_paged_decode_attn")
     return o
 
@@ -166,20 +174,24 @@ def paged_append(key: torch.Tensor, x: torch.Tensor, key_pages: torch.Tensor, x_
     _lib.STATUS.poll()
     _pools(key_pages, x_pages)
     P, Hkv, ps, D = key_pages.shape
-    dev = key_pages.device
+    dev, index = key_pages.device, key_pages.get_device()
     if key.dim() != 4:
         raise ValueError(f"key: expected [B, Hkv, N, D], got {tuple(key.shape)}")
-    B, N = key.shape[0], key.shape[2]
-    key = _rows(key.detach(), "key", (B, Hkv, N, D), dev)
-    x = _rows(x.detach(), "x", (B, Hkv, N, D), dev)
-    tab, t_sb, lens = _table(block_table, lengths, B, dev)
+    B, _, N, _ = key.shape
+    key = _rows(key, "key", (B, Hkv, N, D), dev)
+    x = _rows(x, "x", (B, Hkv, N, D), dev)
+    _index(block_table, "block_table", (B, None), dev)
+    _index(lengths, "lengths", (B,), dev)
     if counts is not None:
         _index(counts, "counts", (B,), dev)
-    with _on(dev):
+    (k0, k1, k2, _), (x0, x1, x2, _) = key.stride(), x.stride()
+    (kp0, kp1, kp2, _), (xp0, xp1, xp2, _) = key_pages.stride(), x_pages.stride()
+    with _on(index):
         rc = lib.lucid_paged_append(
-            B, Hkv, N, D, P, ps, block_table.shape[1], key.data_ptr(), *key.stride()[:3], x.data_ptr(), *x.stride()[:3],
-            key_pages.data_ptr(), *key_pages.stride()[:3], x_pages.data_ptr(), *x_pages.stride()[:3], tab, t_sb, lens,
-            None if counts is None else counts.data_ptr(), _lib.STATUS.device_word(dev.index), _stream())
+            B, Hkv, N, D, P, ps, block_table.shape[1], key.data_ptr(), k0, k1, k2, x.data_ptr(), x0, x1, x2,
+            key_pages.data_ptr(), kp0, kp1, kp2, x_pages.data_ptr(), xp0, xp1, xp2, block_table.data_ptr(),
+            block_table.stride(0), lengths.data_ptr(), None if counts is None else counts.data_ptr(),
+            _lib.STATUS.device_word(index), _raw_stream(index))
     _lib.check(rc, "lucid_paged_append")
 
 
@@ -212,20 +224,21 @@ def copy_pages(key_pages: torch.Tensor, x_pages: torch.Tensor, src, dst) -> None
     strides = []
     for t, name in ((key_pages, "key_pages"), (x_pages, "x_pages")):
         s = t.stride()
-        inner = sorted((st, size) for st, size in zip(s[-3:], shape[-3:]) if size > 1)
-        span = 1
-        for st, size in inner:
-            if st != span:
-                raise ValueError(f"{name}: the pages' [Hkv, page_size, D] blocks must be dense, got strides {s}")
-            span *= size
+        if s[-3:] != (shape[-2] * shape[-1], shape[-1], 1):   # the usual order; any other dense one will do
+            span = 1
+            for st, size in sorted((st, size) for st, size in zip(s[-3:], shape[-3:]) if size > 1):
+                if st != span:
+                    raise ValueError(f"{name}: the pages' [Hkv, page_size, D] blocks must be dense, got strides {s}")
+                span *= size
         strides.append((2 * s[0] if len(shape) == 5 else 0, 2 * s[-4]))
     if len(src) == 0 or layers == 0 or n == 0:
         return
     if n % 4:
         raise ValueError(f"a page of {n} elements is not a multiple of 8 bytes")
-    with _on(key_pages.device):
+    index = key_pages.get_device()
+    with _on(index):
         rc = lib.lucid_copy_pages(layers, P, 2 * n, key_pages.data_ptr(), *strides[0], x_pages.data_ptr(), *strides[1],
-                                  src.buffer_info()[0], dst.buffer_info()[0], len(src), _stream())
+                                  src.buffer_info()[0], dst.buffer_info()[0], len(src), _raw_stream(index))
     if rc == 1:
         raise ValueError(f"copy_pages: pages must lie in [0, {P}), each dst named once and none of them a src")
     _lib.check(rc, "lucid_copy_pages")
