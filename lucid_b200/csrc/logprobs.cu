@@ -19,63 +19,165 @@
 #include "serve_common.cuh"
 
 #include <algorithm>
+#include <atomic>
+#include <climits>
 
 namespace lb {
 
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32;
-constexpr int kLpGroups = 128;   // groups of 4 threads
+constexpr int kLpThreads = 512;  // backward
+constexpr int kLpGroups = 128;   // groups of threads
 constexpr int kLpCap = 512;      // list of elements above T, and of those equal to it
+constexpr int kLpHold = 8;       // vectors a thread holds: 32768 bf16 logits in 512 threads
+constexpr int kLpBwdHold = 4;
 constexpr float kLpFloor = -200.f;  // 2^-200 is 0 in fp32; keeps 0 * -inf out of w
-
-template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f32<bf16>(bf16 v) { return __bfloat162float(v); }
-template <>
-__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ bf16 from_f32<bf16>(float v) { return __float2bfloat16(v); }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half(v); }
-
-// a row as 16-byte vectors from the 16-byte boundary at or below its start: vector v
-// holds the elements [v VE - shift, +VE); the first and last may be partial
-template <typename T>
-struct RowView {
-  static constexpr int VE = 16 / (int)sizeof(T);
-  const T* row;
-  int V, shift, nvec;
-  __device__ RowView(const T* r, int n) : row(r), V(n) {
-    shift = (int)((reinterpret_cast<uintptr_t>(r) & 15u) / sizeof(T));
-    nvec = (int)(((long long)shift + n + VE - 1) / VE);
-  }
-  __device__ __forceinline__ int first(int v) const { return (int)((long long)v * VE - shift); }
-  __device__ __forceinline__ void load(int v, float (&x)[VE]) const {
-    const int e0 = first(v);
-    if (e0 >= 0 && e0 <= V - VE) {
-      const uint4 u = *reinterpret_cast<const uint4*>(row + e0);
-      const T* p = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) x[i] = to_f32<T>(p[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) x[i] = e0 + i >= 0 && e0 + i < V ? to_f32<T>(row[e0 + i]) : -INFINITY;
-    }
-  }
-};
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// 2^v, flushed to zero below 2^-126
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
+// two fp32 values side by side: one instruction for both
+struct Pair {
+  unsigned long long v;
+};
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 halves(Pair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// A type's 16-byte vector: its VE values as VE / 2 pairs, their maximum (NaN if there is
+// one), the bits of -inf, and the way back from pairs.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<bf16> {
+  static constexpr int VE = 8;
+  static constexpr uint32_t kNegInf = 0xff80ff80u;
+  static __device__ __forceinline__ float value(bf16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ Pair get(const uint4& u, int i) {
+    const uint32_t w = (&u.x)[i];
+    return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float top(uint32_t w) {
+    return max_nan(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t put(Pair p) {
+    const float2 f = halves(p);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ bf16 from(float v) { return __float2bfloat16(v); }
+};
+template <>
+struct Vec<__half> {
+  static constexpr int VE = 8;
+  static constexpr uint32_t kNegInf = 0xfc00fc00u;
+  static __device__ __forceinline__ float value(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ Pair get(const uint4& u, int i) {
+    const uint32_t w = (&u.x)[i];
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return pair(f.x, f.y);
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  static __device__ __forceinline__ float top(uint32_t w) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return max_nan(f.x, f.y);
+  }
+  static __device__ __forceinline__ uint32_t put(Pair p) {
+    const float2 f = halves(p);
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ __half from(float v) { return __float2half(v); }
+};
+template <>
+struct Vec<float> {
+  static constexpr int VE = 4;
+  static constexpr uint32_t kNegInf = 0xff800000u;
+  static __device__ __forceinline__ float value(float v) { return v; }
+  static __device__ __forceinline__ Pair get(const uint4& u, int i) {
+    return pair(__uint_as_float((&u.x)[2 * i]), __uint_as_float((&u.x)[2 * i + 1]));
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float top(uint32_t w) { return __uint_as_float(w); }
+  static __device__ __forceinline__ float from(float v) { return v; }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t vec_max(const uint4& u) {
+  return Vec<T>::max2(Vec<T>::max2(u.x, u.y), Vec<T>::max2(u.z, u.w));
+}
+
+// a row as 16-byte vectors from the 16-byte boundary at or below its start: vector v
+// holds the elements [v VE - shift, +VE); the first and last may be partial
+template <typename T>
+struct RowView {
+  static constexpr int VE = Vec<T>::VE;
+  const T* row;
+  int V, shift, nvec;
+  __device__ RowView(const T* r, int n) : row(r), V(n) {
+    shift = (int)((reinterpret_cast<uintptr_t>(r) & 15u) / sizeof(T));
+    nvec = (shift + n + VE - 1) / VE;
+  }
+  __device__ __forceinline__ int first(int v) const { return v * VE - shift; }
+  // whether the vector that starts at element e0 lies inside the row
+  __device__ __forceinline__ bool whole(int e0) const { return (unsigned)e0 < (unsigned)max(V - VE + 1, 0); }
+  // the bits of vector v; places outside the row hold -inf
+  __device__ __forceinline__ uint4 bits(int v) const {
+    const int e0 = first(v);
+    if (whole(e0)) return *reinterpret_cast<const uint4*>(row + e0);
+    uint4 u = make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
+    T* p = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      if (e0 + i >= 0 && e0 + i < V) p[i] = row[e0 + i];
+    return u;
+  }
+};
+
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
 __device__ __forceinline__ float warp_sum_f(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -91,149 +193,199 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 
+template <int NT>
 struct LpShared {
-  float gmax[kLpGroups];
-  float wm[kLpWarps], wl[kLpWarps], ww[kLpWarps];
-  float T;
-  int na, nb, need;
+  __align__(16) float gmax[kLpGroups];
+  float wm[NT / 32], wl[NT / 32], ww[NT / 32];
+  float T, M, ln;
+  int nh, na, nb;
+  int hit[kLpCap];                 // vectors with an element at or above T
   float av[kLpCap];
   int ai[kLpCap], bi[kLpCap];
   int hist[256];
   uint32_t prefix;
   int remain;
-  int wcount[kLpWarps];
+  int wcount[NT / 32];
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) logprobs_fwd_kernel(const __grid_constant__ LogprobArgs a) {
-  __shared__ LpShared sh;
-  constexpr int VE = RowView<T>::VE;
+// Blocks stay for many rows.  While a block works on the 8 vectors that each thread holds
+// in registers, cp.async brings the thread's next 8 (of this row or the next) into its
+// own places in shared memory, so loads never wait for the joins.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __grid_constant__ LogprobArgs a) {
+  __shared__ LpShared<NT> sh;
+  extern __shared__ uint4 next[];  // [kLpHold][NT]
+  constexpr int VE = RowView<T>::VE, kWarps = NT / 32, kBatch = kLpHold * NT;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long r = blockIdx.x;
-  const RowView<T> row(static_cast<const T*>(a.logits) + (r / a.R1) * a.s0 + (r % a.R1) * a.s1, a.V);
-  // ---- one pass: maximum, sum, entropy sum ----
-  float mx = -INFINITY, l = 0.f, w = 0.f;
-  for (int v = tid; v < row.nvec; v += kLpThreads) {
-    float x[VE];
-    row.load(v, x);
-    float vm = x[0];
+  const unsigned R = (unsigned)(a.R0 * a.R1), R1 = (unsigned)a.R1;
+  auto row_of = [&](unsigned r) {
+    const unsigned r0 = a.R0 == 1 ? 0 : r / R1;
+    return RowView<T>(static_cast<const T*>(a.logits) + (long long)r0 * a.s0 + (long long)(r - r0 * R1) * a.s1, a.V);
+  };
+  const uint32_t own = (uint32_t)__cvta_generic_to_shared(&next[tid]);
+  auto fetch = [&](const RowView<T>& row, int v0) {  // this thread's vectors of the batch at v0
+    const int e0 = row.first(v0 + tid);
+    const T* from = row.row + e0;
 #pragma unroll
-    for (int i = 1; i < VE; ++i) vm = max_nan(vm, x[i]);
+    for (int u = 0; u < kLpHold; ++u) {
+      if (row.whole(e0 + u * NT * VE))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(own + u * NT * 16), "l"(from + u * NT * VE) : "memory");
+      else
+        next[u * NT + tid] = row.bits(v0 + u * NT + tid);  // partly or wholly outside: -inf there
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  RowView<T> row = row_of(blockIdx.x);
+  fetch(row, 0);
+  for (unsigned r = blockIdx.x; r < R; r += gridDim.x) {
+  // ---- one pass: maximum, sum, entropy sum; 8 vectors a thread at a time ----
+  RowView<T> after = row;
+  uint4 raw[kLpHold];
+  float mx = -INFINITY;
+  Pair l2 = pair(0.f, 0.f), w2 = l2;
+  for (int v0 = 0; v0 < row.nvec; v0 += kBatch) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < kLpHold; ++u) raw[u] = next[u * NT + tid];
+    if (v0 + kBatch < row.nvec) {
+      fetch(row, v0 + kBatch);
+    } else if (r + gridDim.x < R) {
+      after = row_of(r + gridDim.x);
+      fetch(after, 0);
+    }
+    uint32_t best = vec_max<T>(raw[0]);
+#pragma unroll
+    for (int u = 1; u < kLpHold; ++u) best = Vec<T>::max2(best, vec_max<T>(raw[u]));
+    const float vm = Vec<T>::top(best);
     if (!(vm <= mx)) {            // larger, or NaN
       const float mn = max_nan(mx, vm);
-      if (l > 0.f) {
-        const float d = fmaxf((mx - mn) * kLog2e, kLpFloor), f = exp2f(d);
-        w = f * (w + d * l);
-        l *= f;
-      }
+      const float d = fmaxf((mx - mn) * kLog2e, kLpFloor), f = ex2(d);  // nothing yet: f = 0
+      w2 = mul2(pair(f, f), fma2(pair(d, d), l2, w2));
+      l2 = mul2(pair(f, f), l2);
       mx = mn;
     }
     if (vm == -INFINITY) continue;  // nothing to add (and mx may not be finite yet)
+    const Pair nm = pair(-mx, -mx), le = pair(kLog2e, kLog2e);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const float t = fmaxf((x[i] - mx) * kLog2e, kLpFloor);
-      const float p = exp2f(t);
-      l += p;
-      w = fmaf(p, t, w);
-    }
-  }
-  // ---- join the block ----
-  float bm = mx;
-  float gm = bm;
+    for (int u = 0; u < kLpHold; ++u)
+      if (v0 + u * NT < row.nvec) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    bm = max_nan(bm, __shfl_xor_sync(0xffffffffu, bm, o));
-    if (o == 2) gm = bm;          // 4 lanes
-  }
-  if ((lane & 3) == 0) sh.gmax[tid >> 2] = gm;
-  if (lane == 0) sh.wm[warp] = bm;
-  if (tid == 0) sh.na = sh.nb = 0;
-  __syncthreads();
-  float M = sh.wm[0];
-#pragma unroll
-  for (int i = 1; i < kLpWarps; ++i) M = max_nan(M, sh.wm[i]);
-  const bool ok = fabsf(M) < INFINITY;  // else no distribution: all -inf, a NaN or +inf
-  float lj = 0.f, wj = 0.f;
-  if (l > 0.f) {
-    const float d = fmaxf((mx - M) * kLog2e, kLpFloor), f = exp2f(d);
-    lj = l * f;
-    wj = f * (w + d * l);
-  }
-  lj = warp_sum_f(lj);
-  wj = warp_sum_f(wj);
-  if (lane == 0) {
-    sh.wl[warp] = lj;
-    sh.ww[warp] = wj;
-  }
-  if (a.top > 0 && ok && tid < kLpGroups) {  // the top-th largest of the group maxima
-    const float v = sh.gmax[tid];
-    int rank = 0;
-    for (int i = 0; i < kLpGroups; ++i) {
-      const float o = sh.gmax[i];
-      rank += o > v || (o == v && i < tid);
-    }
-    if (rank == a.top - 1) sh.T = v;
-  }
-  __syncthreads();
-  float L = 0.f, W = 0.f;
-#pragma unroll
-  for (int i = 0; i < kLpWarps; ++i) {
-    L += sh.wl[i];
-    W += sh.ww[i];
-  }
-  const float ll = log2f(L), ln = logf(L);
-  const float nan = __int_as_float(0x7fc00000);
-  if (tid == 0) {
-    a.entropy[r] = ok ? kLn2 * (ll - W / L) : nan;
-    if (a.stats != nullptr) {
-      a.stats[2 * r] = ok ? M : nan;
-      a.stats[2 * r + 1] = ok ? ll : nan;
-    }
-    if (a.tokens != nullptr) {
-      const long long tok = a.tokens[r];
-      float lp = 0.f;
-      if (tok >= 0 && tok < a.V) lp = ok ? (to_f32<T>(row.row[tok]) - M) - ln : nan;
-      else if (tok != -100) {
-        report(a.status, kStatusToken, kTagLogprobs);
-        lp = nan;
-      }
-      a.logprobs[r] = lp;
-    }
-  }
-  if (a.top == 0) return;
-  if (!ok) {
-    for (int i = tid; i < a.top; i += kLpThreads) {
-      a.top_lp[r * a.top + i] = nan;
-      a.top_tok[r * a.top + i] = -1;
-    }
-    return;
-  }
-  // ---- the top best ----
-  float thr = sh.T;
-  auto collect = [&](float t) {
-    for (int v = tid; v < row.nvec; v += kLpThreads) {
-      float x[VE];
-      row.load(v, x);
-      float vm = x[0];
-#pragma unroll
-      for (int i = 1; i < VE; ++i) vm = fmaxf(vm, x[i]);
-      if (vm < t) continue;
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const int e = row.first(v) + i;
-        if (x[i] >= t && e >= 0 && e < a.V) {
-          if (x[i] > t) {
-            const int at = atomicAdd(&sh.na, 1);
-            if (at < kLpCap) {
-              sh.av[at] = x[i];
-              sh.ai[at] = e;
-            }
-          } else {
-            const int at = atomicAdd(&sh.nb, 1);
-            if (at < kLpCap) sh.bi[at] = e;
-          }
+        for (int i = 0; i < VE / 2; ++i) {
+          const float2 t = halves(mul2(add2(Vec<T>::get(raw[u], i), nm), le));
+          const float tx = fmaxf(t.x, kLpFloor), ty = fmaxf(t.y, kLpFloor);
+          const Pair p = pair(ex2(tx), ex2(ty));
+          l2 = add2(l2, p);
+          w2 = fma2(p, pair(tx, ty), w2);
         }
       }
+  }
+  const float l = halves(l2).x + halves(l2).y, w = halves(w2).x + halves(w2).y;
+  // ---- join the block: warps by shuffles, the rest by the first warp ----
+  if (a.top > 0) {
+    float gm = mx;
+#pragma unroll
+    for (int o = 1; o < NT / kLpGroups; o <<= 1) gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+    if (tid % (NT / kLpGroups) == 0) sh.gmax[tid / (NT / kLpGroups)] = gm;
+    if (tid == 0) sh.nh = sh.na = sh.nb = 0;
+  }
+  {
+    const float wmx = warp_max_nan(mx);
+    const float d = fmaxf((mx - wmx) * kLog2e, kLpFloor), f = ex2(d);  // a thread without elements: l = w = 0
+    const float wl = warp_sum_f(l * f), ww = warp_sum_f(f * fmaf(d, l, w));
+    if (lane == 0) {
+      sh.wm[warp] = wmx;
+      sh.wl[warp] = wl;
+      sh.ww[warp] = ww;
+    }
+  }
+  __syncthreads();
+  const float nan = __int_as_float(0x7fc00000);
+  if (warp == 0) {
+    const float m = lane < kWarps ? sh.wm[lane] : -INFINITY;
+    const float M = warp_max_nan(m);
+    const bool ok = fabsf(M) < INFINITY;  // else no distribution: all -inf, a NaN or +inf
+    const float d = fmaxf((m - M) * kLog2e, kLpFloor), f = ex2(d);
+    const float l0 = lane < kWarps ? sh.wl[lane] : 0.f, w0 = lane < kWarps ? sh.ww[lane] : 0.f;
+    const float L = warp_sum_f(l0 * f), W = warp_sum_f(f * fmaf(d, l0, w0));
+    const float ll = log2f(L), ln = logf(L);
+    if (lane == 0) {
+      sh.M = ok ? M : nan;
+      sh.ln = ln;
+      a.entropy[r] = ok ? kLn2 * (ll - W / L) : nan;
+      if (a.stats != nullptr) {
+        a.stats[2 * (long long)r] = ok ? M : nan;
+        a.stats[2 * (long long)r + 1] = ok ? ll : nan;
+      }
+      if (a.tokens != nullptr) {
+        const long long tok = a.tokens[r];
+        float lp = 0.f;
+        if (tok >= 0 && tok < a.V) lp = ok ? (Vec<T>::value(row.row[tok]) - M) - ln : nan;
+        else if (tok != -100) {
+          report(a.status, kStatusToken, kTagLogprobs);
+          lp = nan;
+        }
+        a.logprobs[r] = lp;
+      }
+    }
+  }
+  if (a.top > 0) {  // the top-th largest of the group maxima: NT / 128 threads rank each
+    constexpr int kTeam = NT / kLpGroups;
+    const int me = tid / kTeam;
+    const float v = sh.gmax[me];
+    int rank = 0;
+#pragma unroll 8
+    for (int q = tid % kTeam; q < kLpGroups / 4; q += kTeam) {
+      const float4 o = *reinterpret_cast<const float4*>(&sh.gmax[4 * q]);
+      rank += (o.x > v || (o.x == v && 4 * q < me)) + (o.y > v || (o.y == v && 4 * q + 1 < me)) +
+              (o.z > v || (o.z == v && 4 * q + 2 < me)) + (o.w > v || (o.w == v && 4 * q + 3 < me));
+    }
+#pragma unroll
+    for (int o = 1; o < kTeam; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (rank == a.top - 1) sh.T = v;
+    __syncthreads();
+  }
+  const float M = sh.M, ln = sh.ln;  // top > 0 only
+  if (a.top > 0 && !(fabsf(M) < INFINITY)) {
+    for (int i = tid; i < a.top; i += NT) {
+      a.top_lp[(long long)r * a.top + i] = nan;
+      a.top_tok[(long long)r * a.top + i] = -1;
+    }
+  } else if (a.top > 0) {
+  // ---- the top best ----
+  float thr = sh.T;
+  auto put = [&](float x, int e, float t) {
+    if (x > t) {
+      const int at = atomicAdd(&sh.na, 1);
+      if (at < kLpCap) {
+        sh.av[at] = x;
+        sh.ai[at] = e;
+      }
+    } else if (x == t) {
+      const int at = atomicAdd(&sh.nb, 1);
+      if (at < kLpCap) sh.bi[at] = e;
+    }
+  };
+  auto collect = [&](float t) {
+    auto look = [&](const uint4& x, int v) {
+      if (Vec<T>::top(vec_max<T>(x)) >= t) {
+        const int at = atomicAdd(&sh.nh, 1);
+        if (at < kLpCap) sh.hit[at] = v;
+      }
+    };
+    if (row.nvec <= kBatch) {      // the row is still in registers
+#pragma unroll
+      for (int u = 0; u < kLpHold; ++u)
+        if (u * NT + tid < row.nvec) look(raw[u], u * NT + tid);
+    } else {
+      for (int v = tid; v < row.nvec; v += NT) look(row.bits(v), v);
+    }
+    __syncthreads();
+    const int nh = sh.nh;
+    // the elements of the few vectors that hold any, or of all
+    const long long some = (long long)(nh <= kLpCap ? nh : row.nvec) * VE;
+    for (long long i = tid; i < some; i += NT) {
+      const int e = row.first(nh <= kLpCap ? sh.hit[i / VE] : (int)(i / VE)) + (int)(i % VE);
+      if (e >= 0 && e < a.V) put(Vec<T>::value(row.row[e]), e, t);
     }
     __syncthreads();
   };
@@ -245,16 +397,16 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_fwd_kernel(const __grid_c
     }
     for (int byte = 3; byte >= 0; --byte) {
       __syncthreads();
-      if (tid < 256) sh.hist[tid] = 0;
+      for (int i = tid; i < 256; i += NT) sh.hist[i] = 0;
       __syncthreads();
       const uint32_t pre = sh.prefix;
-      for (int v = tid; v < row.nvec; v += kLpThreads) {
-        float x[VE];
-        row.load(v, x);
+      for (int v = tid; v < row.nvec; v += NT) {
+        const uint4 x = row.bits(v);
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
           const int e = row.first(v) + i;
-          const uint32_t key = order_key(x[i]);
+          const float2 f = halves(Vec<T>::get(x, i / 2));
+          const uint32_t key = order_key(i & 1 ? f.y : f.x);
           if (e >= 0 && e < a.V && (byte == 3 || (key >> (8 * byte + 8)) == pre)) atomicAdd(&sh.hist[(key >> (8 * byte)) & 255], 1);
         }
       }
@@ -268,7 +420,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_fwd_kernel(const __grid_c
     }
     __syncthreads();
     thr = key_value(sh.prefix);
-    if (tid == 0) sh.na = sh.nb = 0;
+    if (tid == 0) sh.nh = sh.na = sh.nb = 0;
     __syncthreads();
     collect(thr);
   }
@@ -278,14 +430,14 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_fwd_kernel(const __grid_c
     const int need = max(a.top - na, 0);
     __syncthreads();
     int found = 0;
-    for (int e0 = 0; e0 < a.V && found < need; e0 += kLpThreads) {
+    for (int e0 = 0; e0 < a.V && found < need; e0 += NT) {
       const int e = e0 + tid;
-      const bool hit = e < a.V && to_f32<T>(row.row[e]) == thr;
+      const bool hit = e < a.V && Vec<T>::value(row.row[e]) == thr;
       const unsigned bal = __ballot_sync(0xffffffffu, hit);
       if (lane == 0) sh.wcount[warp] = __popc(bal);
       __syncthreads();
       int at = found, all = 0;
-      for (int i = 0; i < kLpWarps; ++i) {
+      for (int i = 0; i < kWarps; ++i) {
         if (i < warp) at += sh.wcount[i];
         all += sh.wcount[i];
       }
@@ -296,78 +448,132 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_fwd_kernel(const __grid_c
     }
     nb = need;
   }
-  // rank: values above the threshold by (value, index), those equal to it by index behind them
-  for (int i = tid; i < na + nb; i += kLpThreads) {
-    int rank;
-    float v;
-    int e;
-    if (i < na) {
-      v = sh.av[i];
-      e = sh.ai[i];
-      rank = 0;
-      for (int q = 0; q < na; ++q) rank += sh.av[q] > v || (sh.av[q] == v && sh.ai[q] < e);
-    } else {
-      v = thr;
-      e = sh.bi[i - na];
-      rank = na;
-      for (int q = 0; q < nb; ++q) rank += sh.bi[q] < e;
+  // rank: values above the threshold by (value, index), those equal to it by index behind
+  // them; a warp per candidate, a lane per rival
+  for (int i = warp; i < na + nb; i += kWarps) {
+    const bool above = i < na;
+    const float v = above ? sh.av[i] : thr;
+    const int e = above ? sh.ai[i] : sh.bi[i - na];
+    int rank = above ? 0 : na;
+    for (int q = lane; q - lane < (above ? na : nb); q += 32) {
+      bool better;
+      if (above) better = q < na && (sh.av[q] > v || (sh.av[q] == v && sh.ai[q] < e));
+      else better = q < nb && sh.bi[q] < e;
+      rank += __popc(__ballot_sync(0xffffffffu, better));
     }
-    if (rank < a.top) {
-      a.top_lp[r * a.top + rank] = (v - M) - ln;
-      a.top_tok[r * a.top + rank] = e;
+    if (lane == 0 && rank < a.top) {
+      a.top_lp[(long long)r * a.top + rank] = (v - M) - ln;
+      a.top_tok[(long long)r * a.top + rank] = e;
     }
+  }
+  }
+  row = after;
+  __syncthreads();                 // the shared state is free for the next row
   }
 }
 
 // d x_i = g_lp (1[i = tok] - p_i) - g_ent p_i (log p_i + H).  Rows with both factors 0
 // (a masked token, say) are written as zeros without being read.
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) logprobs_bwd_kernel(const __grid_constant__ LogprobArgs a) {
+__global__ void __launch_bounds__(kLpThreads, 3) logprobs_bwd_kernel(const __grid_constant__ LogprobArgs a) {
   constexpr int VE = RowView<T>::VE;
   const long long r = blockIdx.x;
-  const long long tok = a.tokens != nullptr ? a.tokens[r] : -100;
-  const float gl = a.g_lp != nullptr && tok >= 0 ? a.g_lp[r] : 0.f;
+  const long long tk = a.tokens != nullptr ? a.tokens[r] : -100;
+  const int tok = tk >= 0 && tk < a.V ? (int)tk : INT_MIN;   // anything else has no element
+  const float gl = a.g_lp != nullptr && tk >= 0 ? a.g_lp[r] : 0.f;
   const float ge = a.g_ent != nullptr ? a.g_ent[r] : 0.f;
   const T* in = static_cast<const T*>(a.logits) + (r / a.R1) * a.s0 + (r % a.R1) * a.s1;
   T* out = static_cast<T*>(a.dlogits) + r * a.V;
-  const bool any = gl != 0.f || ge != 0.f;
-  const float M = a.stats[2 * r], ll = a.stats[2 * r + 1], H = any && ge != 0.f ? a.entropy[r] : 0.f;
-  auto grad = [&](float x, int e) {
-    const float t = max_nan(fmaf(x - M, kLog2e, -ll), kLpFloor);  // a row without a distribution stays NaN
-    const float p = exp2f(t);
-    const float d = -p * (gl + ge * fmaf(t, kLn2, H));
-    return e == tok ? d + gl : d;
-  };
   const RowView<T> src(in, a.V), dst(out, a.V);
-  const bool same = src.shift == dst.shift;
-  for (int v = threadIdx.x; v < dst.nvec; v += kLpThreads) {
-    const int e0 = dst.first(v);
-    const bool full = e0 >= 0 && e0 <= a.V - VE;
-    float x[VE];
-    if (any) {
-      if (same) src.load(v, x);
+  if (gl == 0.f && ge == 0.f) {
+    for (int v = threadIdx.x; v < dst.nvec; v += kLpThreads) {
+      const int e0 = dst.first(v);
+      if (dst.whole(e0)) *reinterpret_cast<uint4*>(out + e0) = make_uint4(0u, 0u, 0u, 0u);
       else
 #pragma unroll
-        for (int i = 0; i < VE; ++i) x[i] = e0 + i >= 0 && e0 + i < a.V ? to_f32<T>(in[e0 + i]) : -INFINITY;
+        for (int i = 0; i < VE; ++i)
+          if (e0 + i >= 0 && e0 + i < a.V) out[e0 + i] = Vec<T>::from(0.f);
     }
-    uint4 u;
-    T* o = reinterpret_cast<T*>(&u);
+    return;
+  }
+  const float M = a.stats[2 * r], ll = a.stats[2 * r + 1];
+  // -p (gl + ge (ln 2 t + H)) = p (c0 + c1 t), t = log2 p
+  const float c0 = ge != 0.f ? -(gl + ge * a.entropy[r]) : -gl, c1 = -ge * kLn2;
+  const Pair nm = pair(-M, -M), nl = pair(-ll, -ll), le = pair(kLog2e, kLog2e), k0 = pair(c0, c0), k1 = pair(c1, c1);
+  auto grad = [&](Pair x) {
+    const float2 t = halves(fma2(add2(x, nm), le, nl));
+    const float tx = max_nan(t.x, kLpFloor), ty = max_nan(t.y, kLpFloor);  // a row without a distribution stays NaN
+    return mul2(pair(ex2(tx), ex2(ty)), fma2(k1, pair(tx, ty), k0));
+  };
+  auto one = [&](float x) { return halves(grad(pair(x, x))).x; };
+  if (src.shift == dst.shift) {  // both rows are vectors at the same places
+    for (int v0 = threadIdx.x; v0 < dst.nvec; v0 += kLpBwdHold * kLpThreads) {
+      uint4 raw[kLpBwdHold];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) o[i] = from_f32<T>(any ? grad(x[i], e0 + i) : 0.f);
-    if (full) *reinterpret_cast<uint4*>(out + e0) = u;
-    else
+      for (int u = 0; u < kLpBwdHold; ++u)
+        if (v0 + u * kLpThreads < dst.nvec) raw[u] = src.bits(v0 + u * kLpThreads);
 #pragma unroll
-      for (int i = 0; i < VE; ++i)
-        if (e0 + i >= 0 && e0 + i < a.V) out[e0 + i] = o[i];
+      for (int u = 0; u < kLpBwdHold; ++u) {
+        const int v = v0 + u * kLpThreads;
+        if (v >= dst.nvec) break;
+        const int e0 = dst.first(v);
+        uint4 y;
+#pragma unroll
+        for (int i = 0; i < VE / 2; ++i) {
+          const Pair d = grad(Vec<T>::get(raw[u], i));
+          if constexpr (VE == 8) {
+            (&y.x)[i] = Vec<T>::put(d);
+          } else {
+            (&y.x)[2 * i] = __float_as_uint(halves(d).x);
+            (&y.x)[2 * i + 1] = __float_as_uint(halves(d).y);
+          }
+        }
+        if (dst.whole(e0)) *reinterpret_cast<uint4*>(out + e0) = y;
+        else
+#pragma unroll
+          for (int i = 0; i < VE; ++i)
+            if (e0 + i >= 0 && e0 + i < a.V) out[e0 + i] = reinterpret_cast<const T*>(&y)[i];
+        // the given token's element gets gl too (this thread has just stored it)
+        if (tok >= e0 && tok < e0 + VE) out[tok] = Vec<T>::from(one(Vec<T>::value(in[tok])) + gl);
+      }
+    }
+  } else {
+    for (int e = threadIdx.x; e < a.V; e += kLpThreads) {
+      const float d = one(Vec<T>::value(in[e]));
+      out[e] = Vec<T>::from(e == tok ? d + gl : d);
+    }
   }
 }
 
-cudaError_t launch_logprobs_fwd(const LogprobArgs& a, int dtype, cudaStream_t st) {
-  const unsigned grid = (unsigned)(a.R0 * a.R1);
-  if (dtype == 0) logprobs_fwd_kernel<bf16><<<grid, kLpThreads, 0, st>>>(a);
-  else if (dtype == 1) logprobs_fwd_kernel<__half><<<grid, kLpThreads, 0, st>>>(a);
-  else logprobs_fwd_kernel<float><<<grid, kLpThreads, 0, st>>>(a);
+template <typename T, int NT>
+static cudaError_t launch_fwd(const LogprobArgs& a, cudaStream_t st) {
+  constexpr int smem = kLpHold * NT * 16, kDevices = 64;
+  static std::atomic<int> known[kDevices];  // the device's SMs, once its shared memory is granted
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < kDevices) sms = known[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(logprobs_fwd_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev < kDevices) known[dev].store(sms, std::memory_order_relaxed);
+  }
+  const long long rows = a.R0 * a.R1;
+  logprobs_fwd_kernel<T, NT><<<(unsigned)std::min<long long>(rows, (long long)sms * (1024 / NT)), NT, smem, st>>>(a);
   return cudaGetLastError();
+}
+
+// Rows of up to 8 vectors a thread in 128 threads (8192 bf16 logits) run 8 to an SM;
+// longer ones take 512 threads.
+template <typename T>
+static cudaError_t launch_fwd_t(const LogprobArgs& a, cudaStream_t st) {
+  return a.V <= kLpHold * 128 * RowView<T>::VE ? launch_fwd<T, 128>(a, st) : launch_fwd<T, 512>(a, st);
+}
+
+cudaError_t launch_logprobs_fwd(const LogprobArgs& a, int dtype, cudaStream_t st) {
+  return dtype == 0 ? launch_fwd_t<bf16>(a, st) : dtype == 1 ? launch_fwd_t<__half>(a, st) : launch_fwd_t<float>(a, st);
 }
 
 cudaError_t launch_logprobs_bwd(const LogprobArgs& a, int dtype, cudaStream_t st) {
