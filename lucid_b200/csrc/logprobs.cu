@@ -26,9 +26,9 @@ namespace lb {
 
 constexpr int kLpThreads = 512;  // backward
 constexpr int kLpGroups = 128;   // groups of threads
-constexpr int kLpCap = 512;      // list of elements above T, and of those equal to it
 constexpr int kLpHold = 8;       // vectors a thread holds: 32768 bf16 logits in 512 threads
 constexpr int kLpBwdHold = 4;
+constexpr int kLpSmallTop = 24;  // up to here 32 group maxima do
 constexpr float kLpFloor = -200.f;  // 2^-200 is 0 in fp32; keeps 0 * -inf out of w
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -94,6 +94,13 @@ struct Vec<bf16> {
   static __device__ __forceinline__ float top(uint32_t w) {
     return max_nan(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
+  // -inf and what is near it as a number so low that its weight stays 0, but for which t
+  // is finite, while |m| < kNear
+  static constexpr float kNear = 1e37f;
+  static __device__ __forceinline__ uint4 bounded(const uint4& u) {
+    constexpr uint32_t low = 0xfe96fe96u;  // -9.97e37
+    return make_uint4(max2(u.x, low), max2(u.y, low), max2(u.z, low), max2(u.w, low));
+  }
   static __device__ __forceinline__ uint32_t put(Pair p) {
     const float2 f = halves(p);
     const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
@@ -120,6 +127,11 @@ struct Vec<__half> {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
     return max_nan(f.x, f.y);
   }
+  static constexpr float kNear = 6e4f;
+  static __device__ __forceinline__ uint4 bounded(const uint4& u) {  // -65504
+    constexpr uint32_t low = 0xfbfffbffu;
+    return make_uint4(max2(u.x, low), max2(u.y, low), max2(u.z, low), max2(u.w, low));
+  }
   static __device__ __forceinline__ uint32_t put(Pair p) {
     const float2 f = halves(p);
     const __half2 h = __floats2half2_rn(f.x, f.y);
@@ -130,6 +142,7 @@ struct Vec<__half> {
 template <>
 struct Vec<float> {
   static constexpr int VE = 4;
+  static constexpr float kNear = 0.f;
   static constexpr uint32_t kNegInf = 0xff800000u;
   static __device__ __forceinline__ float value(float v) { return v; }
   static __device__ __forceinline__ Pair get(const uint4& u, int i) {
@@ -195,11 +208,14 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 
 template <int NT>
 struct LpShared {
+  static constexpr int kLpCap = NT;       // list of elements above T, and of those equal to it
+  static constexpr int kLpHits = NT / 2;  // list of vectors that hold any
   __align__(16) float gmax[kLpGroups];
+  uint4 hit[kLpHits];              // vectors with an element at or above T
+  int hitv[kLpHits];
   float wm[NT / 32], wl[NT / 32], ww[NT / 32];
   float T, M, ln;
   int nh, na, nb;
-  int hit[kLpCap];                 // vectors with an element at or above T
   float av[kLpCap];
   int ai[kLpCap], bi[kLpCap];
   int hist[256];
@@ -213,14 +229,15 @@ struct LpShared {
 // own places in shared memory, so loads never wait for the joins.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __grid_constant__ LogprobArgs a) {
-  __shared__ LpShared<NT> sh;
+  __shared__ LpShared<NT> both[2];
   extern __shared__ uint4 next[];  // [kLpHold][NT]
   constexpr int VE = RowView<T>::VE, kWarps = NT / 32, kBatch = kLpHold * NT;
+  constexpr int kLpCap = LpShared<NT>::kLpCap, kLpHits = LpShared<NT>::kLpHits;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const unsigned R = (unsigned)(a.R0 * a.R1), R1 = (unsigned)a.R1;
   auto row_of = [&](unsigned r) {
     const unsigned r0 = a.R0 == 1 ? 0 : r / R1;
-    return RowView<T>(static_cast<const T*>(a.logits) + (long long)r0 * a.s0 + (long long)(r - r0 * R1) * a.s1, a.V);
+    return static_cast<const T*>(a.logits) + (long long)r0 * a.s0 + (long long)(r - r0 * R1) * a.s1;
   };
   const uint32_t own = (uint32_t)__cvta_generic_to_shared(&next[tid]);
   auto fetch = [&](const RowView<T>& row, int v0) {  // this thread's vectors of the batch at v0
@@ -235,11 +252,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __gri
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  RowView<T> row = row_of(blockIdx.x);
-  fetch(row, 0);
-  for (unsigned r = blockIdx.x; r < R; r += gridDim.x) {
+  const T* at = row_of(blockIdx.x);
+  fetch(RowView<T>(at, a.V), 0);
+  // Rows take the shared state in turn: a warp may start the next row's while others read
+  // this row's, and meets them at the barrier of its first join.
+  int turn = 0;
+  for (unsigned r = blockIdx.x; r < R; r += gridDim.x, turn ^= 1) {
+  LpShared<NT>& sh = both[turn];
+  const RowView<T> row(at, a.V);
   // ---- one pass: maximum, sum, entropy sum; 8 vectors a thread at a time ----
-  RowView<T> after = row;
   uint4 raw[kLpHold];
   float mx = -INFINITY;
   Pair l2 = pair(0.f, 0.f), w2 = l2;
@@ -250,8 +271,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __gri
     if (v0 + kBatch < row.nvec) {
       fetch(row, v0 + kBatch);
     } else if (r + gridDim.x < R) {
-      after = row_of(r + gridDim.x);
-      fetch(after, 0);
+      at = row_of(r + gridDim.x);
+      fetch(RowView<T>(at, a.V), 0);
     }
     uint32_t best = vec_max<T>(raw[0]);
 #pragma unroll
@@ -266,26 +287,48 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __gri
     }
     if (vm == -INFINITY) continue;  // nothing to add (and mx may not be finite yet)
     const Pair nm = pair(-mx, -mx), le = pair(kLog2e, kLog2e);
+    if (VE == 8 && fabsf(mx) < Vec<T>::kNear) {
+      if constexpr (VE == 8) {
 #pragma unroll
-    for (int u = 0; u < kLpHold; ++u)
-      if (v0 + u * NT < row.nvec) {
+        for (int u = 0; u < kLpHold; ++u)
+          if (v0 + u * NT < row.nvec) {
+            const uint4 x = Vec<T>::bounded(raw[u]);
 #pragma unroll
-        for (int i = 0; i < VE / 2; ++i) {
-          const float2 t = halves(mul2(add2(Vec<T>::get(raw[u], i), nm), le));
-          const float tx = fmaxf(t.x, kLpFloor), ty = fmaxf(t.y, kLpFloor);
-          const Pair p = pair(ex2(tx), ex2(ty));
-          l2 = add2(l2, p);
-          w2 = fma2(p, pair(tx, ty), w2);
-        }
+            for (int i = 0; i < VE / 2; ++i) {
+              const Pair t2 = mul2(add2(Vec<T>::get(x, i), nm), le);
+              const float2 t = halves(t2);
+              const Pair p = pair(ex2(t.x), ex2(t.y));
+              l2 = add2(l2, p);
+              w2 = fma2(p, t2, w2);
+            }
+          }
       }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kLpHold; ++u)
+        if (v0 + u * NT < row.nvec) {
+#pragma unroll
+          for (int i = 0; i < VE / 2; ++i) {
+            const float2 t = halves(mul2(add2(Vec<T>::get(raw[u], i), nm), le));
+            const float tx = fmaxf(t.x, kLpFloor), ty = fmaxf(t.y, kLpFloor);
+            const Pair p = pair(ex2(tx), ex2(ty));
+            l2 = add2(l2, p);
+            w2 = fma2(p, pair(tx, ty), w2);
+          }
+        }
+    }
   }
   const float l = halves(l2).x + halves(l2).y, w = halves(w2).x + halves(w2).y;
   // ---- join the block: warps by shuffles, the rest by the first warp ----
-  if (a.top > 0) {
+  const bool small = a.top <= kLpSmallTop && row.nvec >= NT;  // with a vector in every group
+  if (a.top > 0) {                 // the maxima of 32 or 128 groups of neighbouring threads
+    constexpr int kFew = NT / 32, kMany = NT / kLpGroups;
     float gm = mx;
 #pragma unroll
-    for (int o = 1; o < NT / kLpGroups; o <<= 1) gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
-    if (tid % (NT / kLpGroups) == 0) sh.gmax[tid / (NT / kLpGroups)] = gm;
+    for (int o = 1; o < kFew; o <<= 1)
+      if (small || o < kMany) gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+    const int team = small ? kFew : kMany;
+    if ((tid & (team - 1)) == 0) sh.gmax[tid / team] = gm;
     if (tid == 0) sh.nh = sh.na = sh.nb = 0;
   }
   {
@@ -328,7 +371,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __gri
       }
     }
   }
-  if (a.top > 0) {  // the top-th largest of the group maxima: NT / 128 threads rank each
+  if (a.top == 0) continue;
+  // ---- the top best ----
+  float thr;                       // the top-th largest of the group maxima
+  if (small) {                     // every warp sorts the 32, largest first
+    float v = sh.gmax[lane];
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+      for (int o = k >> 1; o > 0; o >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, v, o);
+        v = ((lane & o) == 0) == ((lane & k) == 0) ? fmaxf(v, other) : fminf(v, other);
+      }
+    thr = __shfl_sync(0xffffffffu, v, a.top - 1);
+  } else {                         // NT / 128 threads rank each of 128
     constexpr int kTeam = NT / kLpGroups;
     const int me = tid / kTeam;
     const float v = sh.gmax[me];
@@ -343,16 +399,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __gri
     for (int o = 1; o < kTeam; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
     if (rank == a.top - 1) sh.T = v;
     __syncthreads();
+    thr = sh.T;
   }
-  const float M = sh.M, ln = sh.ln;  // top > 0 only
-  if (a.top > 0 && !(fabsf(M) < INFINITY)) {
-    for (int i = tid; i < a.top; i += NT) {
-      a.top_lp[(long long)r * a.top + i] = nan;
-      a.top_tok[(long long)r * a.top + i] = -1;
-    }
-  } else if (a.top > 0) {
-  // ---- the top best ----
-  float thr = sh.T;
   auto put = [&](float x, int e, float t) {
     if (x > t) {
       const int at = atomicAdd(&sh.na, 1);
@@ -368,28 +416,40 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __gri
   auto collect = [&](float t) {
     auto look = [&](const uint4& x, int v) {
       if (Vec<T>::top(vec_max<T>(x)) >= t) {
-        const int at = atomicAdd(&sh.nh, 1);
-        if (at < kLpCap) sh.hit[at] = v;
+        const int n = atomicAdd(&sh.nh, 1);
+        if (n < kLpHits) {
+          sh.hit[n] = x;
+          sh.hitv[n] = v;
+        }
       }
     };
     if (row.nvec <= kBatch) {      // the row is still in registers
 #pragma unroll
       for (int u = 0; u < kLpHold; ++u)
-        if (u * NT + tid < row.nvec) look(raw[u], u * NT + tid);
+        if (u * NT < row.nvec) look(raw[u], u * NT + tid);
     } else {
       for (int v = tid; v < row.nvec; v += NT) look(row.bits(v), v);
     }
     __syncthreads();
-    const int nh = sh.nh;
-    // the elements of the few vectors that hold any, or of all
-    const long long some = (long long)(nh <= kLpCap ? nh : row.nvec) * VE;
-    for (long long i = tid; i < some; i += NT) {
-      const int e = row.first(nh <= kLpCap ? sh.hit[i / VE] : (int)(i / VE)) + (int)(i % VE);
-      if (e >= 0 && e < a.V) put(Vec<T>::value(row.row[e]), e, t);
+    if (sh.nh <= kLpHits) {        // the elements of the few vectors that hold any
+      for (int i = tid; i < sh.nh * VE; i += NT) {
+        const int e = row.first(sh.hitv[i / VE]) + i % VE;
+        if (e >= 0 && e < a.V) put(Vec<T>::value(reinterpret_cast<const T*>(&sh.hit[i / VE])[i % VE]), e, t);
+      }
+    } else {
+      for (int e = tid; e < a.V; e += NT) put(Vec<T>::value(row.row[e]), e, t);
     }
     __syncthreads();
   };
   collect(thr);
+  const float M = sh.M, ln = sh.ln;  // the first warp's, before the barriers above
+  if (!(fabsf(M) < INFINITY)) {    // uniform
+    for (int i = tid; i < a.top; i += NT) {
+      a.top_lp[(long long)r * a.top + i] = nan;
+      a.top_tok[(long long)r * a.top + i] = -1;
+    }
+    continue;
+  }
   if (sh.na > kLpCap) {  // uniform: make the threshold the exact top-th largest value
     if (tid == 0) {
       sh.prefix = 0;
@@ -466,9 +526,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __gri
       a.top_tok[(long long)r * a.top + rank] = e;
     }
   }
-  }
-  row = after;
-  __syncthreads();                 // the shared state is free for the next row
   }
 }
 
