@@ -4,38 +4,53 @@
 // one launch and one round of dependent loads).
 #include "serve_common.cuh"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace lb {
 
-// One warp per (row, tensor): lanes copy 8- or 16-byte vectors of the row's D elements.
-// Rows past counts[b], of sequences marked unused (negative length), past the block
-// table or on an invalid page are not written.
-template <int CB>
+// A block takes 256 / nv rows at a time, nv being the 8- or 16-byte vectors of a row: a
+// thread keeps its vector, finds its row's page once and copies it for HN heads of both
+// pools, all loads before the stores.  Rows past counts[b], of sequences marked unused
+// (negative length), past the block table or on an invalid page are not written.
+template <int CB, int HN>
 __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
   using V = typename std::conditional<CB == 16, uint4, uint2>::type;
-  const int per = CB / 2, nv = a.D / per;           // vectors per row
-  const int b = blockIdx.z;
+  constexpr int per = CB / 2;
+  const int nv = a.D / per, rows = 256 / nv;
+  const int b = blockIdx.z, mine = threadIdx.x / nv, v = threadIdx.x - mine * nv;
   const int len = a.lengths[b], cnt = a.counts ? min(a.counts[b], a.N) : a.N;
-  if (len < 0) return;
-  const long long total = (long long)max(cnt, 0) * nv;  // vectors of one head
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (long long)gridDim.x * blockDim.x) {
-    const int n = (int)(i / nv), v = (int)(i % nv);
-    const long long pos = (long long)len + n;
-    const long long pi = pos / a.ps, row = pos % a.ps;
-    if (pi >= a.M) {
+  if (len < 0 || mine >= rows) return;
+  const bf16* ks = a.k + (long long)b * a.k_sb + v * per;
+  const bf16* xs = a.x + (long long)b * a.x_sb + v * per;
+  for (long long n = (long long)blockIdx.x * rows + mine; n < cnt; n += (long long)gridDim.x * rows) {
+    const long long pos = len + n;
+    if (pos >= (long long)a.M * a.ps) {
       report(a.status, kStatusLength, kTagPagedAppend);
-      continue;
+      return;
     }
+    const unsigned pi = (unsigned)pos / (unsigned)a.ps, row = (unsigned)pos - pi * a.ps;
     const int page = a.table[(long long)b * a.t_sb + pi];
     if (page < 0 || page >= a.P) {
       report(a.status, kStatusPage, kTagPagedAppend);
       continue;
     }
-    for (int h = blockIdx.y; h < a.H; h += gridDim.y) {
-      const V kv = *reinterpret_cast<const V*>(a.k + (long long)b * a.k_sb + (long long)h * a.k_sh + (long long)n * a.k_sn + v * per);
-      const V xv = *reinterpret_cast<const V*>(a.x + (long long)b * a.x_sb + (long long)h * a.x_sh + (long long)n * a.x_sn + v * per);
-      *reinterpret_cast<V*>(a.kp.p + (long long)page * a.kp.sp + (long long)h * a.kp.sh + row * a.kp.sn + v * per) = kv;
-      *reinterpret_cast<V*>(a.xp.p + (long long)page * a.xp.sp + (long long)h * a.xp.sh + row * a.xp.sn + v * per) = xv;
+    bf16* kd = a.kp.p + page * a.kp.sp + row * a.kp.sn + v * per;
+    bf16* xd = a.xp.p + page * a.xp.sp + row * a.xp.sn + v * per;
+    for (int h0 = blockIdx.y * HN; h0 < a.H; h0 += gridDim.y * HN) {
+      V kv[HN], xv[HN];
+#pragma unroll
+      for (int u = 0; u < HN; ++u)
+        if (h0 + u < a.H) {
+          kv[u] = *reinterpret_cast<const V*>(ks + (h0 + u) * a.k_sh + n * a.k_sn);
+          xv[u] = *reinterpret_cast<const V*>(xs + (h0 + u) * a.x_sh + n * a.x_sn);
+        }
+#pragma unroll
+      for (int u = 0; u < HN; ++u)
+        if (h0 + u < a.H) {
+          *reinterpret_cast<V*>(kd + (h0 + u) * a.kp.sh) = kv[u];
+          *reinterpret_cast<V*>(xd + (h0 + u) * a.xp.sh) = xv[u];
+        }
     }
   }
 }
@@ -45,11 +60,18 @@ cudaError_t launch_paged_append(const PagedAppendArgs& a, cudaStream_t st) {
                      reinterpret_cast<uintptr_t>(a.kp.p) | reinterpret_cast<uintptr_t>(a.xp.p)) & 15u) == 0 &&
                    ((a.k_sb | a.k_sh | a.k_sn | a.x_sb | a.x_sh | a.x_sn | a.kp.sp | a.kp.sh | a.kp.sn | a.xp.sp |
                      a.xp.sh | a.xp.sn | a.D) & 7) == 0;
-  const long long vec = (long long)a.N * (a.D / (a16 ? 8 : 4));
-  const unsigned gx = (unsigned)min((vec + 255) / 256, 1024LL);
-  const dim3 grid(gx, (unsigned)min(a.H, 65535), (unsigned)a.B);
-  if (a16) paged_append_kernel<16><<<grid, 256, 0, st>>>(a);
-  else paged_append_kernel<8><<<grid, 256, 0, st>>>(a);
+  const int rows = 256 / (a.D / (a16 ? 8 : 4));
+  const unsigned gx = (unsigned)std::min(((long long)a.N + rows - 1) / rows, 4096LL);
+  // few rows: a block per head, for the latency; many: four heads a thread
+  const bool few = (long long)gx * a.B < 296;
+  const dim3 grid(gx, (unsigned)std::min(few ? a.H : (a.H + 3) / 4, 65535), (unsigned)a.B);
+  if (few) {
+    if (a16) paged_append_kernel<16, 1><<<grid, 256, 0, st>>>(a);
+    else paged_append_kernel<8, 1><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (a16) paged_append_kernel<16, 4><<<grid, 256, 0, st>>>(a);
+    else paged_append_kernel<8, 4><<<grid, 256, 0, st>>>(a);
+  }
   return cudaGetLastError();
 }
 
