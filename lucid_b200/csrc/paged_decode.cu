@@ -559,15 +559,88 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
   copy_wait<0>();
 }
 
-// One block per (sequence, kv head) and query row merges the item's segments and, in the
-// step, adds the new token.  Warp w takes the segments w, w + 8, ... (a row of 128 floats
-// is one 16-byte load per lane, all of them independent), then the warps join in order.
-constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+// The join: merges an item's segments and, in the step, adds the new token.  Blocks
+// (sequence and kv head, y).  Few segments: the block y = 0 gives a warp to each query row,
+// lane i holding columns 4 i .. 4 i + 3.  Many (a long sequence over many CTAs): each query
+// row takes a whole block, warp w the segments w, w + 8, ...  Either way a segment's row is one
+// 16-byte load per lane, all of them independent, and the order of the sums is fixed.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinFew = 16, kJoinAhead = 6;
+
+// (max, denominator, weighted sum) of `cnt` segment rows at p, p + step, ...; the lanes
+// together read the maxima first.  Lanes past D (col false) sum nothing.
+struct JoinRow {
+  float M, L;
+  float4 acc;
+};
+__device__ __forceinline__ JoinRow join_rows(const float* p, long long step, int cnt, int D, bool col, int lane) {
+  JoinRow r{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int i0 = 0; i0 < cnt; i0 += 32) {
+    float mi = -INFINITY, li = 0.f;
+    if (i0 + lane < cnt) {
+      const float2 ml = *reinterpret_cast<const float2*>(p + (i0 + lane) * step + D);
+      mi = ml.x;
+      li = ml.y;
+    }
+    const int k = min(32, cnt - i0);
+    float4 v[kJoinAhead];
+    auto fetch = [&](int q0) {       // all loads of a group before any use
+#pragma unroll
+      for (int q = 0; q < kJoinAhead; ++q) {
+        v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (col && q0 + q < k) v[q] = *reinterpret_cast<const float4*>(p + (i0 + q0 + q) * step + 4 * lane);
+      }
+    };
+    fetch(0);
+    float mx = mi;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float mn = fmaxf(r.M, mx), ms = mn == -INFINITY ? 0.f : mn;
+    const float f = ex2(mi - ms), fo = ex2(r.M - ms);
+    float ls = f * li;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
+    r.L = r.L * fo + ls;
+    r.acc.x *= fo; r.acc.y *= fo; r.acc.z *= fo; r.acc.w *= fo;
+    r.M = mn;
+    for (int q0 = 0; q0 < k; q0 += kJoinAhead) {
+      if (q0 > 0) fetch(q0);
+#pragma unroll
+      for (int q = 0; q < kJoinAhead; ++q) {
+        const float fq = __shfl_sync(0xffffffffu, f, (q0 + q) & 31);  // 0 past the last segment's lane
+        r.acc.x = fmaf(fq, v[q].x, r.acc.x);
+        r.acc.y = fmaf(fq, v[q].y, r.acc.y);
+        r.acc.z = fmaf(fq, v[q].z, r.acc.z);
+        r.acc.w = fmaf(fq, v[q].w, r.acc.w);
+      }
+    }
+  }
+  return r;
+}
+// plain sum of `cnt` rows
+__device__ __forceinline__ float4 join_sum(const float* p, long long step, int cnt, bool col, int lane) {
+  float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int q0 = 0; q0 < cnt; q0 += kJoinAhead) {
+    float4 v[kJoinAhead];
+#pragma unroll
+    for (int q = 0; q < kJoinAhead; ++q) {
+      v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (col && q0 + q < cnt) v[q] = *reinterpret_cast<const float4*>(p + (q0 + q) * step + 4 * lane);
+    }
+#pragma unroll
+    for (int q = 0; q < kJoinAhead; ++q) { u.x += v[q].x; u.y += v[q].y; u.z += v[q].z; u.w += v[q].w; }
+  }
+  return u;
+}
+__device__ __forceinline__ float4 load4(const bf16* p) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  const float2 x = unpack_bf16(v.x), y = unpack_bf16(v.y);
+  return make_float4(x.x, x.y, y.x, y.y);
+}
 
 template <bool STEP>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedDecodeArgs a) {
+__global__ void __launch_bounds__(kJoinThreads, 3) paged_join_kernel(const __grid_constant__ PagedDecodeArgs a) {
   __shared__ __align__(16) float sum_a[kJoinWarps][128], sum_u[kJoinWarps][128];
-  __shared__ float wm[kJoinWarps], wl[kJoinWarps], wz[kJoinWarps];
+  __shared__ float wm[kJoinWarps], wl[kJoinWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / a.H, h = blockIdx.x % a.H;
   const int raw = a.lengths[b];
@@ -602,125 +675,130 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     cnt = (int)pd_div((last + 1) * G - 1, T) - i0 + 1;
     return a.part + (i0 + (long long)blockIdx.x * a.nblk + blk) * slot;
   };
+  int cnt0;
+  const float* p0 = range(0, cnt0);
+  const bool few = cnt0 <= kJoinFew;   // the other blocks of query rows differ by one segment at most
+  if (few && blockIdx.y > 0) return;
   const bool col = 4 * lane < a.D;
   const float c1 = a.s * kLog2e;
-  // the new key and value are nothing that the tile pass writes
-  bf16 kb = __float2bfloat16(0.f);
-  float vv = 0.f;
-  if (STEP && used && tid < a.D) {
-    kb = a.kn[(long long)b * a.kn_sb + (long long)h * a.kn_sh + tid];
-    vv = __bfloat162float(a.vn[(long long)b * a.vn_sb + (long long)h * a.vn_sh + tid]);
+  // what the tile pass does not write: this lane's columns of the new key and value, and
+  // the place of the new row
+  float4 kn = make_float4(0.f, 0.f, 0.f, 0.f), vn = kn;
+  int page = -1;
+  if (STEP && used && col) {
+    kn = load4(a.kn + (long long)b * a.kn_sb + (long long)h * a.kn_sh + 4 * lane);
+    vn = load4(a.vn + (long long)b * a.vn_sb + (long long)h * a.vn_sh + 4 * lane);
+  }
+  if (STEP && used && a.append && blockIdx.y == 0) {
+    const int pi = n / a.ps;
+    page = pi < a.M ? a.table[(long long)b * a.t_sb + pi] : -1;
+    if (page < 0 || page >= a.P) {
+      if (tid == 0) report(a.status, pi < a.M ? kStatusPage : kStatusLength, kTagPagedDecode);
+      page = -1;
+    }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the tile pass has ended and its stores are seen
 
-  float xv = 0.f;
-  if constexpr (STEP) {
-    int cnt;
-    const float* p = range(0, cnt) + (long long)min(a.gq, a.rows) * pr + 4 * lane;
-    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (col) {
-#pragma unroll 8
-      for (int i = warp; i < cnt; i += kJoinWarps) {
-        const float4 v = *reinterpret_cast<const float4*>(p + i * slot);
-        u.x += v.x; u.y += v.y; u.z += v.z; u.w += v.w;
+  // x_new as the cache holds it, from the sum u; one warp of the sequence and head writes it
+  auto solved = [&](const float4& u, bool write) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!col) return x;
+    const uint32_t lo = pack_bf16(vn.x - u.x, vn.y - u.y), hi = pack_bf16(vn.z - u.z, vn.w - u.w);
+    const float2 x0 = unpack_bf16(lo), x1 = unpack_bf16(hi);
+    x = make_float4(x0.x, x0.y, x1.x, x1.y);
+    if (write) {
+      *reinterpret_cast<uint2*>(a.xo + (long long)b * a.xo_sb + (long long)h * a.xo_sh + 4 * lane) = make_uint2(lo, hi);
+      if (page >= 0) {
+        const long long row = n % a.ps;
+        *reinterpret_cast<uint2*>(a.k.p + (long long)page * a.k.sp + (long long)h * a.k.sh + row * a.k.sn + 4 * lane) =
+            make_uint2(pack_bf16(kn.x, kn.y), pack_bf16(kn.z, kn.w));
+        *reinterpret_cast<uint2*>(a.x.p + (long long)page * a.x.sp + (long long)h * a.x.sh + row * a.x.sn + 4 * lane) =
+            make_uint2(lo, hi);
       }
     }
-    *reinterpret_cast<float4*>(&sum_u[warp][4 * lane]) = u;
-  }
-  for (int r = blockIdx.y; r < a.gq; r += gridDim.y) {
-    int cnt;
-    const float* p = range(r / a.rows, cnt) + (long long)(r % a.rows) * pr;
-    float M = -INFINITY, L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = warp; i0 < cnt; i0 += 32 * kJoinWarps) {  // at most 32 segments of this warp at a time
-      const int mine = i0 + lane * kJoinWarps;
-      float mi = -INFINITY, li = 0.f;
-      if (mine < cnt) {
-        mi = p[mine * slot + a.D];
-        li = p[mine * slot + a.D + 1];
+    return x;
+  };
+  // the row's output from its merged sums and the new token
+  auto finish = [&](int r, float M, float L, float4 acc, const float4& x) {
+    if constexpr (STEP) {
+      float z = 0.f;
+      if (col) {
+        const float4 q = load4(a.q + (long long)b * a.q_sb + (long long)(h * a.gq + r) * a.q_sh + 4 * lane);
+        z = (q.x * kn.x + q.y * kn.y) + (q.z * kn.z + q.w * kn.w);
       }
-      float mx = mi;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float mn = fmaxf(M, mx), ms = mn == -INFINITY ? 0.f : mn;
-      const float f = ex2(mi - ms), fo = ex2(M - ms);
-      float ls = f * li;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, o);
-      L = L * fo + ls;
-      acc.x *= fo; acc.y *= fo; acc.z *= fo; acc.w *= fo;
-      M = mn;
-      const int k = min(32, (cnt - i0 + kJoinWarps - 1) / kJoinWarps);
-#pragma unroll 8
-      for (int q = 0; q < k; ++q) {
-        const float fq = __shfl_sync(0xffffffffu, f, q);
-        if (col) {
-          const float4 v = *reinterpret_cast<const float4*>(p + (long long)(i0 + q * kJoinWarps) * slot + 4 * lane);
-          acc.x = fmaf(fq, v.x, acc.x);
-          acc.y = fmaf(fq, v.y, acc.y);
-          acc.z = fmaf(fq, v.z, acc.z);
-          acc.w = fmaf(fq, v.w, acc.w);
-        }
-      }
-    }
-    float z = 0.f;
-    if constexpr (STEP) {  // the new token's score: thread d < 128 has element d
-      if (tid < a.D)
-        z = __bfloat162float(a.q[(long long)b * a.q_sb + (long long)(h * a.gq + r) * a.q_sh + tid]) * __bfloat162float(kb);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      z *= c1;
+      const float mn = fmaxf(M, z), ms = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2(M - ms), p = ex2(z - ms);
+      L = fmaf(L, f, p);
+      acc = make_float4(fmaf(acc.x, f, p * x.x), fmaf(acc.y, f, p * x.y), fmaf(acc.z, f, p * x.z), fmaf(acc.w, f, p * x.w));
     }
-    *reinterpret_cast<float4*>(&sum_a[warp][4 * lane]) = acc;
-    if (lane == 0) {
-      wm[warp] = M;
-      wl[warp] = L;
-      wz[warp] = z;
-    }
-    __syncthreads();
-    if (tid < a.D) {
-      if (STEP && r == (int)blockIdx.y) {  // x_new, as the cache holds it
-        float u = 0.f;
-#pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) u += sum_u[w][tid];
-        const bf16 xb = __float2bfloat16(vv - u);
-        xv = __bfloat162float(xb);
-        if (blockIdx.y == 0) {
-          a.xo[(long long)b * a.xo_sb + (long long)h * a.xo_sh + tid] = xb;
-          if (a.append && used) {
-            const int pi = n / a.ps;
-            const int page = pi < a.M ? a.table[(long long)b * a.t_sb + pi] : -1;
-            if (page < 0 || page >= a.P) {
-              if (tid == 0) report(a.status, pi < a.M ? kStatusPage : kStatusLength, kTagPagedDecode);
-            } else {
-              const long long row = n % a.ps;
-              a.k.p[(long long)page * a.k.sp + (long long)h * a.k.sh + row * a.k.sn + tid] = kb;
-              a.x.p[(long long)page * a.x.sp + (long long)h * a.x.sh + row * a.x.sn + tid] = xb;
-            }
-          }
+    const bool none = !used || (!STEP && nt == 0);  // no token to attend to
+    if (col)
+      *reinterpret_cast<uint2*>(a.o + (long long)b * a.o_sb + (long long)(h * a.gq + r) * a.o_sh + 4 * lane) =
+          none ? make_uint2(0u, 0u) : make_uint2(pack_bf16(acc.x / L, acc.y / L), pack_bf16(acc.z / L, acc.w / L));
+  };
+  const long long upd = (long long)min(a.gq, a.rows) * pr;  // the update row of block 0's segments
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool have_x = false;
+  for (int blk = 0; blk < a.nblk; ++blk) {
+    int cnt;
+    const float* p = range(blk, cnt);
+    const int r0 = blk * a.rows, r1 = min(a.gq, r0 + a.rows);
+    if (few) {
+      for (int r = r0 + warp; r < r1; r += kJoinWarps) {
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (STEP && !have_x) u = join_sum(p0 + upd, slot, cnt0, col, lane);
+        const JoinRow j = join_rows(p + (r - r0) * (long long)pr, slot, cnt, a.D, col, lane);
+        if (STEP && !have_x) {
+          x = solved(u, r == 0);
+          have_x = true;
         }
+        finish(r, j.M, j.L, j.acc, x);
       }
-      float mx = -INFINITY, zn = -INFINITY;
-      if constexpr (STEP) zn = ((wz[0] + wz[1]) + (wz[2] + wz[3])) * c1;
-      mx = zn;
+    } else {
+      if (STEP && blk == 0) {
+        *reinterpret_cast<float4*>(&sum_u[warp][4 * lane]) =
+            join_sum(p0 + upd + warp * slot, kJoinWarps * slot, (cnt0 - warp + kJoinWarps - 1) / kJoinWarps, col, lane);
+        __syncthreads();
+        float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) mx = fmaxf(mx, wm[w]);
-      const float ms = mx == -INFINITY ? 0.f : mx;
-      float Ls = 0.f, o = 0.f;
+        for (int w = 0; w < kJoinWarps; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(&sum_u[w][4 * lane]);
+          u.x += v.x; u.y += v.y; u.z += v.z; u.w += v.w;
+        }
+        x = solved(u, blockIdx.y == 0 && warp == 0);
+      }
+      for (int r = r0; r < r1; ++r) {
+        if (r % (int)gridDim.y != (int)blockIdx.y) continue;
+        const JoinRow j = join_rows(p + (r - r0) * (long long)pr + warp * slot, kJoinWarps * slot,
+                                    (cnt - warp + kJoinWarps - 1) / kJoinWarps, a.D, col, lane);
+        *reinterpret_cast<float4*>(&sum_a[warp][4 * lane]) = j.acc;
+        if (lane == 0) {
+          wm[warp] = j.M;
+          wl[warp] = j.L;
+        }
+        __syncthreads();
+        if (warp == 0) {
+          float M = wm[0];
 #pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) {
-        const float f = ex2(wm[w] - ms);
-        Ls = fmaf(f, wl[w], Ls);
-        o = fmaf(f, sum_a[w][tid], o);
+          for (int w = 1; w < kJoinWarps; ++w) M = fmaxf(M, wm[w]);
+          const float ms = M == -INFINITY ? 0.f : M;
+          float L = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kJoinWarps; ++w) {
+            const float f = ex2(wm[w] - ms);
+            const float4 v = *reinterpret_cast<const float4*>(&sum_a[w][4 * lane]);
+            L = fmaf(f, wl[w], L);
+            acc = make_float4(fmaf(f, v.x, acc.x), fmaf(f, v.y, acc.y), fmaf(f, v.z, acc.z), fmaf(f, v.w, acc.w));
+          }
+          finish(r, M, L, acc, x);
+        }
+        __syncthreads();  // the sums are free again
       }
-      if constexpr (STEP) {
-        const float pn = ex2(zn - ms);
-        Ls += pn;
-        o = fmaf(pn, xv, o);
-      }
-      const bool none = !used || (!STEP && nt == 0);  // no token to attend to
-      a.o[(long long)b * a.o_sb + (long long)(h * a.gq + r) * a.o_sh + tid] = __float2bfloat16(none ? 0.f : o / Ls);
     }
-    __syncthreads();  // the sums are free again
   }
 }
 
@@ -794,7 +872,7 @@ cudaError_t launch_paged_decode(PagedDecodeArgs a, bool step, cudaStream_t st) {
   cudaError_t e = step ? (rows <= 8 ? launch_pd_d<true, true>(a, st) : launch_pd_d<true, false>(a, st))
                        : (rows <= 8 ? launch_pd_d<false, true>(a, st) : launch_pd_d<false, false>(a, st));
   if (e != cudaSuccess) return e;
-  // one block per query row while that fills the GPU only a few times over.  The join's
+  // a block for each query row while that fills the GPU only a few times over.  The join's
   // blocks may start while the tile pass ends (they wait before reading its results).
   const int bh = a.B * a.H;
   cudaLaunchConfig_t cfg = {};

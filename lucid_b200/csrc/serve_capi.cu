@@ -48,10 +48,12 @@ int decode(bool step, int B, int Hq, int Hkv, int D, int P, int ps, int M, float
   if (!heads_ok(B, Hq, Hkv, D) || !pool_ok(P, ps, M)) return LUCID_ERR_SHAPE;
   if (B == 0 || Hq == 0) return LUCID_OK;
   if (Hq / Hkv > 65535) return LUCID_ERR_SHAPE;
-  if (!ptr_ok(q, 8) || !ptr_ok(kp, 8) || !ptr_ok(xp, 8) || !ptr_ok(table, 4) || !ptr_ok(lengths, 4) || !ptr_ok(o, 2) ||
-      !m4(q_sb, q_sh) || !m4(kp_sp, kp_sh, kp_sn) || !m4(xp_sp, xp_sh, xp_sn))
+  if (!ptr_ok(q, 8) || !ptr_ok(kp, 8) || !ptr_ok(xp, 8) || !ptr_ok(table, 4) || !ptr_ok(lengths, 4) || !ptr_ok(o, 8) ||
+      !m4(q_sb, q_sh) || !m4(o_sb, o_sh) || !m4(kp_sp, kp_sh, kp_sn) || !m4(xp_sp, xp_sh, xp_sn))
     return LUCID_ERR_ALIGN;
-  if (step && (!ptr_ok(kn, 8) || !ptr_ok(vn, 2) || !ptr_ok(xo, 2) || !m4(kn_sb, kn_sh))) return LUCID_ERR_ALIGN;
+  if (step && (!ptr_ok(kn, 8) || !ptr_ok(vn, 8) || !ptr_ok(xo, 8) || !m4(kn_sb, kn_sh) || !m4(vn_sb, vn_sh) ||
+               !m4(xo_sb, xo_sh)))
+    return LUCID_ERR_ALIGN;
   if (!ptr_ok(workspace, 16) || workspace_bytes < decode_bytes(B, Hq, Hkv, D, step)) return LUCID_ERR_WORKSPACE;
   PagedDecodeArgs a{};
   a.B = B; a.H = Hkv; a.Hq = Hq; a.D = D; a.P = P; a.ps = ps; a.M = M;
