@@ -28,6 +28,7 @@ constexpr int kLpThreads = 512;  // backward
 constexpr int kLpGroups = 128;   // groups of threads
 constexpr int kLpHold = 8;       // vectors a thread holds: 32768 bf16 logits in 512 threads
 constexpr int kLpBwdHold = 4;
+constexpr int kLpManyRows = 900;
 constexpr int kLpSmallTop = 24;  // up to here 32 group maxima do
 constexpr float kLpFloor = -200.f;  // 2^-200 is 0 in fp32; keeps 0 * -inf out of w
 
@@ -106,6 +107,13 @@ struct Vec<bf16> {
     const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  // whether either half of a vec_max reaches v, a value of the type given in both halves
+  static __device__ __forceinline__ uint32_t twice(float v) { return put(pair(v, v)); }
+  static __device__ __forceinline__ bool reaches(uint32_t w, uint32_t v) {
+    uint32_t r;
+    asm("{\n.reg .pred p, q;\nsetp.ge.bf16x2 p|q, %1, %2;\nor.pred p, p, q;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r) : "r"(w), "r"(v));
+    return r != 0;
+  }
   static __device__ __forceinline__ bf16 from(float v) { return __float2bfloat16(v); }
 };
 template <>
@@ -137,6 +145,12 @@ struct Vec<__half> {
     const __half2 h = __floats2half2_rn(f.x, f.y);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  static __device__ __forceinline__ uint32_t twice(float v) { return put(pair(v, v)); }
+  static __device__ __forceinline__ bool reaches(uint32_t w, uint32_t v) {
+    uint32_t r;
+    asm("{\n.reg .pred p, q;\nsetp.ge.f16x2 p|q, %1, %2;\nor.pred p, p, q;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r) : "r"(w), "r"(v));
+    return r != 0;
+  }
   static __device__ __forceinline__ __half from(float v) { return __float2half(v); }
 };
 template <>
@@ -152,6 +166,8 @@ struct Vec<float> {
     return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
   }
   static __device__ __forceinline__ float top(uint32_t w) { return __uint_as_float(w); }
+  static __device__ __forceinline__ uint32_t twice(float v) { return __float_as_uint(v); }
+  static __device__ __forceinline__ bool reaches(uint32_t w, uint32_t v) { return __uint_as_float(w) >= __uint_as_float(v); }
   static __device__ __forceinline__ float from(float v) { return v; }
 };
 template <typename T>
@@ -206,35 +222,39 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 
-template <int NT>
+template <int NT, bool TOP>
 struct LpShared {
-  static constexpr int kLpCap = NT;       // list of elements above T, and of those equal to it
-  static constexpr int kLpHits = NT / 2;  // list of vectors that hold any
-  __align__(16) float gmax[kLpGroups];
-  uint4 hit[kLpHits];              // vectors with an element at or above T
-  int hitv[kLpHits];
-  float wm[NT / 32], wl[NT / 32], ww[NT / 32];
+  static constexpr int kCap = !TOP ? 1 : NT == 128 ? 256 : 512;   // list of elements above T, and of those equal to it
+  static constexpr int kHits = !TOP ? 1 : NT == 128 ? 384 : 256;  // list of vectors that hold any
+  __align__(16) float gmax[2][TOP ? kLpGroups : 1];
+  uint4 hit[kHits];
+  int hitv[kHits];
+  float wm[2][NT / 32], wl[2][NT / 32], ww[2][NT / 32];
   float T, M, ln;
   int nh, na, nb;
-  float av[kLpCap];
-  int ai[kLpCap], bi[kLpCap];
-  int hist[256];
+  unsigned long long above[kCap];  // (value, lowest index first) as one key
+  int equal[kCap];                 // indices
+  int hist[TOP ? 256 : 1];
   uint32_t prefix;
   int remain;
   int wcount[NT / 32];
 };
 
+// blocks to an SM: 64 registers a thread, 72 for the short block with alternatives
+constexpr int lp_blocks(int nt, bool top) { return nt == 128 && top ? 7 : 1024 / nt; }
+
 // Blocks stay for many rows.  While a block works on the 8 vectors that each thread holds
-// in registers, cp.async brings the thread's next 8 (of this row or the next) into its
-// own places in shared memory, so loads never wait for the joins.
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __grid_constant__ LogprobArgs a) {
-  __shared__ LpShared<NT> both[2];
+// in registers (a batch), cp.async brings the thread's next 8 (of this row or the next)
+// into its own places in shared memory, so loads never wait for the joins.
+template <typename T, int NT, bool TOP>
+__global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(const __grid_constant__ LogprobArgs a) {
+  __shared__ LpShared<NT, TOP> sh;
   extern __shared__ uint4 next[];  // [kLpHold][NT]
   constexpr int VE = RowView<T>::VE, kWarps = NT / 32, kBatch = kLpHold * NT;
-  constexpr int kLpCap = LpShared<NT>::kLpCap, kLpHits = LpShared<NT>::kLpHits;
+  constexpr int kCap = LpShared<NT, TOP>::kCap, kHits = LpShared<NT, TOP>::kHits;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const unsigned R = (unsigned)(a.R0 * a.R1), R1 = (unsigned)a.R1;
+  const float nan = __int_as_float(0x7fc00000);
   auto row_of = [&](unsigned r) {
     const unsigned r0 = a.R0 == 1 ? 0 : r / R1;
     return static_cast<const T*>(a.logits) + (long long)r0 * a.s0 + (long long)(r - r0 * R1) * a.s1;
@@ -254,278 +274,298 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logprobs_fwd_kernel(const __gri
   };
   const T* at = row_of(blockIdx.x);
   fetch(RowView<T>(at, a.V), 0);
-  // Rows take the shared state in turn: a warp may start the next row's while others read
-  // this row's, and meets them at the barrier of its first join.
+  // Without alternatives a row has one barrier: a warp may be at its next row while others
+  // read this row's sums, which the rows therefore keep in turn.
   int turn = 0;
   for (unsigned r = blockIdx.x; r < R; r += gridDim.x, turn ^= 1) {
-  LpShared<NT>& sh = both[turn];
-  const RowView<T> row(at, a.V);
-  // ---- one pass: maximum, sum, entropy sum; 8 vectors a thread at a time ----
-  uint4 raw[kLpHold];
-  float mx = -INFINITY;
-  Pair l2 = pair(0.f, 0.f), w2 = l2;
-  for (int v0 = 0; v0 < row.nvec; v0 += kBatch) {
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const RowView<T> row(at, a.V);
+    const bool multi = row.nvec > kBatch;  // else the whole row stays in registers
+    const bool small = a.top <= kLpSmallTop && row.nvec >= NT;  // 32 groups do, with a vector in each
+    // the maxima so far of 32 or 128 groups of neighbouring threads (which = 0: of the first batch)
+    auto publish = [&](int which, float mx) {
+      constexpr int kFew = NT / 32, kMany = NT / kLpGroups;
+      float gm = mx;
 #pragma unroll
-    for (int u = 0; u < kLpHold; ++u) raw[u] = next[u * NT + tid];
-    if (v0 + kBatch < row.nvec) {
-      fetch(row, v0 + kBatch);
-    } else if (r + gridDim.x < R) {
-      at = row_of(r + gridDim.x);
-      fetch(RowView<T>(at, a.V), 0);
-    }
-    uint32_t best = vec_max<T>(raw[0]);
+      for (int o = 1; o < kFew; o <<= 1)
+        if (small || o < kMany) gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+      const int team = small ? kFew : kMany;
+      if ((tid & (team - 1)) == 0) sh.gmax[which][tid / team] = gm;
+    };
+    // after a barrier: the top-th largest of them
+    auto select = [&](int which) -> float {
+      if (small) {                   // every warp sorts the 32, largest first
+        float v = sh.gmax[which][lane];
 #pragma unroll
-    for (int u = 1; u < kLpHold; ++u) best = Vec<T>::max2(best, vec_max<T>(raw[u]));
-    const float vm = Vec<T>::top(best);
-    if (!(vm <= mx)) {            // larger, or NaN
-      const float mn = max_nan(mx, vm);
-      const float d = fmaxf((mx - mn) * kLog2e, kLpFloor), f = ex2(d);  // nothing yet: f = 0
-      w2 = mul2(pair(f, f), fma2(pair(d, d), l2, w2));
-      l2 = mul2(pair(f, f), l2);
-      mx = mn;
-    }
-    if (vm == -INFINITY) continue;  // nothing to add (and mx may not be finite yet)
-    const Pair nm = pair(-mx, -mx), le = pair(kLog2e, kLog2e);
-    if (VE == 8 && fabsf(mx) < Vec<T>::kNear) {
-      if constexpr (VE == 8) {
+        for (int k = 2; k <= 32; k <<= 1)
 #pragma unroll
-        for (int u = 0; u < kLpHold; ++u)
-          if (v0 + u * NT < row.nvec) {
-            const uint4 x = Vec<T>::bounded(raw[u]);
-#pragma unroll
-            for (int i = 0; i < VE / 2; ++i) {
-              const Pair t2 = mul2(add2(Vec<T>::get(x, i), nm), le);
-              const float2 t = halves(t2);
-              const Pair p = pair(ex2(t.x), ex2(t.y));
-              l2 = add2(l2, p);
-              w2 = fma2(p, t2, w2);
-            }
+          for (int o = k >> 1; o > 0; o >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, v, o);
+            v = ((lane & o) == 0) == ((lane & k) == 0) ? fmaxf(v, other) : fminf(v, other);
           }
+        return __shfl_sync(0xffffffffu, v, a.top - 1);
       }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kLpHold; ++u)
-        if (v0 + u * NT < row.nvec) {
-#pragma unroll
-          for (int i = 0; i < VE / 2; ++i) {
-            const float2 t = halves(mul2(add2(Vec<T>::get(raw[u], i), nm), le));
-            const float tx = fmaxf(t.x, kLpFloor), ty = fmaxf(t.y, kLpFloor);
-            const Pair p = pair(ex2(tx), ex2(ty));
-            l2 = add2(l2, p);
-            w2 = fma2(p, pair(tx, ty), w2);
-          }
-        }
-    }
-  }
-  const float l = halves(l2).x + halves(l2).y, w = halves(w2).x + halves(w2).y;
-  // ---- join the block: warps by shuffles, the rest by the first warp ----
-  const bool small = a.top <= kLpSmallTop && row.nvec >= NT;  // with a vector in every group
-  if (a.top > 0) {                 // the maxima of 32 or 128 groups of neighbouring threads
-    constexpr int kFew = NT / 32, kMany = NT / kLpGroups;
-    float gm = mx;
-#pragma unroll
-    for (int o = 1; o < kFew; o <<= 1)
-      if (small || o < kMany) gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
-    const int team = small ? kFew : kMany;
-    if ((tid & (team - 1)) == 0) sh.gmax[tid / team] = gm;
-    if (tid == 0) sh.nh = sh.na = sh.nb = 0;
-  }
-  {
-    const float wmx = warp_max_nan(mx);
-    const float d = fmaxf((mx - wmx) * kLog2e, kLpFloor), f = ex2(d);  // a thread without elements: l = w = 0
-    const float wl = warp_sum_f(l * f), ww = warp_sum_f(f * fmaf(d, l, w));
-    if (lane == 0) {
-      sh.wm[warp] = wmx;
-      sh.wl[warp] = wl;
-      sh.ww[warp] = ww;
-    }
-  }
-  __syncthreads();
-  const float nan = __int_as_float(0x7fc00000);
-  if (warp == 0) {
-    const float m = lane < kWarps ? sh.wm[lane] : -INFINITY;
-    const float M = warp_max_nan(m);
-    const bool ok = fabsf(M) < INFINITY;  // else no distribution: all -inf, a NaN or +inf
-    const float d = fmaxf((m - M) * kLog2e, kLpFloor), f = ex2(d);
-    const float l0 = lane < kWarps ? sh.wl[lane] : 0.f, w0 = lane < kWarps ? sh.ww[lane] : 0.f;
-    const float L = warp_sum_f(l0 * f), W = warp_sum_f(f * fmaf(d, l0, w0));
-    const float ll = log2f(L), ln = logf(L);
-    if (lane == 0) {
-      sh.M = ok ? M : nan;
-      sh.ln = ln;
-      a.entropy[r] = ok ? kLn2 * (ll - W / L) : nan;
-      if (a.stats != nullptr) {
-        a.stats[2 * (long long)r] = ok ? M : nan;
-        a.stats[2 * (long long)r + 1] = ok ? ll : nan;
-      }
-      if (a.tokens != nullptr) {
-        const long long tok = a.tokens[r];
-        float lp = 0.f;
-        if (tok >= 0 && tok < a.V) lp = ok ? (Vec<T>::value(row.row[tok]) - M) - ln : nan;
-        else if (tok != -100) {
-          report(a.status, kStatusToken, kTagLogprobs);
-          lp = nan;
-        }
-        a.logprobs[r] = lp;
-      }
-    }
-  }
-  if (a.top == 0) continue;
-  // ---- the top best ----
-  float thr;                       // the top-th largest of the group maxima
-  if (small) {                     // every warp sorts the 32, largest first
-    float v = sh.gmax[lane];
-#pragma unroll
-    for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-      for (int o = k >> 1; o > 0; o >>= 1) {
-        const float other = __shfl_xor_sync(0xffffffffu, v, o);
-        v = ((lane & o) == 0) == ((lane & k) == 0) ? fmaxf(v, other) : fminf(v, other);
-      }
-    thr = __shfl_sync(0xffffffffu, v, a.top - 1);
-  } else {                         // NT / 128 threads rank each of 128
-    constexpr int kTeam = NT / kLpGroups;
-    const int me = tid / kTeam;
-    const float v = sh.gmax[me];
-    int rank = 0;
+      constexpr int kTeam = NT / kLpGroups;  // NT / 128 threads rank each of 128
+      const int me = tid / kTeam;
+      const float v = sh.gmax[which][me];
+      int rank = 0;
 #pragma unroll 8
-    for (int q = tid % kTeam; q < kLpGroups / 4; q += kTeam) {
-      const float4 o = *reinterpret_cast<const float4*>(&sh.gmax[4 * q]);
-      rank += (o.x > v || (o.x == v && 4 * q < me)) + (o.y > v || (o.y == v && 4 * q + 1 < me)) +
-              (o.z > v || (o.z == v && 4 * q + 2 < me)) + (o.w > v || (o.w == v && 4 * q + 3 < me));
-    }
-#pragma unroll
-    for (int o = 1; o < kTeam; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
-    if (rank == a.top - 1) sh.T = v;
-    __syncthreads();
-    thr = sh.T;
-  }
-  auto put = [&](float x, int e, float t) {
-    if (x > t) {
-      const int at = atomicAdd(&sh.na, 1);
-      if (at < kLpCap) {
-        sh.av[at] = x;
-        sh.ai[at] = e;
+      for (int q = tid % kTeam; q < kLpGroups / 4; q += kTeam) {
+        const float4 o = *reinterpret_cast<const float4*>(&sh.gmax[which][4 * q]);
+        rank += (o.x > v || (o.x == v && 4 * q < me)) + (o.y > v || (o.y == v && 4 * q + 1 < me)) +
+                (o.z > v || (o.z == v && 4 * q + 2 < me)) + (o.w > v || (o.w == v && 4 * q + 3 < me));
       }
-    } else if (x == t) {
-      const int at = atomicAdd(&sh.nb, 1);
-      if (at < kLpCap) sh.bi[at] = e;
-    }
-  };
-  auto collect = [&](float t) {
-    auto look = [&](const uint4& x, int v) {
-      if (Vec<T>::top(vec_max<T>(x)) >= t) {
+#pragma unroll
+      for (int o = 1; o < kTeam; o <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      if (rank == a.top - 1) sh.T = v;
+      __syncthreads();
+      return sh.T;
+    };
+    auto look = [&](const uint4& x, int v, uint32_t t) {  // lists vector v if it reaches t
+      if (Vec<T>::reaches(vec_max<T>(x), t) && v < row.nvec) {
         const int n = atomicAdd(&sh.nh, 1);
-        if (n < kLpHits) {
+        if (n < kHits) {
           sh.hit[n] = x;
           sh.hitv[n] = v;
         }
       }
     };
-    if (row.nvec <= kBatch) {      // the row is still in registers
+    if (TOP && tid == 0) sh.nh = sh.na = sh.nb = 0;
+
+    // ---- one pass: maximum, sum, entropy sum ----
+    uint4 raw[kLpHold];
+    float mx = -INFINITY, thr = -INFINITY;
+    Pair l2 = pair(0.f, 0.f), w2 = l2;
+    for (int v0 = 0; v0 < row.nvec; v0 += kBatch) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+      for (int u = 0; u < kLpHold; ++u) raw[u] = next[u * NT + tid];
+      if (v0 + kBatch < row.nvec) {
+        fetch(row, v0 + kBatch);
+      } else if (r + gridDim.x < R) {
+        at = row_of(r + gridDim.x);
+        fetch(RowView<T>(at, a.V), 0);
+      }
+      uint32_t best = vec_max<T>(raw[0]);
+#pragma unroll
+      for (int u = 1; u < kLpHold; ++u) best = Vec<T>::max2(best, vec_max<T>(raw[u]));
+      const float vm = Vec<T>::top(best);
+      if (!(vm <= mx)) {            // larger, or NaN
+        const float mn = max_nan(mx, vm);
+        const float d = fmaxf((mx - mn) * kLog2e, kLpFloor), f = ex2(d);  // nothing yet: f = 0
+        w2 = mul2(pair(f, f), fma2(pair(d, d), l2, w2));
+        l2 = mul2(pair(f, f), l2);
+        mx = mn;
+      }
+      const Pair nm = pair(-mx, -mx), le = pair(kLog2e, kLog2e);
+      if (VE == 8 && fabsf(mx) < Vec<T>::kNear) {
+        if constexpr (VE == 8) {
+#pragma unroll
+          for (int u = 0; u < kLpHold; ++u)
+            if (v0 + u * NT < row.nvec) {
+              const uint4 x = Vec<T>::bounded(raw[u]);
+#pragma unroll
+              for (int i = 0; i < VE / 2; ++i) {
+                const Pair t2 = mul2(add2(Vec<T>::get(x, i), nm), le);
+                const float2 t = halves(t2);
+                const Pair p = pair(ex2(t.x), ex2(t.y));
+                l2 = add2(l2, p);
+                w2 = fma2(p, t2, w2);
+              }
+            }
+        }
+      } else if (vm != -INFINITY) {  // else nothing to add (and mx may not be finite yet)
+#pragma unroll
+        for (int u = 0; u < kLpHold; ++u)
+          if (v0 + u * NT < row.nvec) {
+#pragma unroll
+            for (int i = 0; i < VE / 2; ++i) {
+              const float2 t = halves(mul2(add2(Vec<T>::get(raw[u], i), nm), le));
+              const float tx = fmaxf(t.x, kLpFloor), ty = fmaxf(t.y, kLpFloor);
+              const Pair p = pair(ex2(tx), ex2(ty));
+              l2 = add2(l2, p);
+              w2 = fma2(p, pair(tx, ty), w2);
+            }
+          }
+      }
+      // A row of several batches lists its candidates as it goes, by the first batch's
+      // threshold, which the final one is not below.
+      if (TOP && multi) {      // uniform
+        if (v0 == 0) {
+          publish(0, mx);
+          __syncthreads();
+          thr = select(0);
+        }
+#pragma unroll
+        for (int u = 0; u < kLpHold; ++u) look(raw[u], v0 + u * NT + tid, Vec<T>::twice(thr));
+      }
+    }
+    // ---- join the block: warps by shuffles, the rest by the first warp ----
+    if constexpr (TOP) publish(1, mx);
+    {
+      const float l = halves(l2).x + halves(l2).y, w = halves(w2).x + halves(w2).y;
+      const float wmx = warp_max_nan(mx);
+      const float d = fmaxf((mx - wmx) * kLog2e, kLpFloor), f = ex2(d);  // a thread without elements: l = w = 0
+      const float wl = warp_sum_f(l * f), ww = warp_sum_f(f * fmaf(d, l, w));
+      if (lane == 0) {
+        sh.wm[turn][warp] = wmx;
+        sh.wl[turn][warp] = wl;
+        sh.ww[turn][warp] = ww;
+      }
+    }
+    __syncthreads();
+    if (warp == 0) {
+      const float m = lane < kWarps ? sh.wm[turn][lane] : -INFINITY;
+      const float M = warp_max_nan(m);
+      const bool ok = fabsf(M) < INFINITY;  // else no distribution: all -inf, a NaN or +inf
+      const float d = fmaxf((m - M) * kLog2e, kLpFloor), f = ex2(d);
+      const float l0 = lane < kWarps ? sh.wl[turn][lane] : 0.f, w0 = lane < kWarps ? sh.ww[turn][lane] : 0.f;
+      const float L = warp_sum_f(l0 * f), W = warp_sum_f(f * fmaf(d, l0, w0));
+      const float ll = log2f(L), ln = logf(L);
+      if (lane == 0) {
+        sh.M = ok ? M : nan;
+        sh.ln = ln;
+        a.entropy[r] = ok ? kLn2 * (ll - W / L) : nan;
+        if (a.stats != nullptr) {
+          a.stats[2 * (long long)r] = ok ? M : nan;
+          a.stats[2 * (long long)r + 1] = ok ? ll : nan;
+        }
+        if (a.tokens != nullptr) {
+          const long long tok = a.tokens[r];
+          float lp = 0.f;
+          if (tok >= 0 && tok < a.V) lp = ok ? (Vec<T>::value(row.row[tok]) - M) - ln : nan;
+          else if (tok != -100) {
+            report(a.status, kStatusToken, kTagLogprobs);
+            lp = nan;
+          }
+          a.logprobs[r] = lp;
+        }
+      }
+    }
+    if constexpr (TOP) {
+
+    // ---- the top best ----
+    auto put = [&](float x, int e, float t) {
+      if (x > t) {
+        const int n = atomicAdd(&sh.na, 1);
+        if (n < kCap) sh.above[n] = (unsigned long long)order_key(x) << 32 | (0xffffffffu - (uint32_t)e);
+      } else if (x == t) {
+        const int n = atomicAdd(&sh.nb, 1);
+        if (n < kCap) sh.equal[n] = e;
+      }
+    };
+    // after a barrier behind the last look: the elements of the few listed vectors, or, where
+    // the list was too short, all
+    auto collect = [&](float t) {
+      const int nh = sh.nh;
+      if (nh <= kHits) {
+        for (int i = tid; i < nh; i += NT) {
+          if (!Vec<T>::reaches(vec_max<T>(sh.hit[i]), Vec<T>::twice(t))) continue;
+          const int e0 = row.first(sh.hitv[i]);
+          for (int q = 0; q < VE; ++q)
+            if (e0 + q >= 0 && e0 + q < a.V) put(Vec<T>::value(reinterpret_cast<const T*>(&sh.hit[i])[q]), e0 + q, t);
+        }
+      } else {
+        for (int e = tid; e < a.V; e += NT) put(Vec<T>::value(row.row[e]), e, t);
+      }
+      __syncthreads();
+    };
+    thr = select(1);
+    if (!multi) {
 #pragma unroll
       for (int u = 0; u < kLpHold; ++u)
-        if (u * NT < row.nvec) look(raw[u], u * NT + tid);
-    } else {
-      for (int v = tid; v < row.nvec; v += NT) look(row.bits(v), v);
+        if (u * NT < row.nvec) look(raw[u], u * NT + tid, Vec<T>::twice(thr));
+      __syncthreads();
     }
-    __syncthreads();
-    if (sh.nh <= kLpHits) {        // the elements of the few vectors that hold any
-      for (int i = tid; i < sh.nh * VE; i += NT) {
-        const int e = row.first(sh.hitv[i / VE]) + i % VE;
-        if (e >= 0 && e < a.V) put(Vec<T>::value(reinterpret_cast<const T*>(&sh.hit[i / VE])[i % VE]), e, t);
+    collect(thr);
+    const float M = sh.M, ln = sh.ln;  // the first warp's, before the barrier above
+    if (!(fabsf(M) < INFINITY)) {    // uniform
+      for (int i = tid; i < a.top; i += NT) {
+        a.top_lp[(long long)r * a.top + i] = nan;
+        a.top_tok[(long long)r * a.top + i] = -1;
       }
     } else {
-      for (int e = tid; e < a.V; e += NT) put(Vec<T>::value(row.row[e]), e, t);
-    }
-    __syncthreads();
-  };
-  collect(thr);
-  const float M = sh.M, ln = sh.ln;  // the first warp's, before the barriers above
-  if (!(fabsf(M) < INFINITY)) {    // uniform
-    for (int i = tid; i < a.top; i += NT) {
-      a.top_lp[(long long)r * a.top + i] = nan;
-      a.top_tok[(long long)r * a.top + i] = -1;
-    }
-    continue;
-  }
-  if (sh.na > kLpCap) {  // uniform: make the threshold the exact top-th largest value
-    if (tid == 0) {
-      sh.prefix = 0;
-      sh.remain = a.top;
-    }
-    for (int byte = 3; byte >= 0; --byte) {
-      __syncthreads();
-      for (int i = tid; i < 256; i += NT) sh.hist[i] = 0;
-      __syncthreads();
-      const uint32_t pre = sh.prefix;
-      for (int v = tid; v < row.nvec; v += NT) {
-        const uint4 x = row.bits(v);
+    if (sh.na > kCap) {  // uniform: make the threshold the exact top-th largest value
+      if (tid == 0) {
+        sh.prefix = 0;
+        sh.remain = a.top;
+      }
+      for (int byte = 3; byte >= 0; --byte) {
+        __syncthreads();
+        for (int i = tid; i < 256; i += NT) sh.hist[i] = 0;
+        __syncthreads();
+        const uint32_t pre = sh.prefix;
+        for (int v = tid; v < row.nvec; v += NT) {
+          const uint4 x = row.bits(v);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          const int e = row.first(v) + i;
-          const float2 f = halves(Vec<T>::get(x, i / 2));
-          const uint32_t key = order_key(i & 1 ? f.y : f.x);
-          if (e >= 0 && e < a.V && (byte == 3 || (key >> (8 * byte + 8)) == pre)) atomicAdd(&sh.hist[(key >> (8 * byte)) & 255], 1);
+          for (int i = 0; i < VE; ++i) {
+            const int e = row.first(v) + i;
+            const float2 f = halves(Vec<T>::get(x, i / 2));
+            const uint32_t key = order_key(i & 1 ? f.y : f.x);
+            if (e >= 0 && e < a.V && (byte == 3 || (key >> (8 * byte + 8)) == pre)) atomicAdd(&sh.hist[(key >> (8 * byte)) & 255], 1);
+          }
+        }
+        __syncthreads();
+        if (tid == 0) {
+          int need = sh.remain, d = 255;
+          while (d > 0 && sh.hist[d] < need) need -= sh.hist[d--];
+          sh.remain = need;
+          sh.prefix = (pre << 8) | (uint32_t)d;
         }
       }
       __syncthreads();
-      if (tid == 0) {
-        int need = sh.remain, d = 255;
-        while (d > 0 && sh.hist[d] < need) need -= sh.hist[d--];
-        sh.remain = need;
-        sh.prefix = (pre << 8) | (uint32_t)d;
-      }
-    }
-    __syncthreads();
-    thr = key_value(sh.prefix);
-    if (tid == 0) sh.nh = sh.na = sh.nb = 0;
-    __syncthreads();
-    collect(thr);
-  }
-  const int na = sh.na;
-  int nb = sh.nb;
-  if (nb > kLpCap) {  // uniform: the lowest indices equal to the threshold, by a scan in order
-    const int need = max(a.top - na, 0);
-    __syncthreads();
-    int found = 0;
-    for (int e0 = 0; e0 < a.V && found < need; e0 += NT) {
-      const int e = e0 + tid;
-      const bool hit = e < a.V && Vec<T>::value(row.row[e]) == thr;
-      const unsigned bal = __ballot_sync(0xffffffffu, hit);
-      if (lane == 0) sh.wcount[warp] = __popc(bal);
+      thr = key_value(sh.prefix);
+      if (tid == 0) sh.na = sh.nb = 0;
       __syncthreads();
-      int at = found, all = 0;
-      for (int i = 0; i < kWarps; ++i) {
-        if (i < warp) at += sh.wcount[i];
-        all += sh.wcount[i];
-      }
-      at += __popc(bal & ((1u << lane) - 1u));
-      if (hit && at < need) sh.bi[at] = e;
-      found += all;
+      for (int e = tid; e < a.V; e += NT) put(Vec<T>::value(row.row[e]), e, thr);
       __syncthreads();
     }
-    nb = need;
-  }
-  // rank: values above the threshold by (value, index), those equal to it by index behind
-  // them; a warp per candidate, a lane per rival
-  for (int i = warp; i < na + nb; i += kWarps) {
-    const bool above = i < na;
-    const float v = above ? sh.av[i] : thr;
-    const int e = above ? sh.ai[i] : sh.bi[i - na];
-    int rank = above ? 0 : na;
-    for (int q = lane; q - lane < (above ? na : nb); q += 32) {
-      bool better;
-      if (above) better = q < na && (sh.av[q] > v || (sh.av[q] == v && sh.ai[q] < e));
-      else better = q < nb && sh.bi[q] < e;
-      rank += __popc(__ballot_sync(0xffffffffu, better));
+    const int na = sh.na;
+    int nb = sh.nb;
+    if (nb > kCap) {  // uniform: the lowest indices equal to the threshold, by a scan in order
+      const int need = max(a.top - na, 0);
+      __syncthreads();
+      int found = 0;
+      for (int e0 = 0; e0 < a.V && found < need; e0 += NT) {
+        const int e = e0 + tid;
+        const bool hit = e < a.V && Vec<T>::value(row.row[e]) == thr;
+        const unsigned bal = __ballot_sync(0xffffffffu, hit);
+        if (lane == 0) sh.wcount[warp] = __popc(bal);
+        __syncthreads();
+        int at = found, all = 0;
+        for (int i = 0; i < kWarps; ++i) {
+          if (i < warp) at += sh.wcount[i];
+          all += sh.wcount[i];
+        }
+        at += __popc(bal & ((1u << lane) - 1u));
+        if (hit && at < need) sh.equal[at] = e;
+        found += all;
+        __syncthreads();
+      }
+      nb = need;
     }
-    if (lane == 0 && rank < a.top) {
-      a.top_lp[(long long)r * a.top + rank] = (v - M) - ln;
-      a.top_tok[(long long)r * a.top + rank] = e;
+    // rank: values above the threshold by (value, index), those equal to it by index behind
+    // them; four lanes share a candidate's rivals
+    for (int c = tid >> 2; c - (lane >> 2) < na + nb; c += NT / 4) {  // uniform in the warp
+      const bool above = c < na;
+      const unsigned long long key = above ? sh.above[c] : 0;
+      const int e = above ? (int)(0xffffffffu - (uint32_t)key) : c < na + nb ? sh.equal[c - na] : 0;
+      int rank = 0;
+      if (above) {
+        for (int q = tid & 3; q < na; q += 4) rank += sh.above[q] > key;
+      } else {
+        for (int q = tid & 3; q < nb; q += 4) rank += sh.equal[q] < e;
+      }
+      rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+      rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+      if (!above) rank += na;
+      if ((tid & 3) == 0 && c < na + nb && rank < a.top) {
+        a.top_lp[(long long)r * a.top + rank] = ((above ? key_value((uint32_t)(key >> 32)) : thr) - M) - ln;
+        a.top_tok[(long long)r * a.top + rank] = e;
+      }
     }
-  }
+    }
+    __syncthreads();                 // the lists are free for the next row
+    }
   }
 }
 
@@ -602,7 +642,7 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_bwd_kernel(const __gri
   }
 }
 
-template <typename T, int NT>
+template <typename T, int NT, bool TOP>
 static cudaError_t launch_fwd(const LogprobArgs& a, cudaStream_t st) {
   constexpr int smem = kLpHold * NT * 16, kDevices = 64;
   static std::atomic<int> known[kDevices];  // the device's SMs, once its shared memory is granted
@@ -613,20 +653,25 @@ static cudaError_t launch_fwd(const LogprobArgs& a, cudaStream_t st) {
   if (sms == 0) {
     e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(logprobs_fwd_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      e = cudaFuncSetAttribute(logprobs_fwd_kernel<T, NT, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     if (dev < kDevices) known[dev].store(sms, std::memory_order_relaxed);
   }
   const long long rows = a.R0 * a.R1;
-  logprobs_fwd_kernel<T, NT><<<(unsigned)std::min<long long>(rows, (long long)sms * (1024 / NT)), NT, smem, st>>>(a);
+  const unsigned grid = (unsigned)std::min<long long>(rows, (long long)sms * lp_blocks(NT, TOP));
+  logprobs_fwd_kernel<T, NT, TOP><<<grid, NT, smem, st>>>(a);
   return cudaGetLastError();
 }
 
-// Rows of up to 8 vectors a thread in 128 threads (8192 bf16 logits) run 8 to an SM;
-// longer ones take 512 threads.
+// Many rows, or short ones: 128 threads a row, 8 rows to an SM, whose joins hide behind one
+// another (8190 rows of 32000 bf16: 109 us, with 512 threads 119; 20 alternatives 193 and
+// 209).  Few rows: 512 threads a row, for the latency (600 rows, 20 alternatives: 24 and
+// 22 us); and for more alternatives than the 32 groups serve (50 of 8190: 326 and 284).
 template <typename T>
 static cudaError_t launch_fwd_t(const LogprobArgs& a, cudaStream_t st) {
-  return a.V <= kLpHold * 128 * RowView<T>::VE ? launch_fwd<T, 128>(a, st) : launch_fwd<T, 512>(a, st);
+  const bool narrow = a.V <= kLpHold * 128 * RowView<T>::VE || (a.R0 * a.R1 >= kLpManyRows && a.top <= kLpSmallTop);
+  if (a.top > 0) return narrow ? launch_fwd<T, 128, true>(a, st) : launch_fwd<T, 512, true>(a, st);
+  return narrow ? launch_fwd<T, 128, false>(a, st) : launch_fwd<T, 512, false>(a, st);
 }
 
 cudaError_t launch_logprobs_fwd(const LogprobArgs& a, int dtype, cudaStream_t st) {
