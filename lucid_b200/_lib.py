@@ -207,10 +207,14 @@ class _StatusWatch:
     def device_word(self, index: int) -> int:
         """Address of a device's status word in mapped host memory, for kernels that write
         it only on a failure: nothing is copied or queued on a call that goes well, and
-        a captured graph's replays report through it too."""
+        a captured graph's replays report through it too.  0 (nothing is recorded) for a
+        call captured before any other call has made the word: memory cannot be pinned
+        while a capture runs."""
         got = self.words.get(index)
         if got is None:
             import torch
+            if torch.cuda.is_current_stream_capturing():
+                return 0
             with self.lock:
                 if index not in self.words:
                     host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
@@ -242,7 +246,7 @@ class _StatusWatch:
     def poll(self) -> None:
         if self.pending:
             self._take(False)
-        for _, word, _ in self.words.values():
+        for _, word, _ in tuple(self.words.values()):
             if word.value:
                 self._take_words()
 

@@ -192,7 +192,9 @@ struct RowView {
   // the bits of vector v; places outside the row hold -inf
   __device__ __forceinline__ uint4 bits(int v) const {
     const int e0 = first(v);
-    if (whole(e0)) return *reinterpret_cast<const uint4*>(row + e0);
+    return whole(e0) ? *reinterpret_cast<const uint4*>(row + e0) : edge(e0);
+  }
+  __device__ __noinline__ uint4 edge(int e0) const {  // rare, and long where it is inlined
     uint4 u = make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
     T* p = reinterpret_cast<T*>(&u);
 #pragma unroll
@@ -227,8 +229,8 @@ struct LpShared {
   static constexpr int kCap = !TOP ? 1 : NT == 128 ? 256 : 512;   // list of elements above T, and of those equal to it
   static constexpr int kHits = !TOP ? 1 : NT == 128 ? 384 : 256;  // list of vectors that hold any
   __align__(16) float gmax[2][TOP ? kLpGroups : 1];
-  uint4 hit[kHits];
-  int hitv[kHits];
+  int hit[kHits];
+  uint4 kept[TOP && NT != 128 ? kHits : 1];                       // their bits (the short block reads them again)
   float wm[2][NT / 32], wl[2][NT / 32], ww[2][NT / 32];
   float T, M, ln;
   int nh, na, nb;
@@ -254,23 +256,32 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
   constexpr int kCap = LpShared<NT, TOP>::kCap, kHits = LpShared<NT, TOP>::kHits;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const unsigned R = (unsigned)(a.R0 * a.R1), R1 = (unsigned)a.R1;
+  constexpr bool kKeep = NT != 128;
   const float nan = __int_as_float(0x7fc00000);
   auto row_of = [&](unsigned r) {
     const unsigned r0 = a.R0 == 1 ? 0 : r / R1;
     return static_cast<const T*>(a.logits) + (long long)r0 * a.s0 + (long long)(r - r0 * R1) * a.s1;
   };
   const uint32_t own = (uint32_t)__cvta_generic_to_shared(&next[tid]);
-  auto fetch = [&](const RowView<T>& row, int v0) {  // this thread's vectors of the batch at v0
+  // Code size matters here: blocks are at different places of it, and what the
+  // instruction cache cannot hold they wait for.  Rare cases are loops, not unrolled.
+  auto fetch = [&](const RowView<T> row, int v0) {  // this thread's vectors of the batch at v0
     const int e0 = row.first(v0 + tid);
     const T* from = row.row + e0;
+    bool all = true;
 #pragma unroll
     for (int u = 0; u < kLpHold; ++u) {
-      if (row.whole(e0 + u * NT * VE))
+      const bool in = row.whole(e0 + u * NT * VE);
+      all = all && in;
+      if (in)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(own + u * NT * 16), "l"(from + u * NT * VE) : "memory");
-      else
-        next[u * NT + tid] = row.bits(v0 + u * NT + tid);  // partly or wholly outside: -inf there
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+    if (!all) {
+#pragma unroll 1
+      for (int u = 0; u < kLpHold; ++u)
+        if (!row.whole(e0 + u * NT * VE)) next[u * NT + tid] = row.edge(e0 + u * NT * VE);  // -inf outside
+    }
   };
   const T* at = row_of(blockIdx.x);
   fetch(RowView<T>(at, a.V), 0);
@@ -320,12 +331,28 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
       __syncthreads();
       return sh.T;
     };
-    auto look = [&](const uint4& x, int v, uint32_t t) {  // lists vector v if it reaches t
-      if (Vec<T>::reaches(vec_max<T>(x), t) && v < row.nvec) {
-        const int n = atomicAdd(&sh.nh, 1);
-        if (n < kHits) {
-          sh.hit[n] = x;
-          sh.hitv[n] = v;
+    auto look = [&](const uint4 (&x)[kLpHold], int v0, float t) {  // lists this thread's vectors that reach t
+      const uint32_t t2 = Vec<T>::twice(t);
+      if constexpr (kKeep) {
+#pragma unroll
+        for (int u = 0; u < kLpHold; ++u)
+          if (Vec<T>::reaches(vec_max<T>(x[u]), t2) && v0 + u * NT + tid < row.nvec) {
+            const int n = atomicAdd(&sh.nh, 1);
+            if (n < kHits) {
+              sh.hit[n] = v0 + u * NT + tid;
+              sh.kept[n] = x[u];
+            }
+          }
+      } else {
+        unsigned found = 0;
+#pragma unroll
+        for (int u = 0; u < kLpHold; ++u) found |= Vec<T>::reaches(vec_max<T>(x[u]), t2) ? 1u << u : 0u;
+#pragma unroll 1
+        for (; found; found &= found - 1) {
+          const int v = v0 + (__ffs(found) - 1) * NT + tid;
+          if (v >= row.nvec) break;
+          const int n = atomicAdd(&sh.nh, 1);
+          if (n < kHits) sh.hit[n] = v;
         }
       }
     };
@@ -339,12 +366,9 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
       asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
       for (int u = 0; u < kLpHold; ++u) raw[u] = next[u * NT + tid];
-      if (v0 + kBatch < row.nvec) {
-        fetch(row, v0 + kBatch);
-      } else if (r + gridDim.x < R) {
-        at = row_of(r + gridDim.x);
-        fetch(RowView<T>(at, a.V), 0);
-      }
+      const bool last = v0 + kBatch >= row.nvec;
+      if (last && r + gridDim.x < R) at = row_of(r + gridDim.x);
+      if (!last || r + gridDim.x < R) fetch(RowView<T>(at, a.V), last ? 0 : v0 + kBatch);
       uint32_t best = vec_max<T>(raw[0]);
 #pragma unroll
       for (int u = 1; u < kLpHold; ++u) best = Vec<T>::max2(best, vec_max<T>(raw[u]));
@@ -374,18 +398,24 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
             }
         }
       } else if (vm != -INFINITY) {  // else nothing to add (and mx may not be finite yet)
+        auto add = [&](const uint4& x) {
 #pragma unroll
-        for (int u = 0; u < kLpHold; ++u)
-          if (v0 + u * NT < row.nvec) {
-#pragma unroll
-            for (int i = 0; i < VE / 2; ++i) {
-              const float2 t = halves(mul2(add2(Vec<T>::get(raw[u], i), nm), le));
-              const float tx = fmaxf(t.x, kLpFloor), ty = fmaxf(t.y, kLpFloor);
-              const Pair p = pair(ex2(tx), ex2(ty));
-              l2 = add2(l2, p);
-              w2 = fma2(p, pair(tx, ty), w2);
-            }
+          for (int i = 0; i < VE / 2; ++i) {
+            const float2 t = halves(mul2(add2(Vec<T>::get(x, i), nm), le));
+            const float tx = fmaxf(t.x, kLpFloor), ty = fmaxf(t.y, kLpFloor);
+            const Pair p = pair(ex2(tx), ex2(ty));
+            l2 = add2(l2, p);
+            w2 = fma2(p, pair(tx, ty), w2);
           }
+        };
+        if constexpr (VE == 4) {
+#pragma unroll
+          for (int u = 0; u < kLpHold; ++u)
+            if (v0 + u * NT < row.nvec) add(raw[u]);
+        } else {                     // a maximum near the type's ends: rare
+#pragma unroll 1
+          for (int v = v0 + tid; v < min(row.nvec, v0 + kBatch); v += NT) add(row.bits(v));
+        }
       }
       // A row of several batches lists its candidates as it goes, by the first batch's
       // threshold, which the final one is not below.
@@ -395,8 +425,7 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
           __syncthreads();
           thr = select(0);
         }
-#pragma unroll
-        for (int u = 0; u < kLpHold; ++u) look(raw[u], v0 + u * NT + tid, Vec<T>::twice(thr));
+        look(raw, v0, thr);
       }
     }
     // ---- join the block: warps by shuffles, the rest by the first warp ----
@@ -459,10 +488,12 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
       const int nh = sh.nh;
       if (nh <= kHits) {
         for (int i = tid; i < nh; i += NT) {
-          if (!Vec<T>::reaches(vec_max<T>(sh.hit[i]), Vec<T>::twice(t))) continue;
-          const int e0 = row.first(sh.hitv[i]);
-          for (int q = 0; q < VE; ++q)
-            if (e0 + q >= 0 && e0 + q < a.V) put(Vec<T>::value(reinterpret_cast<const T*>(&sh.hit[i])[q]), e0 + q, t);
+          const uint4 x = kKeep ? sh.kept[i] : row.bits(sh.hit[i]);
+          if (!Vec<T>::reaches(vec_max<T>(x), Vec<T>::twice(t))) continue;
+          const int e0 = row.first(sh.hit[i]);
+#pragma unroll 1
+          for (int q = max(0, -e0); q < min(VE, a.V - e0); ++q)
+            put(Vec<T>::value(kKeep ? reinterpret_cast<const T*>(&sh.kept[i])[q] : row.row[e0 + q]), e0 + q, t);
         }
       } else {
         for (int e = tid; e < a.V; e += NT) put(Vec<T>::value(row.row[e]), e, t);
@@ -471,9 +502,7 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
     };
     thr = select(1);
     if (!multi) {
-#pragma unroll
-      for (int u = 0; u < kLpHold; ++u)
-        if (u * NT < row.nvec) look(raw[u], u * NT + tid, Vec<T>::twice(thr));
+      look(raw, 0, thr);
       __syncthreads();
     }
     collect(thr);
@@ -496,7 +525,7 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
         const uint32_t pre = sh.prefix;
         for (int v = tid; v < row.nvec; v += NT) {
           const uint4 x = row.bits(v);
-#pragma unroll
+#pragma unroll 1
           for (int i = 0; i < VE; ++i) {
             const int e = row.first(v) + i;
             const float2 f = halves(Vec<T>::get(x, i / 2));
@@ -663,10 +692,11 @@ static cudaError_t launch_fwd(const LogprobArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// Many rows, or short ones: 128 threads a row, 8 rows to an SM, whose joins hide behind one
-// another (8190 rows of 32000 bf16: 109 us, with 512 threads 119; 20 alternatives 193 and
-// 209).  Few rows: 512 threads a row, for the latency (600 rows, 20 alternatives: 24 and
-// 22 us); and for more alternatives than the 32 groups serve (50 of 8190: 326 and 284).
+// Many rows, or short ones: 128 threads a row, 7 or 8 rows to an SM, whose joins hide
+// behind one another (8190 rows of 32000 bf16: 98 us, with 512 threads 125; with 20
+// alternatives 174 and 230).  Few rows: 512 threads a row, for the latency (300 rows, 20
+// alternatives: 23 and 17 us; 900 rows: equal); and for more alternatives than the 32 groups
+// serve (50 of 8190 rows: 283 and 260 us).
 template <typename T>
 static cudaError_t launch_fwd_t(const LogprobArgs& a, cudaStream_t st) {
   const bool narrow = a.V <= kLpHold * 128 * RowView<T>::VE || (a.R0 * a.R1 >= kLpManyRows && a.top <= kLpSmallTop);

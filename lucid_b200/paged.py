@@ -16,7 +16,10 @@ see (a page outside the pool, a length past the block table) is not followed but
 reported: the next call of this package or ``check_status()`` raises LucidError.
 
 These operators are inference only; their outputs carry no gradient.  They can be captured
-into CUDA graphs; the workspace of a captured call belongs to its graph.
+into CUDA graphs; the workspace of a captured call belongs to its graph.  A sequence's
+results do not depend on timing, but their last bits may depend on what else is in the
+batch: the split of the cached tokens over the GPU, and so the order of the fp32 sums, follows
+all its lengths.
 """
 from __future__ import annotations
 
@@ -124,11 +127,11 @@ def paged_decode_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     (kp0, kp1, kp2, _), (xp0, xp1, xp2, _) = key_pages.stride(), x_pages.stride()
     x_new = key_pages.new_empty((B, Hkv, 1, D))
     o = key_pages.new_empty((B, 1, Hq, D))
-    nbytes = lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 1)
-    ws = lengths.new_empty(nbytes + 3 >> 2)
     with _on(index):
+        nbytes = lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 1)
+        ws = lengths.new_empty(nbytes + 3 >> 2)
         rc = lib.lucid_paged_decode_step(
-            B, Hq, Hkv, D, P, ps, block_table.shape[1], scale, eps, query.data_ptr(), q0, q1, key.data_ptr(), k0, k1,
+            B, Hq, Hkv, D, P, ps, block_table.shape[1], float(scale), float(eps), query.data_ptr(), q0, q1, key.data_ptr(), k0, k1,
             value.data_ptr(), v0, v1, key_pages.data_ptr(), kp0, kp1, kp2, x_pages.data_ptr(), xp0, xp1, xp2,
             block_table.data_ptr(), block_table.stride(0), lengths.data_ptr(), x_new.data_ptr(), Hkv * D, D,
             o.data_ptr(), Hq * D, D, append, _lib.STATUS.device_word(index), ws.data_ptr(), nbytes, _raw_stream(index))
@@ -153,11 +156,11 @@ def paged_decode_attention(query: torch.Tensor, key_pages: torch.Tensor, x_pages
     q0, q1, _, _ = query.stride()
     (kp0, kp1, kp2, _), (xp0, xp1, xp2, _) = key_pages.stride(), x_pages.stride()
     o = key_pages.new_empty((B, 1, Hq, D))
-    nbytes = lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 0)
-    ws = lengths.new_empty(nbytes + 3 >> 2)
     with _on(index):
+        nbytes = lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 0)
+        ws = lengths.new_empty(nbytes + 3 >> 2)
         rc = lib.lucid_paged_decode_attn(
-            B, Hq, Hkv, D, P, ps, block_table.shape[1], scale, query.data_ptr(), q0, q1, key_pages.data_ptr(), kp0, kp1,
+            B, Hq, Hkv, D, P, ps, block_table.shape[1], float(scale), query.data_ptr(), q0, q1, key_pages.data_ptr(), kp0, kp1,
             kp2, x_pages.data_ptr(), xp0, xp1, xp2, block_table.data_ptr(), block_table.stride(0), lengths.data_ptr(),
             o.data_ptr(), Hq * D, D, _lib.STATUS.device_word(index), ws.data_ptr(), nbytes, _raw_stream(index))
     _lib.check(rc, "lucid_paged_decode_attn")
@@ -166,7 +169,7 @@ def paged_decode_attention(query: torch.Tensor, key_pages: torch.Tensor, x_pages
 
 def paged_append(key: torch.Tensor, x: torch.Tensor, key_pages: torch.Tensor, x_pages: torch.Tensor,
                  block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None = None) -> None:
-    """Writes rows i < counts[b] (None: all N) of key and x [B,Hkv,N,D] into the rows
+    """Writes rows i < counts[b] (at most N; None: all N) of key and x [B,Hkv,N,D] into the rows
     lengths[b] + i of sequence b's pages, in place; rows past the counts (a padded batch)
     are not touched, nor are ``lengths``.  The caller has assigned the pages, and no two
     sequences of the call write the same one."""

@@ -332,6 +332,35 @@ def test_graph_replays_follow_the_lengths(cuda_device):
     _lib.check_status()
 
 
+def test_a_capture_may_be_the_first_call(cuda_device):
+    """In a fresh process, with nothing called before the capture."""
+    code = """
+import sys; sys.path.insert(0, 'tests')
+import torch, lucid_b200 as lb, test_paged_gpu as T
+s = T.make('cuda', [100, 3], 8, 2, 68, 16)
+x = torch.randn(4, 500, device='cuda'); t = torch.zeros(4, dtype=torch.int64, device='cuda')
+k = torch.ones(2, 2, 1, 68, dtype=torch.bfloat16, device='cuda')
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    o, xn = T.run_step(s, append=False)
+    lb.paged_append(k, k, s['kp'], s['xp'], s['table'], s['lens'])
+    said = lb.token_logprobs(x, t, top=3)
+g.replay(); torch.cuda.synchronize()
+T.check_step(s, o, xn)
+assert torch.equal(said.top_tokens, x.topk(3).indices)
+assert all((s['kp'][int(s['table'][b, n // 16]), :, n % 16] == 1).all() for b, n in enumerate((100, 3)))
+lb.check_status()
+print('fine')
+"""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    got = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and got.stdout.strip().endswith("fine"), got.stderr[-2000:]
+
+
 def test_two_streams_at_once(cuda_device):
     s = [make(cuda_device, [4000, 100], 8, 2, 128, 64, seed=i) for i in range(2)]
     want = [run_step(x, append=False) for x in s]
