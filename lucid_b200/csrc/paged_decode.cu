@@ -10,8 +10,9 @@
 //   S = A K^T (mma m16n8k16: exact bf16 products, fp32 sums), the scores scaled
 //   afterwards in fp32 (softmax rows by s, the update row by s rstd_new rstd_t), and
 //   acc += P X with P split into bf16 hi + lo, so that P keeps 16 bits.
-// sum(k_t^2) is the diagonal of K K^T, computed by the same instruction: the B fragment
-// of a key tile is also its A fragment.
+// sum(k_t^2) is the diagonal of K K^T, computed by the same instructions: the B fragment
+// of a key tile is also its A fragment, and with at most 8 query rows it rides in the
+// rows of A that S leaves empty.
 //
 // The cached tokens of all (sequence, kv head, row block) items are cut into tiles of
 // 64 tokens; the tiles, in item order, are dealt to the CTAs in equal contiguous
@@ -156,11 +157,18 @@ __device__ __forceinline__ void load_chunk(const unsigned char* p, uint32_t (&r)
 // Shared-memory rows: 16 tokens of each pool per warp and stage, RB bytes each (128 up to
 // D = 64, else 256), a chunk's place in its row swizzled so that the fragment reads below
 // are free of bank conflicts (8 lanes read 16-byte, 16 lanes 8-byte chunks at a time: key
-// reads take chunks 4 i + j of rows g, value reads chunks 8 c + g of rows 2 j + const).
+// reads take chunks 4 i + j of rows g; 16-byte value chunks are read by ldmatrix, 8 rows of
+// one chunk at a time, 8-byte ones as chunks 8 c + g of rows 2 j + const).
 template <int CE>
 __device__ __forceinline__ int pd_kswz(int row) { return CE == 8 ? (row & 1) * 4 : (row & 3) * 4; }
 template <int CE>
-__device__ __forceinline__ int pd_xswz(int row) { return ((row >> 1) & 3) * (CE == 8 ? 2 : 4); }
+__device__ __forceinline__ int pd_xswz(int row) { return CE == 8 ? row & 7 : ((row >> 1) & 3) * 4; }
+
+// B fragments (16 tokens x 8 columns) of two 8-column tiles from rows of values
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
 
 // How rows reach shared memory.  kRows: any strides, row by row.  kFull: rows of exactly
 // the fragments' width, the same with constant places.  kFlat: rows that follow one another
@@ -237,7 +245,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
   // this lane's copies by rows: element 32 u + lane of the 16 x nc chunks; packed as row,
   // element offset in the row, place of a key and of a value chunk in the stage
   const int nc = a.D / CE, inv_nc = (65535 + nc) / nc;   // e / nc = e inv_nc >> 16 for e < 2048
-  uint32_t todo[MODE == kFlat ? 1 : NU], place[MODE == kFlat ? 1 : NU];
+  uint32_t todo[MODE == kFlat ? 1 : NU] = {}, place[MODE == kFlat ? 1 : NU] = {};
   if constexpr (MODE != kFlat) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
@@ -251,6 +259,10 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
     for (int i = lane; i < STAGES * STAGE / 16; i += 32) *reinterpret_cast<uint4*>(own + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
     __syncwarp();
   }
+  // whole rows: consecutive u are RPU rows apart
+  constexpr int RPU = MODE == kFull ? 32 * CB / RB : 1;
+  const long long kfirst = (todo[0] & 0xff) * a.k.sn + (todo[0] >> 8), kstep = RPU * a.k.sn;
+  const long long xfirst = (todo[0] & 0xff) * a.x.sn + (todo[0] >> 8), xstep = RPU * a.x.sn;
   const bool one_page = MODE == kFlat || (a.ps & 15) == 0;  // a warp's 16 tokens never span two pages
   auto issue = [&](int st) {     // copies of the producer's tile, then the look-up of the next
     if (ahead > 0) {
@@ -272,6 +284,17 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
             copy_async<16>(dst + e, kp + from, bytes);
             copy_async<16>(dst + POOL + e, xp + from, bytes);
           }
+        }
+      } else if (MODE == kFull && one_page) {  // rows 2 u + lane / 16 of the page, inside it past `lim` too
+        const bf16* kp = a.k.p + k0 + kfirst;
+        const bf16* xp = a.x.p + x0 + xfirst;
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          const int bytes = (int)(todo[u] & 0xff) < lim ? CB : 0;
+          copy_async<CB>(dst + (place[u] & 0xffff), kp, bytes);
+          copy_async<CB>(dst + (place[u] >> 16), xp, bytes);
+          kp += kstep;
+          xp += xstep;
         }
       } else {
 #pragma unroll
@@ -301,6 +324,8 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) issue(s);
   int st = 0;                    // stage of the consumer's tile
+  // ldmatrix: lane l addresses row l & 7 (+ 8 for the odd matrices) of chunk i + l / 16
+  const int xat = POOL + ((lane & 7) + (lane & 8)) * RB, xsw = (lane >> 4) ^ (lane & 7);
 
   while (left > 0) {
     // ---- one segment: the run's tiles of one item ----
@@ -354,6 +379,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
       copy_wait<STAGES - 1>();            // this lane's copies of the tile have landed,
       __syncwarp();                          // and the other lanes'
       const unsigned char* in = own + st * STAGE;
+      const uint32_t in_s = own_s + st * STAGE;
       st = st + 1 == STAGES ? 0 : st + 1;
       const int base = (c.tile + it) * kPdTile + 16 * warp;
       if (base >= c.n) continue;             // uniform in the warp
@@ -380,9 +406,12 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
           const int ks = i * (CE / 4) + u;
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt) {
-            if constexpr (R8) mma16816(S[kt], qa[ks][0], 0u, qa[ks][1], 0u, kr[kt][i][2 * u], kr[kt][i][2 * u + 1]);
-            else mma16816(S[kt], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kr[kt][i][2 * u], kr[kt][i][2 * u + 1]);
-            if constexpr (STEP)
+            const uint32_t b0 = kr[kt][i][2 * u], b1 = kr[kt][i][2 * u + 1];
+            // rows 8-15 are free at 8 rows: the step puts the tile's own keys there, whose
+            // squared norms then come out on the diagonal of the same instruction
+            if constexpr (R8) mma16816(S[kt], qa[ks][0], STEP ? b0 : 0u, qa[ks][1], STEP ? b1 : 0u, b0, b1);
+            else mma16816(S[kt], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b0, b1);
+            if constexpr (STEP && !R8)
               mma16816(dg[kt], kr[0][i][2 * u], kr[1][i][2 * u], kr[0][i][2 * u + 1], kr[1][i][2 * u + 1],
                        kr[kt][i][2 * u], kr[kt][i][2 * u + 1]);
           }
@@ -391,8 +420,9 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
       // key q (of its tile) sits in lane 4 q + q / 2
       float rk[4] = {1.f, 1.f, 1.f, 1.f};
       if constexpr (STEP) {
-        const float v0 = rsqrtf(((g & 1) ? dg[0][1] : dg[0][0]) * inv_d + a.eps);
-        const float v1 = rsqrtf(((g & 1) ? dg[1][3] : dg[1][2]) * inv_d + a.eps);
+        const float d0 = R8 ? ((g & 1) ? S[0][3] : S[0][2]) : ((g & 1) ? dg[0][1] : dg[0][0]);
+        const float d1 = R8 ? ((g & 1) ? S[1][3] : S[1][2]) : ((g & 1) ? dg[1][3] : dg[1][2]);
+        const float v0 = rsqrtf(d0 * inv_d + a.eps), v1 = rsqrtf(d1 * inv_d + a.eps);
         rk[0] = __shfl_sync(0xffffffffu, v0, 9 * j);
         rk[1] = __shfl_sync(0xffffffffu, v0, 9 * j + 4);
         rk[2] = __shfl_sync(0xffffffffu, v1, 9 * j);
@@ -444,32 +474,46 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
           acc[i][3] *= al[1];
         }
       }
-      // values: rows 2j, 2j+1, 8+2j, 9+2j, chunk 8 c + g
-#pragma unroll
-      for (int cx = 0; cx < NX; ++cx) {
-        uint32_t xr[4][KR];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int r = 8 * (q >> 1) + 2 * j + (q & 1);
-          if constexpr (MODE == kFlat) load_chunk<KR>(in + POOL + r * 2 * a.D + (8 * cx + g) * CB, xr[q]);
-          else load_chunk<KR>(in + POOL + r * RB + ((8 * cx + g) ^ pd_xswz<CE>(2 * j)) * CB, xr[q]);
+      auto weigh = [&](float (&d)[4], uint32_t b0, uint32_t b1) {
+        if constexpr (R8) {
+          mma16816(d, phi[0], plo[0], phi[1], plo[1], b0, b1);
+        } else {
+          mma16816(d, phi[0], phi[2], phi[1], phi[3], b0, b1);
+          mma16816(d, plo[0], plo[2], plo[1], plo[3], b0, b1);
         }
+      };
+      if constexpr (CE == 8) {               // columns in order: tile i holds 8 i .. 8 i + 7
 #pragma unroll
-        for (int e = 0; e < CE; ++e) {
-          const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
-          const uint32_t b0 = __byte_perm(xr[0][e >> 1], xr[1][e >> 1], sel);
-          const uint32_t b1 = __byte_perm(xr[2][e >> 1], xr[3][e >> 1], sel);
-          if constexpr (R8) {
-            mma16816(acc[cx * CE + e], phi[0], plo[0], phi[1], plo[1], b0, b1);
-          } else {
-            mma16816(acc[cx * CE + e], phi[0], phi[2], phi[1], phi[3], b0, b1);
-            mma16816(acc[cx * CE + e], plo[0], plo[2], plo[1], plo[3], b0, b1);
+        for (int i = 0; i < NT; i += 2) {
+          uint32_t x[4];
+          ldmatrix_x4_trans(x, in_s + xat + ((i ^ xsw) << 4));
+          weigh(acc[i], x[0], x[1]);
+          weigh(acc[i + 1], x[2], x[3]);
+        }
+      } else {                               // rows 2j, 2j+1, 8+2j, 9+2j, chunk 8 c + g
+#pragma unroll
+        for (int cx = 0; cx < NX; ++cx) {
+          uint32_t xr[4][KR];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int r = 8 * (q >> 1) + 2 * j + (q & 1);
+            if constexpr (MODE == kFlat) load_chunk<KR>(in + POOL + r * 2 * a.D + (8 * cx + g) * CB, xr[q]);
+            else load_chunk<KR>(in + POOL + r * RB + ((8 * cx + g) ^ pd_xswz<CE>(2 * j)) * CB, xr[q]);
+          }
+#pragma unroll
+          for (int e = 0; e < CE; ++e) {
+            const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
+            weigh(acc[cx * CE + e], __byte_perm(xr[0][e >> 1], xr[1][e >> 1], sel),
+                  __byte_perm(xr[2][e >> 1], xr[3][e >> 1], sel));
           }
         }
       }
     }
 
     // ---- the segment's rows: merge the four warps in fixed order ----
+    auto column = [&](int i, int u) {        // of accumulator acc[i][u]
+      return CE == 8 ? 8 * i + 2 * j + u : ((i / CE) * 8 + 2 * j + u) * CE + i % CE;
+    };
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
@@ -514,7 +558,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int u = 0; u < (R8 ? 2 : 4); ++u) {
-          const int col = ((i / CE) * 8 + 2 * j + (u & 1)) * CE + i % CE;
+          const int col = column(i, u & 1);
           if (put && col < 128) red[buf][g + 8 * (u >> 1)][col] = round == 0 ? acc[i][u] * f[u >> 1] : acc[i][u];
         }
       __syncthreads();
@@ -523,7 +567,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
         for (int i = 0; i < NT; ++i)
 #pragma unroll
           for (int u = 0; u < (R8 ? 2 : 4); ++u) {
-            const int col = ((i / CE) * 8 + 2 * j + (u & 1)) * CE + i % CE;
+            const int col = column(i, u & 1);
             const float v = round == 0 ? acc[i][u] * f[u >> 1] : acc[i][u];
             if (col < 128) acc[i][u] = v + red[buf][g + 8 * (u >> 1)][col];
           }
@@ -542,7 +586,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
         for (int i = 0; i < NT; ++i)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int col = ((i / CE) * 8 + 2 * j + u) * CE + i % CE;
+            const int col = column(i, u);
             if (col < a.D) d[col] = acc[i][2 * hf + u];
           }
         if (j == 0) {
