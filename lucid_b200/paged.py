@@ -44,9 +44,11 @@ def _on(index: int):
     return _NO_GUARD if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
-def _rows(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
-    """A bf16 CUDA operand of the given shape, copied if its rows are not 8-byte aligned."""
-    if t.dtype != _BF16 or t.shape != shape or t.device != device:
+def _rows(t: torch.Tensor, name: str, shape, device):
+    """A bf16 CUDA operand of the given shape, copied if its rows are not 8-byte aligned:
+    (tensor, address, strides)."""
+    s, at = t.stride(), t.data_ptr()
+    if t.dtype is not _BF16 or t.shape != shape or t.device != device:
         if not t.is_cuda:
             raise RuntimeError(f"{name}: LUCID B200 kernels need CUDA tensors (no CPU fallback)")
         if t.dtype != _BF16:
@@ -54,14 +56,32 @@ def _rows(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
         if t.shape != shape:
             raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
         raise ValueError(f"{name} is on {t.device}, the pool on {device}")
-    s0, s1, s2, s3 = t.stride()
-    if s3 == 1 and (s0 | s1 | s2 | t.data_ptr() >> 1) & 3 == 0:
-        return t
-    return t.detach().clone(memory_format=torch.contiguous_format)  # contiguous() keeps an odd start
+    if s[3] == 1 and not (s[0] | s[1] | s[2] | at >> 1) & 3:
+        return t, at, s
+    t = t.detach().clone(memory_format=torch.contiguous_format)  # contiguous() keeps an odd start
+    return t, t.data_ptr(), t.stride()
 
 
-def _pools(key_pages: torch.Tensor, x_pages: torch.Tensor, dims: int = 4) -> None:
-    """The pools as they are: never copied, so what the kernels cannot address is refused."""
+def _pools(key_pages: torch.Tensor, x_pages: torch.Tensor, dims: int = 4):
+    """The pools as they are, never copied: what the kernels cannot address is refused.
+    Returns (device, its index, key address and strides, value address and strides)."""
+    ks, xs = key_pages.stride(), x_pages.stride()
+    kp, xp = key_pages.data_ptr(), x_pages.data_ptr()
+    device = key_pages.device
+    low = kp >> 1 | xp >> 1
+    for s in ks[:-1]:
+        low |= s
+    for s in xs[:-1]:
+        low |= s
+    if (device.type != "cuda" or key_pages.dtype is not _BF16 or x_pages.dtype is not _BF16 or len(ks) != dims
+            or x_pages.shape != key_pages.shape or x_pages.device != device or ks[-1] != 1 or xs[-1] != 1 or low & 3
+            or 0 in ks or 0 in xs):
+        _refuse_pools(key_pages, x_pages, dims)
+    return device, device.index, kp, ks, xp, xs
+
+
+def _refuse_pools(key_pages, x_pages, dims) -> None:
+    """Says what is wrong with the pools, if anything (a dimension of one may have stride 0)."""
     for t, name in ((key_pages, "key_pages"), (x_pages, "x_pages")):
         if not t.is_cuda:
             raise RuntimeError(f"{name}: LUCID B200 kernels need CUDA tensors (no CPU fallback)")
@@ -70,10 +90,7 @@ def _pools(key_pages: torch.Tensor, x_pages: torch.Tensor, dims: int = 4) -> Non
         s = t.stride()
         if len(s) != dims:
             raise ValueError(f"{name}: expected a {dims}-D pool, got shape {tuple(t.shape)}")
-        low = s[0]
-        for st in s[:-1]:
-            low |= st
-        if s[-1] != 1 or (low | t.data_ptr() >> 1) & 3 or (0 in s and any(st == 0 and n > 1 for st, n in zip(s, t.shape))):
+        if s[-1] != 1 or t.data_ptr() % 8 or any(st % 4 or st == 0 and n > 1 for st, n in zip(s[:-1], t.shape[:-1])):
             raise ValueError(f"{name}: needs a unit innermost stride, the others nonzero multiples of 4 elements, "
                              f"and an 8-byte aligned base; got strides {s}")
     if x_pages.shape != key_pages.shape or x_pages.device != key_pages.device:
@@ -81,10 +98,10 @@ def _pools(key_pages: torch.Tensor, x_pages: torch.Tensor, dims: int = 4) -> Non
                          f"{tuple(x_pages.shape)} on {x_pages.device} must match")
 
 
-def _index(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
-    """An int32 table or vector on the pool's device; None in ``shape`` is any size."""
+def _index(t: torch.Tensor, name: str, shape, device) -> int:
+    """Address of an int32 table or vector on the pool's device; None in ``shape`` is any size."""
     s = t.shape
-    if t.dtype != _INT32 or t.device != device or len(s) != len(shape) or s[0] != shape[0] or t.stride(-1) != 1 and s[-1] > 1:
+    if t.dtype is not _INT32 or t.device != device or len(s) != len(shape) or s[0] != shape[0] or t.stride(-1) != 1 and s[-1] > 1:
         if t.dtype != _INT32:
             raise TypeError(f"{name}: expected int32, got {t.dtype}")
         if t.device != device:
@@ -92,7 +109,7 @@ def _index(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
         if len(s) != len(shape) or s[0] != shape[0]:
             raise ValueError(f"{name}: expected shape {shape}, got {tuple(s)}")
         raise ValueError(f"{name}: needs a unit innermost stride")
-    return t
+    return t.data_ptr()
 
 
 def _one_token(query: torch.Tensor):
@@ -114,27 +131,24 @@ def paged_decode_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     Returns (O [B,1,Hq,D], x_new [B,Hkv,1,D])."""
     lib = _lib.load()
     _lib.STATUS.poll()
-    _pools(key_pages, x_pages)
+    dev, index, kp, ks, xp, xs = _pools(key_pages, x_pages)
     P, Hkv, ps, D = key_pages.shape
-    dev, index = key_pages.device, key_pages.get_device()
     B, Hq = _one_token(query)
-    query = _rows(query, "query", (B, Hq, 1, D), dev)
-    key = _rows(key, "key", (B, Hkv, 1, D), dev)
-    value = _rows(value, "value", (B, Hkv, 1, D), dev)
-    _index(block_table, "block_table", (B, None), dev)
-    _index(lengths, "lengths", (B,), dev)
-    (q0, q1, _, _), (k0, k1, _, _), (v0, v1, _, _) = query.stride(), key.stride(), value.stride()
-    (kp0, kp1, kp2, _), (xp0, xp1, xp2, _) = key_pages.stride(), x_pages.stride()
+    query, qp, qs = _rows(query, "query", (B, Hq, 1, D), dev)
+    key, kn, kns = _rows(key, "key", (B, Hkv, 1, D), dev)
+    value, vn, vns = _rows(value, "value", (B, Hkv, 1, D), dev)
+    table = _index(block_table, "block_table", (B, None), dev)
+    lens = _index(lengths, "lengths", (B,), dev)
     x_new = key_pages.new_empty((B, Hkv, 1, D))
     o = key_pages.new_empty((B, 1, Hq, D))
     with _on(index):
         nbytes = lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 1)
         ws = lengths.new_empty(nbytes + 3 >> 2)
         rc = lib.lucid_paged_decode_step(
-            B, Hq, Hkv, D, P, ps, block_table.shape[1], float(scale), float(eps), query.data_ptr(), q0, q1, key.data_ptr(), k0, k1,
-            value.data_ptr(), v0, v1, key_pages.data_ptr(), kp0, kp1, kp2, x_pages.data_ptr(), xp0, xp1, xp2,
-            block_table.data_ptr(), block_table.stride(0), lengths.data_ptr(), x_new.data_ptr(), Hkv * D, D,
-            o.data_ptr(), Hq * D, D, append, _lib.STATUS.device_word(index), ws.data_ptr(), nbytes, _raw_stream(index))
+            B, Hq, Hkv, D, P, ps, block_table.shape[1], float(scale), float(eps), qp, qs[0], qs[1], kn, kns[0], kns[1],
+            vn, vns[0], vns[1], kp, ks[0], ks[1], ks[2], xp, xs[0], xs[1], xs[2], table, block_table.stride(0), lens,
+            x_new.data_ptr(), Hkv * D, D, o.data_ptr(), Hq * D, D, append, _lib.STATUS.device_word(index),
+            ws.data_ptr(), nbytes, _raw_stream(index))
     _lib.check(rc, "lucid_paged_decode_step")
     return o, x_new
 
@@ -146,23 +160,20 @@ def paged_decode_attention(query: torch.Tensor, key_pages: torch.Tensor, x_pages
     cache).  query [B,Hq,1,D]; a sequence without tokens gives zeros.  Returns O [B,1,Hq,D]."""
     lib = _lib.load()
     _lib.STATUS.poll()
-    _pools(key_pages, x_pages)
+    dev, index, kp, ks, xp, xs = _pools(key_pages, x_pages)
     P, Hkv, ps, D = key_pages.shape
-    dev, index = key_pages.device, key_pages.get_device()
     B, Hq = _one_token(query)
-    query = _rows(query, "query", (B, Hq, 1, D), dev)
-    _index(block_table, "block_table", (B, None), dev)
-    _index(lengths, "lengths", (B,), dev)
-    q0, q1, _, _ = query.stride()
-    (kp0, kp1, kp2, _), (xp0, xp1, xp2, _) = key_pages.stride(), x_pages.stride()
+    query, qp, qs = _rows(query, "query", (B, Hq, 1, D), dev)
+    table = _index(block_table, "block_table", (B, None), dev)
+    lens = _index(lengths, "lengths", (B,), dev)
     o = key_pages.new_empty((B, 1, Hq, D))
     with _on(index):
         nbytes = lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 0)
         ws = lengths.new_empty(nbytes + 3 >> 2)
         rc = lib.lucid_paged_decode_attn(
-            B, Hq, Hkv, D, P, ps, block_table.shape[1], float(scale), query.data_ptr(), q0, q1, key_pages.data_ptr(), kp0, kp1,
-            kp2, x_pages.data_ptr(), xp0, xp1, xp2, block_table.data_ptr(), block_table.stride(0), lengths.data_ptr(),
-            o.data_ptr(), Hq * D, D, _lib.STATUS.device_word(index), ws.data_ptr(), nbytes, _raw_stream(index))
+            B, Hq, Hkv, D, P, ps, block_table.shape[1], float(scale), qp, qs[0], qs[1], kp, ks[0], ks[1], ks[2], xp, xs[0],
+            xs[1], xs[2], table, block_table.stride(0), lens, o.data_ptr(), Hq * D, D, _lib.STATUS.device_word(index),
+            ws.data_ptr(), nbytes, _raw_stream(index))
     _lib.check(rc, "lucid_paged_decode_attn")
     return o
 
@@ -175,26 +186,21 @@ def paged_append(key: torch.Tensor, x: torch.Tensor, key_pages: torch.Tensor, x_
     sequences of the call write the same one."""
     lib = _lib.load()
     _lib.STATUS.poll()
-    _pools(key_pages, x_pages)
+    dev, index, kp, ks, xp, xs = _pools(key_pages, x_pages)
     P, Hkv, ps, D = key_pages.shape
-    dev, index = key_pages.device, key_pages.get_device()
     if key.dim() != 4:
         raise ValueError(f"key: expected [B, Hkv, N, D], got {tuple(key.shape)}")
     B, _, N, _ = key.shape
-    key = _rows(key, "key", (B, Hkv, N, D), dev)
-    x = _rows(x, "x", (B, Hkv, N, D), dev)
-    _index(block_table, "block_table", (B, None), dev)
-    _index(lengths, "lengths", (B,), dev)
-    if counts is not None:
-        _index(counts, "counts", (B,), dev)
-    (k0, k1, k2, _), (x0, x1, x2, _) = key.stride(), x.stride()
-    (kp0, kp1, kp2, _), (xp0, xp1, xp2, _) = key_pages.stride(), x_pages.stride()
+    key, kr, krs = _rows(key, "key", (B, Hkv, N, D), dev)
+    x, xr, xrs = _rows(x, "x", (B, Hkv, N, D), dev)
+    table = _index(block_table, "block_table", (B, None), dev)
+    lens = _index(lengths, "lengths", (B,), dev)
     with _on(index):
         rc = lib.lucid_paged_append(
-            B, Hkv, N, D, P, ps, block_table.shape[1], key.data_ptr(), k0, k1, k2, x.data_ptr(), x0, x1, x2,
-            key_pages.data_ptr(), kp0, kp1, kp2, x_pages.data_ptr(), xp0, xp1, xp2, block_table.data_ptr(),
-            block_table.stride(0), lengths.data_ptr(), None if counts is None else counts.data_ptr(),
-            _lib.STATUS.device_word(index), _raw_stream(index))
+            B, Hkv, N, D, P, ps, block_table.shape[1], kr, krs[0], krs[1], krs[2], xr, xrs[0], xrs[1], xrs[2],
+            kp, ks[0], ks[1], ks[2], xp, xs[0], xs[1], xs[2], table, block_table.stride(0), lens,
+            None if counts is None else _index(counts, "counts", (B,), dev), _lib.STATUS.device_word(index),
+            _raw_stream(index))
     _lib.check(rc, "lucid_paged_append")
 
 
@@ -217,30 +223,28 @@ def copy_pages(key_pages: torch.Tensor, x_pages: torch.Tensor, src, dst) -> None
     copies is free.  A page's [Hkv,ps,D] block must be dense."""
     lib = _lib.load()
     _lib.STATUS.poll()
-    _pools(key_pages, x_pages, 5 if key_pages.dim() == 5 else 4)
     shape = key_pages.shape
+    _, index, kp, ks, xp, xs = _pools(key_pages, x_pages, 5 if len(shape) == 5 else 4)
     layers, P = (shape[0], shape[1]) if len(shape) == 5 else (1, shape[0])
     src, dst = _ids(src, "src"), _ids(dst, "dst")
     if len(src) != len(dst):
         raise ValueError(f"src names {len(src)} pages, dst {len(dst)}")
     n = shape[-3] * shape[-2] * shape[-1]
-    strides = []
-    for t, name in ((key_pages, "key_pages"), (x_pages, "x_pages")):
-        s = t.stride()
-        if s[-3:] != (shape[-2] * shape[-1], shape[-1], 1):   # the usual order; any other dense one will do
+    usual = (shape[-2] * shape[-1], shape[-1], 1)
+    for s, name in ((ks, "key_pages"), (xs, "x_pages")):
+        if s[-3:] != usual:               # any other dense order will do
             span = 1
             for st, size in sorted((st, size) for st, size in zip(s[-3:], shape[-3:]) if size > 1):
                 if st != span:
                     raise ValueError(f"{name}: the pages' [Hkv, page_size, D] blocks must be dense, got strides {s}")
                 span *= size
-        strides.append((2 * s[0] if len(shape) == 5 else 0, 2 * s[-4]))
     if len(src) == 0 or layers == 0 or n == 0:
         return
     if n % 4:
         raise ValueError(f"a page of {n} elements is not a multiple of 8 bytes")
-    index = key_pages.get_device()
     with _on(index):
-        rc = lib.lucid_copy_pages(layers, P, 2 * n, key_pages.data_ptr(), *strides[0], x_pages.data_ptr(), *strides[1],
+        rc = lib.lucid_copy_pages(layers, P, 2 * n, kp, 2 * ks[0] if len(shape) == 5 else 0, 2 * ks[-4],
+                                  xp, 2 * xs[0] if len(shape) == 5 else 0, 2 * xs[-4],
                                   src.buffer_info()[0], dst.buffer_info()[0], len(src), _raw_stream(index))
     if rc == 1:
         raise ValueError(f"copy_pages: pages must lie in [0, {P}), each dst named once and none of them a src")
