@@ -227,7 +227,7 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 template <int NT, bool TOP>
 struct LpShared {
   static constexpr int kCap = !TOP ? 1 : NT == 128 ? 256 : 512;   // list of elements above T, and of those equal to it
-  static constexpr int kHits = !TOP ? 1 : NT == 128 ? 384 : 256;  // list of vectors that hold any
+  static constexpr int kHits = !TOP ? 1 : NT == 128 ? 384 : 1024;  // list of vectors that hold any
   __align__(16) float gmax[2][TOP ? kLpGroups : 1];
   int hit[kHits];
   uint4 kept[TOP && NT != 128 ? kHits : 1];                       // their bits (the short block reads them again)
@@ -485,6 +485,23 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
     // after a barrier behind the last look: the elements of the few listed vectors, or, where
     // the list was too short, all
     auto collect = [&](float t) {
+      if (sh.nh > kHits && multi) {  // uniform: listed by a threshold below t, so once more by t
+        __syncthreads();
+        if (tid == 0) sh.nh = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int v = tid; v < row.nvec; v += NT) {
+          const uint4 x = row.bits(v);
+          if (Vec<T>::reaches(vec_max<T>(x), Vec<T>::twice(t))) {
+            const int n = atomicAdd(&sh.nh, 1);
+            if (n < kHits) {
+              sh.hit[n] = v;
+              if constexpr (kKeep) sh.kept[n] = x;
+            }
+          }
+        }
+        __syncthreads();
+      }
       const int nh = sh.nh;
       if (nh <= kHits) {
         for (int i = tid; i < nh; i += NT) {

@@ -77,6 +77,30 @@ def test_matches_64_bits(cuda_device, dtype, R, V, top):
     check(x, some_tokens(x), top)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("R,V,top", [(1000, 9001, 20), (950, 20000, 24), (950, 8192, 25), (3, 174683, 50), (901, 4097, 0)])
+def test_many_rows_and_long_rows(cuda_device, dtype, R, V, top):
+    """Both block widths over several batches of a row, the second one's alternatives listed
+    by the first one's threshold."""
+    x = rows(cuda_device, (R, V), dtype, seed=R)
+    check(x, some_tokens(x), top)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("R,V,top", [(905, 20000, 20), (2, 120000, 50)])
+def test_a_first_batch_that_says_nothing(cuda_device, dtype, R, V, top):
+    """The start of a row far below the rest, or banned: the candidate list overflows and is
+    made again by the final threshold, or, in constant rows, left for a scan."""
+    x = rows(cuda_device, (R, V), dtype, seed=V)
+    x[:, : V // 2] -= 40
+    x[0, : V // 2] = -math.inf
+    x[1] = 1.0
+    check(x, some_tokens(x), top)
+    x[0], x[0, :7] = -math.inf, 0.5
+    x[1, V // 2:] = 2.0
+    check(x, torch.zeros(R, dtype=torch.int64, device=cuda_device), top)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_views_are_read_in_place(cuda_device, dtype):
     x = rows(cuda_device, (3, 6, 1003), dtype)
