@@ -228,18 +228,19 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
   // ---- the producer's side: cursor `pc` runs ahead of `c` ----
   PdCursor pc = c;
   int ahead = left;              // tiles from the one whose offsets are in (koff, xoff)
+  int ph = pc.hb / a.nblk;       // its kv head
   long long koff = 0, xoff = 0;  // element offsets of the row of token 16 warp + (lane & 15)
   auto look_up = [&]() {
     const int tok = pc.tile * kPdTile + 16 * warp + (lane & 15);
     if (ahead > 0 && tok < pc.n) {
-      const int pi = tok / a.ps, row = tok - pi * a.ps, h = pc.hb / a.nblk;
+      const int pi = a.ps_shift >= 0 ? tok >> a.ps_shift : tok / a.ps, row = tok - pi * a.ps;
       int page = a.table[(long long)pc.b * a.t_sb + pi];
       if (page < 0 || page >= a.P) {
         report(a.status, kStatusPage, kTagPagedDecode);
         page = 0;
       }
-      koff = page * a.k.sp + h * a.k.sh + row * a.k.sn;
-      xoff = page * a.x.sp + h * a.x.sh + row * a.x.sn;
+      koff = page * a.k.sp + ph * a.k.sh + row * a.k.sn;
+      xoff = page * a.x.sp + ph * a.x.sh + row * a.x.sn;
     }
   };
   // this lane's copies by rows: element 32 u + lane of the 16 x nc chunks; packed as row,
@@ -263,6 +264,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
   constexpr int RPU = MODE == kFull ? 32 * CB / RB : 1;
   const long long kfirst = (todo[0] & 0xff) * a.k.sn + (todo[0] >> 8), kstep = RPU * a.k.sn;
   const long long xfirst = (todo[0] & 0xff) * a.x.sn + (todo[0] >> 8), xstep = RPU * a.x.sn;
+  const bool dense = MODE == kFull && (a.ps & 15) == 0 && a.k.sn == a.D && a.x.sn == a.D;
   const bool one_page = MODE == kFlat || (a.ps & 15) == 0;  // a warp's 16 tokens never span two pages
   auto issue = [&](int st) {     // copies of the producer's tile, then the look-up of the next
     if (ahead > 0) {
@@ -274,16 +276,37 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
         x0 = __shfl_sync(0xffffffffu, xoff, 0);
       }
       if constexpr (MODE == kFlat) {
-        const int most = max(0, min(lim, 16)) * a.D * 2;   // bytes of the run that are tokens
-        const bf16* kp = a.k.p + k0;
-        const bf16* xp = a.x.p + x0;
+        const uint32_t to = dst + 16 * lane;
+        const bf16* kp = a.k.p + k0 + 8 * lane;
+        const bf16* xp = a.x.p + x0 + 8 * lane;
+        if (lim >= 16) {
+#pragma unroll
+          for (int u = 0; u < NU; ++u)
+            if (u < NU - 1 || 16 * (32 * u + lane) < 32 * a.D) {
+              copy_async<16>(to + 512 * u, kp + 256 * u, 16);
+              copy_async<16>(to + POOL + 512 * u, xp + 256 * u, 16);
+            }
+        } else {
+          const int most = max(0, lim) * a.D * 2;          // bytes of the run that are tokens
+#pragma unroll 1
+          for (int u = 0; u < NU; ++u) {
+            const int e = 16 * (32 * u + lane), bytes = max(0, min(16, most - e));
+            if (e < 32 * a.D) {                            // a page's 16 rows, inside it past `lim` too
+              copy_async<16>(dst + e, kp + 256 * u, bytes);
+              copy_async<16>(dst + POOL + e, xp + 256 * u, bytes);
+            }
+          }
+        }
+      } else if (MODE == kFull && dense) {  // the 16 rows are one run
+        const bf16* kp = a.k.p + k0 + 8 * lane;
+        const bf16* xp = a.x.p + x0 + 8 * lane;
+        const uint32_t kto = dst + (place[0] & 0xffff);
+        const int rl = lim - (int)(todo[0] & 0xff);
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-          const int e = 16 * (32 * u + lane), bytes = max(0, min(16, most - e)), from = bytes > 0 ? e / 2 : 0;
-          if (e < 32 * a.D) {
-            copy_async<16>(dst + e, kp + from, bytes);
-            copy_async<16>(dst + POOL + e, xp + from, bytes);
-          }
+          const int bytes = RPU * u < rl ? CB : 0;         // rows past `lim` are in the page too
+          copy_async<CB>(kto + 512 * u, kp + 256 * u, bytes);
+          copy_async<CB>(dst + (place[u] >> 16), xp + 256 * u, bytes);
         }
       } else if (MODE == kFull && one_page) {  // rows 2 u + lane / 16 of the page, inside it past `lim` too
         const bf16* kp = a.k.p + k0 + kfirst;
@@ -315,7 +338,10 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
           }
         }
       }
-      if (--ahead > 0 && ++pc.tile == pc.nt) pd_next_item(a, pc);
+      if (--ahead > 0 && ++pc.tile == pc.nt) {
+        pd_next_item(a, pc);
+        ph = pc.hb / a.nblk;
+      }
       look_up();
     }
     copy_commit();
@@ -333,6 +359,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
     const int r_first = blk * a.rows;                      // first query row of the block
     const int nq = min(a.gq - r_first, a.rows);            // query rows of the block
     const int upd = STEP && blk == 0 ? nq : -1;            // the update row
+    const bool lone = STEP && !R8 && upd == 8;             // and nothing else in rows 8-15
     const int tiles = min(c.nt - c.tile, left);
     // operand A: rows g and g + 8
     uint32_t qa[KS][R8 ? 2 : 4];
@@ -371,7 +398,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
       for (int u = 0; u < 4; ++u) acc[i][u] = 0.f;
     float m[2], l[2] = {0.f, 0.f};
     m[0] = STEP && g == upd ? 0.f : -INFINITY;
-    m[1] = STEP && g + 8 == upd ? 0.f : -INFINITY;
+    m[1] = STEP && (g + 8 == upd || lone) ? 0.f : -INFINITY;
 
     for (int it = 0; it < tiles; ++it) {
       __syncwarp();                          // every lane has read the stage that is filled next
@@ -432,7 +459,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
       float al[2] = {1.f, 1.f};
 #pragma unroll
       for (int hf = 0; hf < (R8 ? 1 : 2); ++hf) {
-        const bool is_upd = STEP && g + 8 * hf == upd;
+        const bool is_upd = STEP && (g + 8 * hf == upd || (hf == 1 && lone));
         float z[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -444,14 +471,16 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
           for (int q = 0; q < 4; ++q)
             if (base + 8 * (q >> 1) + 2 * j + (q & 1) >= c.n) z[q] = -INFINITY;
         }
-        float mx = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // the reference point moves only when a score passes it by kPdSlack: until then
-        // the weights stay below 2^kPdSlack, whose digits fp32 and bf16 pairs hold alike
-        if (!is_upd && mx > m[hf] + kPdSlack) {
-          al[hf] = ex2(m[hf] - mx);          // 0 while nothing has been seen
-          m[hf] = mx;
+        if (!(STEP && hf == 1 && lone)) {    // uniform: the update row alone needs no maximum
+          float mx = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          // the reference point moves only when a score passes it by kPdSlack: until then
+          // the weights stay below 2^kPdSlack, whose digits fp32 and bf16 pairs hold alike
+          if (!is_upd && mx > m[hf] + kPdSlack) {
+            al[hf] = ex2(m[hf] - mx);        // 0 while nothing has been seen
+            m[hf] = mx;
+          }
         }
         const float ms = m[hf] == -INFINITY ? 0.f : m[hf];
         float p[4];

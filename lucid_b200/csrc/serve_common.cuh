@@ -32,6 +32,7 @@ struct PoolView {
 struct PagedDecodeArgs {
   int B, H, Hq, D;             // sequences, kv heads, query heads, head dimension
   int P, ps, M;                // pool pages, page size, block table width
+  int ps_shift;                // log2 of the page size, -1 if it is no power of two
   int gq, nblk, rows, nctas;   // query heads per kv head, row blocks of them, rows per block, CTAs (set by the launch)
   float s, eps;
   const bf16* q;  long long q_sb, q_sh;
