@@ -242,8 +242,8 @@ struct LpShared {
   int wcount[NT / 32];
 };
 
-// blocks to an SM: 64 registers a thread, 72 for the short block with alternatives
-constexpr int lp_blocks(int nt, bool top) { return nt == 128 && top ? 7 : 1024 / nt; }
+// blocks to an SM: 64 registers a thread, 80 for the short block with alternatives
+constexpr int lp_blocks(int nt, bool top) { return nt == 128 && top ? 6 : 1024 / nt; }
 
 // Blocks stay for many rows.  While a block works on the 8 vectors that each thread holds
 // in registers (a batch), cp.async brings the thread's next 8 (of this row or the next)
@@ -299,8 +299,11 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
 #pragma unroll
       for (int o = 1; o < kFew; o <<= 1)
         if (small || o < kMany) gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
-      const int team = small ? kFew : kMany;
-      if ((tid & (team - 1)) == 0) sh.gmax[which][tid / team] = gm;
+      if (small) {
+        if (tid % kFew == 0) sh.gmax[which][tid / kFew] = gm;
+      } else {
+        if (tid % kMany == 0) sh.gmax[which][tid / kMany] = gm;
+      }
     };
     // after a barrier: the top-th largest of them
     auto select = [&](int which) -> float {
@@ -505,12 +508,18 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
       const int nh = sh.nh;
       if (nh <= kHits) {
         for (int i = tid; i < nh; i += NT) {
-          const uint4 x = kKeep ? sh.kept[i] : row.bits(sh.hit[i]);
+          uint4 x = kKeep ? sh.kept[i] : row.bits(sh.hit[i]);
           if (!Vec<T>::reaches(vec_max<T>(x), Vec<T>::twice(t))) continue;
           const int e0 = row.first(sh.hit[i]);
 #pragma unroll 1
-          for (int q = max(0, -e0); q < min(VE, a.V - e0); ++q)
-            put(Vec<T>::value(kKeep ? reinterpret_cast<const T*>(&sh.kept[i])[q] : row.row[e0 + q]), e0 + q, t);
+          for (int q = 0; q < VE; ++q) {  // the first element, then the rest moved up
+            const float f = halves(Vec<T>::get(x, 0)).x;
+            if (f >= t && e0 + q >= 0 && e0 + q < a.V) put(f, e0 + q, t);
+            x.x = __funnelshift_rc(x.x, x.y, 128 / VE);
+            x.y = __funnelshift_rc(x.y, x.z, 128 / VE);
+            x.z = __funnelshift_rc(x.z, x.w, 128 / VE);
+            x.w = __funnelshift_rc(x.w, 0u, 128 / VE);
+          }
         }
       } else {
         for (int e = tid; e < a.V; e += NT) put(Vec<T>::value(row.row[e]), e, t);
