@@ -222,6 +222,14 @@ class _StatusWatch:
             got = self.words[index]
         return got[2]
 
+    def settle(self) -> None:
+        """After a call that reports through its device's word: waits under
+        LUCID_B200_SYNC_STATUS=1."""
+        if self.sync:
+            import torch
+            if not torch.cuda.is_current_stream_capturing():
+                self.wait_all()
+
     def _take_words(self):
         bad = []
         for index, (_, word, _) in list(self.words.items()):

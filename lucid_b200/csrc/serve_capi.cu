@@ -136,8 +136,9 @@ int lucid_paged_append(int B, int Hkv, int N, int D, int P, int ps, int M,
 int lucid_copy_pages(int layers, int P, int64_t page_bytes, void* k_pages, int64_t k_layer, int64_t k_page,
                      void* x_pages, int64_t x_layer, int64_t x_page, const int* src, const int* dst, int pairs,
                      void* stream) {
+  // at most one grid of blocks, one per 8 KB of a page, for a launch's pairs
   if (layers < 0 || P < 0 || page_bytes <= 0 || page_bytes % 8 || pairs < 0 ||
-      page_bytes / 8192 * 2 * layers > INT_MAX / kCopyPairs)
+      (page_bytes + 8191) / 8192 > INT_MAX / 2 / kCopyPairs / (layers > 0 ? layers : 1))
     return LUCID_ERR_SHAPE;
   if (pairs == 0 || layers == 0) return LUCID_OK;
   if (src == nullptr || dst == nullptr) return LUCID_ERR_SHAPE;

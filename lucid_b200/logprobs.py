@@ -60,6 +60,7 @@ def _forward(logits, tokens, top, keep):
             entropy.data_ptr(), stats.data_ptr() if keep else None, top_lp.data_ptr(), top_tok.data_ptr(),
             _lib.STATUS.device_word(index), _raw_stream(index))
     _lib.check(rc, "lucid_token_logprobs")
+    _lib.STATUS.settle()
     return logprobs, entropy, top_lp, top_tok, stats
 
 

@@ -147,9 +147,10 @@ def paged_decode_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
         rc = lib.lucid_paged_decode_step(
             B, Hq, Hkv, D, P, ps, block_table.shape[1], float(scale), float(eps), qp, qs[0], qs[1], kn, kns[0], kns[1],
             vn, vns[0], vns[1], kp, ks[0], ks[1], ks[2], xp, xs[0], xs[1], xs[2], table, block_table.stride(0), lens,
-            x_new.data_ptr(), Hkv * D, D, o.data_ptr(), Hq * D, D, append, _lib.STATUS.device_word(index),
+            x_new.data_ptr(), Hkv * D, D, o.data_ptr(), Hq * D, D, 1 if append else 0, _lib.STATUS.device_word(index),
             ws.data_ptr(), nbytes, _raw_stream(index))
     _lib.check(rc, "lucid_paged_decode_step")
+    _lib.STATUS.settle()
     return o, x_new
 
 
@@ -175,6 +176,7 @@ def paged_decode_attention(query: torch.Tensor, key_pages: torch.Tensor, x_pages
             xs[1], xs[2], table, block_table.stride(0), lens, o.data_ptr(), Hq * D, D, _lib.STATUS.device_word(index),
             ws.data_ptr(), nbytes, _raw_stream(index))
     _lib.check(rc, "lucid_paged_decode_attn")
+    _lib.STATUS.settle()
     return o
 
 
@@ -202,6 +204,7 @@ def paged_append(key: torch.Tensor, x: torch.Tensor, key_pages: torch.Tensor, x_
             None if counts is None else _index(counts, "counts", (B,), dev), _lib.STATUS.device_word(index),
             _raw_stream(index))
     _lib.check(rc, "lucid_paged_append")
+    _lib.STATUS.settle()
 
 
 def _ids(v, name: str) -> array.array:
@@ -252,11 +255,12 @@ def copy_pages(key_pages: torch.Tensor, x_pages: torch.Tensor, src, dst) -> None
 
 
 class _Sequence:
-    __slots__ = ("pages", "length")
+    __slots__ = ("pages", "length", "edits")
 
-    def __init__(self):
-        self.pages: list[int] = []
-        self.length = 0
+    def __init__(self, pages=(), length: int = 0):
+        self.pages: list[int] = list(pages)
+        self.length = length
+        self.edits = 0          # grows with every change of ``pages``
 
 
 class PagedCache:
@@ -335,8 +339,7 @@ class PagedCache:
         them goes on to fill is copied first (``PagedBatch.reserve``)."""
         pages = self.pages(sequence)
         child, = self.new()
-        self._sequences[child].pages = pages
-        self._sequences[child].length = self._sequences[sequence].length
+        self._sequences[child] = _Sequence(pages, self._sequences[sequence].length)
         for p in pages:
             self._refs[p] += 1
         self._version += 1
@@ -360,6 +363,7 @@ class PagedCache:
         to = dict(zip(src, dst))
         for s in self._sequences.values():
             s.pages = [to.get(p, p) for p in s.pages]
+            s.edits += 1
         for a, b in to.items():
             self._refs[b], self._refs[a] = self._refs[a], 0
         self._free = list(range(used, len(self._refs)))
@@ -386,7 +390,8 @@ class PagedBatch:
             cache._get(s)
         self._counts: list[int] | None = None   # reserved and not advanced yet
         self._version = -1
-        self._on_device: list[list[int]] = []
+        self._table = torch.empty(0, 0, dtype=torch.int32)   # the block table on the host
+        self._edits: list[int] = []                          # and the edits it shows
         self._host_lengths: list[int] = []
         self._host_counts: list[int] = []
         self.block_table = self.lengths = self.counts = None
@@ -430,10 +435,12 @@ class PagedBatch:
             src.append(s.pages[at])
             dst.append(c._take())
             c._refs[src[-1]] -= 1
-            s.pages = s.pages[:at] + [dst[-1]] + s.pages[at + 1:]
+            s.pages[at] = dst[-1]
+            s.edits += 1
         for s, n in zip(seqs, counts):
-            while len(s.pages) * ps < s.length + n:
-                s.pages.append(c._take())
+            if len(s.pages) * ps < s.length + n:
+                s.pages += [c._take() for _ in range(-(-(s.length + n) // ps) - len(s.pages))]
+                s.edits += 1
         if src:
             copy_pages(c.key_pages, c.x_pages, src, dst)
         self._counts, self._version = counts, c._version
@@ -442,13 +449,16 @@ class PagedBatch:
     def _upload(self, seqs, counts) -> None:
         """Brings the device tensors up to date, touching those that changed."""
         dev = self.cache.key_pages.device
-        pages = [list(s.pages) for s in seqs]
-        if pages != self._on_device or self.block_table is None:
-            width = max(1, max(map(len, pages)))
-            table = torch.full((len(pages), width), -1, dtype=torch.int32)
-            for i, row in enumerate(pages):
-                table[i, :len(row)] = torch.tensor(row, dtype=torch.int32)
-            self.block_table, self._on_device = table.to(dev), pages
+        edits = [s.edits for s in seqs]
+        if edits != self._edits or self.block_table is None:
+            width = max(1, max(len(s.pages) for s in seqs))
+            if width > self._table.shape[1]:                 # with room to grow: a page at a time is usual
+                self._table = torch.full((len(seqs), width + width // 2 + 8), -1, dtype=torch.int32)
+                self._edits = []
+            for i, s in enumerate(seqs):
+                if not self._edits or self._edits[i] != edits[i]:
+                    self._table[i, :len(s.pages)] = torch.tensor(s.pages, dtype=torch.int32)
+            self.block_table, self._edits = self._table.to(dev, copy=True), edits
         lengths = [s.length for s in seqs]
         if lengths != self._host_lengths or self.lengths is None:
             self.lengths = torch.tensor(lengths, dtype=torch.int32).to(dev)
