@@ -498,7 +498,7 @@ int lucid_copy_pages(int layers, int P, int64_t page_bytes, void* k_pages, int64
  *   entropy[r]  = -sum p log p
  *   top_tokens / top_logprobs [R][top]: the most likely tokens, likeliest first, ties to
  *                 the lowest index; top at most LUCID_MAX_TOP and V
- *   stats [R][2]: for the backward (NULL: not written)
+ *   stats [R][3]: for the backward (NULL: not written)
  * Entries of -inf have probability 0.  A row without a distribution (all -inf, a NaN or
  * +inf) gives NaN, top tokens -1.
  * lucid_token_logprobs_bwd: dlogits [R][V] (contiguous, the logits' dtype) =
@@ -510,8 +510,8 @@ int lucid_token_logprobs(int64_t R0, int64_t R1, int V, int dtype, const void* l
                          const int64_t* tokens, int top, float* logprobs, float* entropy, float* stats,
                          float* top_logprobs, int64_t* top_tokens, int* status, void* stream);
 int lucid_token_logprobs_bwd(int64_t R0, int64_t R1, int V, int dtype, const void* logits, int64_t s0, int64_t s1,
-                             const int64_t* tokens, const float* stats, const float* entropy, const float* g_logprobs,
-                             const float* g_entropy, void* dlogits, void* stream);
+                             const int64_t* tokens, const float* stats, const float* g_logprobs, const float* g_entropy,
+                             void* dlogits, void* stream);
 
 /*
  * Kernel timing hook (benchmarks).  While enabled for one kernel family,

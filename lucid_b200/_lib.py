@@ -106,7 +106,7 @@ SIGNATURES = {
                          + [c_void_p]),
     "lucid_token_logprobs": (c_int, [c_int64, c_int64, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int]
                              + [c_void_p] * 7),
-    "lucid_token_logprobs_bwd": (c_int, [c_int64, c_int64, c_int, c_int, c_void_p, c_int64, c_int64] + [c_void_p] * 7),
+    "lucid_token_logprobs_bwd": (c_int, [c_int64, c_int64, c_int, c_int, c_void_p, c_int64, c_int64] + [c_void_p] * 6),
     "lucid_selftest_umma": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "lucid_profile_enable": (c_int, [c_int]),
     "lucid_profile_read": (c_int, [c_float_p, ctypes.POINTER(c_int)]),

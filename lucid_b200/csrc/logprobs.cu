@@ -458,8 +458,9 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
         sh.ln = ln;
         a.entropy[r] = ok ? kLn2 * (ll - W / L) : nan;
         if (a.stats != nullptr) {
-          a.stats[2 * (long long)r] = ok ? M : nan;
-          a.stats[2 * (long long)r + 1] = ok ? ll : nan;
+          a.stats[3 * (long long)r] = ok ? M : nan;
+          a.stats[3 * (long long)r + 1] = ll;
+          a.stats[3 * (long long)r + 2] = kLn2 * (ll - W / L);
         }
         if (a.tokens != nullptr) {
           const long long tok = a.tokens[r];
@@ -648,9 +649,9 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_bwd_kernel(const __gri
     }
     return;
   }
-  const float M = a.stats[2 * r], ll = a.stats[2 * r + 1];
+  const float M = a.stats[3 * r], ll = a.stats[3 * r + 1];
   // -p (gl + ge (ln 2 t + H)) = p (c0 + c1 t), t = log2 p
-  const float c0 = ge != 0.f ? -(gl + ge * a.entropy[r]) : -gl, c1 = -ge * kLn2;
+  const float c0 = ge != 0.f ? -(gl + ge * a.stats[3 * r + 2]) : -gl, c1 = -ge * kLn2;
   const Pair nm = pair(-M, -M), nl = pair(-ll, -ll), le = pair(kLog2e, kLog2e), k0 = pair(c0, c0), k1 = pair(c1, c1);
   auto grad = [&](Pair x) {
     const float2 t = halves(fma2(add2(x, nm), le, nl));
@@ -722,10 +723,14 @@ static cudaError_t launch_fwd(const LogprobArgs& a, cudaStream_t st) {
 // behind one another (8190 rows of 32000 bf16: 98 us, with 512 threads 125; with 20
 // alternatives 174 and 230).  Few rows: 512 threads a row, for the latency (300 rows, 20
 // alternatives: 23 and 17 us; 900 rows: equal); and for more alternatives than the 32 groups
-// serve (50 of 8190 rows: 283 and 260 us).
+// serve (50 of 8190 rows: 283 and 260 us), or in rows of more than four short batches, whose
+// first one sets too low a threshold for them (1665 x 65060 fp32, 20
+// best: 286 and 100 us).
 template <typename T>
 static cudaError_t launch_fwd_t(const LogprobArgs& a, cudaStream_t st) {
-  const bool narrow = a.V <= kLpHold * 128 * RowView<T>::VE || (a.R0 * a.R1 >= kLpManyRows && a.top <= kLpSmallTop);
+  constexpr int kShort = kLpHold * 128 * RowView<T>::VE;  // a batch of 128 threads
+  const bool narrow = a.V <= kShort || (a.R0 * a.R1 >= kLpManyRows &&
+                                        (a.top == 0 || (a.top <= kLpSmallTop && a.V <= 4 * kShort)));
   if (a.top > 0) return narrow ? launch_fwd<T, 128, true>(a, st) : launch_fwd<T, 512, true>(a, st);
   return narrow ? launch_fwd<T, 128, false>(a, st) : launch_fwd<T, 512, false>(a, st);
 }

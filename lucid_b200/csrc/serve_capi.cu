@@ -197,18 +197,18 @@ int lucid_token_logprobs(int64_t R0, int64_t R1, int V, int dtype, const void* l
 }
 
 int lucid_token_logprobs_bwd(int64_t R0, int64_t R1, int V, int dtype, const void* logits, int64_t s0, int64_t s1,
-                             const int64_t* tokens, const float* stats, const float* entropy, const float* g_logprobs,
-                             const float* g_entropy, void* dlogits, void* stream) {
+                             const int64_t* tokens, const float* stats, const float* g_logprobs, const float* g_entropy,
+                             void* dlogits, void* stream) {
   if (!logprob_shape(R0, R1, V, dtype)) return LUCID_ERR_SHAPE;
   if (R0 == 0 || R1 == 0) return LUCID_OK;
   const unsigned es = dtype == 2 ? 4 : 2;
-  if (!ptr_ok(logits, es) || !ptr_ok(dlogits, es) || !ptr_ok(stats, 4) || !ptr_ok(entropy, 4) ||
+  if (!ptr_ok(logits, es) || !ptr_ok(dlogits, es) || !ptr_ok(stats, 4) ||
       (tokens != nullptr && !ptr_ok(tokens, 8)))
     return LUCID_ERR_ALIGN;
   LogprobArgs a{};
   a.logits = logits; a.R0 = R0; a.R1 = R1; a.s0 = s0; a.s1 = s1; a.V = V;
   a.tokens = reinterpret_cast<const long long*>(tokens);
-  a.entropy = const_cast<float*>(entropy); a.stats = const_cast<float*>(stats);
+  a.stats = const_cast<float*>(stats);
   a.g_lp = g_logprobs; a.g_ent = g_entropy; a.dlogits = dlogits;
   ProfileScope ps_(LUCID_KERNEL_LOGPROBS, stream_of(stream));
   return done(launch_logprobs_bwd(a, dtype, stream_of(stream)));

@@ -77,7 +77,7 @@ struct LogprobArgs {
   const long long* tokens;                  // [R] or null
   float* logprobs;                          // [R] (with tokens)
   float* entropy;                           // [R]
-  float* stats;                             // [R][2]: maximum and log2 of the sum (forward: or null)
+  float* stats;                             // [R][3]: maximum, log2 of the sum, entropy (forward: or null)
   float* top_lp;                            // [R][top]
   long long* top_tok;                       // [R][top]
   const float* g_lp;                        // backward: [R] or null

@@ -45,12 +45,12 @@ def _row_view(logits: torch.Tensor):
 
 def _forward(logits, tokens, top, keep):
     """The outputs, and with ``keep`` the rows' statistics for the backward."""
-    lib = _lib.load()
+    lib = _lib._lib or _lib.load()
     index, lead = logits.get_device(), logits.shape[:-1]
     view, r0, r1, s0, s1 = _row_view(logits)
     entropy = logits.new_empty(lead, dtype=torch.float32)
     logprobs = torch.empty_like(entropy) if tokens is not None else None
-    stats = entropy.new_empty((*lead, 2)) if keep else None
+    stats = entropy.new_empty((*lead, 3)) if keep else None
     top_lp = entropy.new_empty((*lead, top))
     top_tok = logits.new_empty((*lead, top), dtype=torch.int64)
     with _on(index):
@@ -65,23 +65,24 @@ def _forward(logits, tokens, top, keep):
 
 
 class TokenLogprobsFunction(torch.autograd.Function):
-    """logprobs and entropy with the gradient of the logits; the alternatives carry none."""
+    """logprobs and entropy with the gradient of the logits.  The alternatives carry none:
+    they go into the list ``beside`` and stay out of the graph."""
 
     @staticmethod
-    def forward(ctx, logits, tokens, top: int):
-        logprobs, entropy, top_lp, top_tok, stats = _forward(logits, tokens, top, True)
-        ctx.save_for_backward(logits, tokens, stats, entropy)
+    def forward(ctx, logits, tokens, top: int, beside: list):
+        logprobs, entropy, top_lp, top_tok, ctx.stats = _forward(logits, tokens, top, True)
+        ctx.save_for_backward(logits, tokens)
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(top_lp, top_tok)
-        return logprobs, entropy, top_lp, top_tok
+        beside += (top_lp, top_tok)
+        return logprobs, entropy
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logprobs, g_entropy, _top_lp, _top_tok):
+    def backward(ctx, g_logprobs, g_entropy):
         if g_logprobs is None and g_entropy is None:
-            return None, None, None
-        lib = _lib.load()
-        logits, tokens, stats, entropy = ctx.saved_tensors
+            return None, None, None, None
+        lib = _lib._lib or _lib.load()
+        logits, tokens = ctx.saved_tensors
         index = logits.get_device()
         view, r0, r1, s0, s1 = _row_view(logits)
         gl, ge = (None if g is None else g.float().contiguous() for g in (g_logprobs, g_entropy))
@@ -89,11 +90,11 @@ class TokenLogprobsFunction(torch.autograd.Function):
         with _on(index):
             rc = lib.lucid_token_logprobs_bwd(
                 r0, r1, logits.shape[-1], _DTYPES[logits.dtype], view.data_ptr(), s0, s1,
-                None if tokens is None else tokens.data_ptr(), stats.data_ptr(), entropy.data_ptr(),
+                None if tokens is None else tokens.data_ptr(), ctx.stats.data_ptr(),
                 None if gl is None else gl.data_ptr(), None if ge is None else ge.data_ptr(), dlogits.data_ptr(),
                 _raw_stream(index))
         _lib.check(rc, "lucid_token_logprobs_bwd")
-        return dlogits, None, None
+        return dlogits, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int = 0) -> TokenLogprobs:
@@ -128,5 +129,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
             tokens = tokens.to(torch.int64).contiguous()
     _lib.STATUS.poll()
     if torch.is_grad_enabled() and logits.requires_grad:
-        return TokenLogprobs(*TokenLogprobsFunction.apply(logits, tokens, top))
+        beside: list = []
+        logprobs, entropy = TokenLogprobsFunction.apply(logits, tokens, top, beside)
+        return TokenLogprobs(logprobs, entropy, *beside)
     return TokenLogprobs(*_forward(logits, tokens, top, False)[:4])

@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import array
 import contextlib
+import functools
 import heapq
 
 import torch
@@ -37,11 +38,18 @@ __all__ = ["paged_decode_step", "paged_decode_attention", "paged_append", "copy_
 _NO_GUARD = contextlib.nullcontext()
 _BF16, _INT32 = torch.bfloat16, torch.int32
 _raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(i).cuda_stream without building a Stream
+_current_device = torch._C._cuda_getDevice
 
 
 def _on(index: int):
-    """Context in which device ``index`` is the current one."""
-    return _NO_GUARD if torch.cuda.current_device() == index else torch.cuda.device(index)
+    """Context in which device ``index``, which holds a tensor, is the current one."""
+    return _NO_GUARD if _current_device() == index else torch.cuda.device(index)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_words(index: int, B: int, Hq: int, Hkv: int, D: int, step: int) -> int:
+    """Decoding workspace on device ``index`` (the current one), in 4-byte words."""
+    return _lib.load().lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, step) + 3 >> 2
 
 
 def _rows(t: torch.Tensor, name: str, shape, device):
@@ -129,7 +137,7 @@ def paged_decode_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     and its solved value are also written into row lengths[b] of sequence b, whose page the
     caller has assigned (and shares with no other sequence); ``lengths`` stays as it is.
     Returns (O [B,1,Hq,D], x_new [B,Hkv,1,D])."""
-    lib = _lib.load()
+    lib = _lib._lib or _lib.load()
     _lib.STATUS.poll()
     dev, index, kp, ks, xp, xs = _pools(key_pages, x_pages)
     P, Hkv, ps, D = key_pages.shape
@@ -142,13 +150,13 @@ def paged_decode_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     x_new = key_pages.new_empty((B, Hkv, 1, D))
     o = key_pages.new_empty((B, 1, Hq, D))
     with _on(index):
-        nbytes = lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 1)
-        ws = lengths.new_empty(nbytes + 3 >> 2)
+        words = _workspace_words(index, B, Hq, Hkv, D, 1)
+        ws = lengths.new_empty(words)
         rc = lib.lucid_paged_decode_step(
             B, Hq, Hkv, D, P, ps, block_table.shape[1], float(scale), float(eps), qp, qs[0], qs[1], kn, kns[0], kns[1],
             vn, vns[0], vns[1], kp, ks[0], ks[1], ks[2], xp, xs[0], xs[1], xs[2], table, block_table.stride(0), lens,
             x_new.data_ptr(), Hkv * D, D, o.data_ptr(), Hq * D, D, 1 if append else 0, _lib.STATUS.device_word(index),
-            ws.data_ptr(), nbytes, _raw_stream(index))
+            ws.data_ptr(), 4 * words, _raw_stream(index))
     _lib.check(rc, "lucid_paged_decode_step")
     _lib.STATUS.settle()
     return o, x_new
@@ -159,7 +167,7 @@ def paged_decode_attention(query: torch.Tensor, key_pages: torch.Tensor, x_pages
     """softmax(s q K^T) X of one new query per sequence over its ``lengths`` cached tokens
     (eager_lucid_attention_forward during decoding, the new token's row already in the
     cache).  query [B,Hq,1,D]; a sequence without tokens gives zeros.  Returns O [B,1,Hq,D]."""
-    lib = _lib.load()
+    lib = _lib._lib or _lib.load()
     _lib.STATUS.poll()
     dev, index, kp, ks, xp, xs = _pools(key_pages, x_pages)
     P, Hkv, ps, D = key_pages.shape
@@ -169,12 +177,12 @@ def paged_decode_attention(query: torch.Tensor, key_pages: torch.Tensor, x_pages
     lens = _index(lengths, "lengths", (B,), dev)
     o = key_pages.new_empty((B, 1, Hq, D))
     with _on(index):
-        nbytes = lib.lucid_paged_decode_workspace_bytes(B, Hq, Hkv, D, 0)
-        ws = lengths.new_empty(nbytes + 3 >> 2)
+        words = _workspace_words(index, B, Hq, Hkv, D, 0)
+        ws = lengths.new_empty(words)
         rc = lib.lucid_paged_decode_attn(
             B, Hq, Hkv, D, P, ps, block_table.shape[1], float(scale), qp, qs[0], qs[1], kp, ks[0], ks[1], ks[2], xp, xs[0],
             xs[1], xs[2], table, block_table.stride(0), lens, o.data_ptr(), Hq * D, D, _lib.STATUS.device_word(index),
-            ws.data_ptr(), nbytes, _raw_stream(index))
+            ws.data_ptr(), 4 * words, _raw_stream(index))
     _lib.check(rc, "lucid_paged_decode_attn")
     _lib.STATUS.settle()
     return o
@@ -186,7 +194,7 @@ def paged_append(key: torch.Tensor, x: torch.Tensor, key_pages: torch.Tensor, x_
     lengths[b] + i of sequence b's pages, in place; rows past the counts (a padded batch)
     are not touched, nor are ``lengths``.  The caller has assigned the pages, and no two
     sequences of the call write the same one."""
-    lib = _lib.load()
+    lib = _lib._lib or _lib.load()
     _lib.STATUS.poll()
     dev, index, kp, ks, xp, xs = _pools(key_pages, x_pages)
     P, Hkv, ps, D = key_pages.shape
@@ -224,7 +232,7 @@ def copy_pages(key_pages: torch.Tensor, x_pages: torch.Tensor, src, dst) -> None
     [layers,P,Hkv,ps,D] for all layers at once.  src and dst are host sequences (or CPU
     tensors) of page numbers; each dst is named once and is no src, so the order of the
     copies is free.  A page's [Hkv,ps,D] block must be dense."""
-    lib = _lib.load()
+    lib = _lib._lib or _lib.load()
     _lib.STATUS.poll()
     shape = key_pages.shape
     _, index, kp, ks, xp, xs = _pools(key_pages, x_pages, 5 if len(shape) == 5 else 4)

@@ -102,7 +102,7 @@ def test_token_logprobs_argument_errors(lib):
     assert fwd(R0=0) == 0 and fwd(R1=0) == 0
     odd = ctypes.c_void_p(4097)
     assert fwd(x=odd) == 2 and fwd(x=ODD, dtype=2) == 2 and fwd(lp=None) == 2 and fwd(ent=None) == 2 and fwd(tv=None) == 2
-    bwd = lambda V=100, x=P, d=P: lib.lucid_token_logprobs_bwd(1, 4, V, 0, x, 0, 100, P, P, P, P, P, d, None)
+    bwd = lambda V=100, x=P, d=P: lib.lucid_token_logprobs_bwd(1, 4, V, 0, x, 0, 100, P, P, P, P, d, None)
     assert bwd(V=0) == 1 and bwd(x=odd) == 2 and bwd(d=None) == 2
 
 
