@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
       for (int e = tid; e < a.V; e += NT) put(Vec<T>::value(row.row[e]), e, thr);
       __syncthreads();
     }
-    const int na = sh.na;
+    const int na = min(sh.na, kCap);  // fewer than that, unless somebody changes the row meanwhile
     int nb = sh.nb;
     if (nb > kCap) {  // uniform: the lowest indices equal to the threshold, by a scan in order
       const int need = max(a.top - na, 0);

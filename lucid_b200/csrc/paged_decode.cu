@@ -21,6 +21,11 @@
 // to slot cta + item of the workspace (each next segment has a higher cta or item, so
 // slots never collide), and the join kernel merges an item's segments in cta order:
 // results do not depend on timing.
+//
+// The products are mma.sync's: a kv head brings 1 to 16 rows a step, where a tcgen05 tile
+// has 64 or more and would hand its scores back through tensor memory for the softmax.
+// HBM bounds the pass (4 x 32765 tokens, 32 heads of 128: 2.15 GB in 327 us, 6.5 TB/s), the
+// tensor pipe is active 16 % of it.
 #include "serve_common.cuh"
 
 #include <algorithm>
@@ -141,20 +146,26 @@ __device__ __forceinline__ PdCursor pd_seek(const PagedDecodeArgs& a, long long 
     }
     acc += __shfl_sync(0xffffffffu, incl, 31);
   }
+  c.b = a.B;
   return c;
 }
 
-// the next item with at least one tile (the caller never asks past the last tile)
-__device__ __forceinline__ void pd_next_item(const PagedDecodeArgs& a, PdCursor& c) {
+// the next item with at least one tile; `left` becomes 0 behind the last sequence, which a
+// CTA with units left reaches only if somebody changes the lengths meanwhile
+__device__ __forceinline__ void pd_next_item(const PagedDecodeArgs& a, PdCursor& c, int& left) {
   c.tile = -kPdItemCost;
   if (++c.hb == a.H * a.nblk) {
     c.hb = 0;
     do {
-      ++c.b;
-      c.n = c.b < a.B ? pd_len(a, c.b) : 1;
+      if (++c.b >= a.B) {
+        left = 0;
+        return;
+      }
+      c.n = pd_len(a, c.b);
     } while (c.n == 0);
     c.nt = pd_tiles(c.n);
   }
+  pd_enter(c, left);
 }
 
 template <int KR>
@@ -201,7 +212,7 @@ struct PdShape {
   static constexpr int kRowBytes = MODE == kFlat ? 0 : kCols <= 64 ? 128 : 256;
   static constexpr int kPool = MODE == kFlat ? 16 * 2 * ((NK * 16 < kCols ? NK * 16 : kCols) - 4) : 16 * kRowBytes;  // bytes of a pool in a stage, at most
   static constexpr int kCtas = kCols <= 64 || MODE != kRows && (R8 || kCols <= 96) ? 3 : 2;
-  static constexpr int kStages = kCtas == 2 || kPool <= 3072 ? 3 : 2;
+  static constexpr int kStages = kCtas == 2 || kPool <= 2560 ? 3 : 2;
   // reads of the columns past D may run up to 192 bytes past a flat run
   static constexpr int kSmem = kPdWarps * kStages * 2 * kPool + (MODE == kFlat ? 256 : 0);
 };
@@ -235,6 +246,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
   const long long t0 = pd_div(blockIdx.x * T, G);
   int left = (int)(pd_div((blockIdx.x + 1) * T, G) - t0);  // units of this CTA
   PdCursor c = pd_seek(a, t0, lane);
+  if (c.b >= a.B) return;        // the lengths have just changed
   pd_enter(c, left);
   const float c1 = a.s * kLog2e, c2 = kLog2e / a.s, inv_d = 1.f / (float)a.D;
   unsigned char* own = ring + warp * (STAGES * STAGE);
@@ -354,8 +366,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
         }
       }
       if (--ahead > 0 && ++pc.tile == pc.nt) {
-        pd_next_item(a, pc);
-        pd_enter(pc, ahead);
+        pd_next_item(a, pc, ahead);
         ph = pc.hb / a.nblk;
       }
       look_up();
@@ -643,10 +654,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
     // ---- on to the next item ----
     left -= tiles;
     c.tile += tiles;
-    if (c.tile == c.nt && left > 0) {
-      pd_next_item(a, c);
-      pd_enter(c, left);
-    }
+    if (c.tile == c.nt && left > 0) pd_next_item(a, c, left);
   }
   copy_wait<0>();
 }

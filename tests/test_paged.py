@@ -316,3 +316,73 @@ def test_decoder_refuses_what_a_paged_cache_cannot_take(on_cpu):
     batch.advance()
     with pytest.raises(NotImplementedError, match="3 tokens"):
         model(ids, batch)
+
+
+# ---------------------------------------------------------------------------
+# the dealing out of tiles (csrc/paged_decode.cu), in plain integers
+# ---------------------------------------------------------------------------
+TILE, COST = 64, 2
+
+
+def _segments(lens, per, nctas):
+    """(cta, item, first tile, tiles) of every segment, as the tile pass walks its units."""
+    tiles = [-(-n // TILE) for n in lens]
+    units = [(t + COST if t else 0) for t in tiles]
+    T = sum(units) * per
+    G, out = min(T, nctas), []
+    for cta in range(G):
+        at, left = cta * T // G, (cta + 1) * T // G - cta * T // G
+        b = 0
+        while at >= units[b] * per:
+            at -= units[b] * per
+            b += 1
+        hb, tile = at // units[b], at % units[b] - COST
+        while left > 0:
+            skip = max(0, min(-tile, left))
+            tile, left = tile + skip, left - skip
+            if left == 0:
+                break
+            n = min(tiles[b] - tile, left)
+            out.append((cta, b * per + hb, tile, n))
+            left, tile = left - n, tile + n
+            if tile == tiles[b] and left > 0:
+                tile, hb = -COST, hb + 1
+                if hb == per:
+                    hb, b = 0, b + 1
+                    while tiles[b] == 0:
+                        b += 1
+    return out, T, G
+
+
+def test_tiles_are_dealt_out_once_and_joined_where_they_went():
+    """Every tile of every item in exactly one segment; an item's segments are those of the
+    CTAs that the join computes, all of them, in order; slots cta + item are never shared
+    and stay inside the workspace."""
+    rng = random.Random(3)
+    for trial in range(300):
+        B, per, nctas = rng.randint(1, 40), rng.choice([1, 2, 4, 6, 32]), rng.choice([1, 7, 148, 444])
+        lens = [rng.choice([0, 1, 63, 64, 65, rng.randint(1, 300), rng.randint(1, 20000)]) for _ in range(B)]
+        got, T, G = _segments(lens, per, nctas)
+        slots = [cta + item for cta, item, _, _ in got]
+        assert len(set(slots)) == len(slots) and max(slots, default=0) < nctas + B * per
+        by_item = {}
+        for cta, item, tile, n in got:
+            assert n > 0
+            by_item.setdefault(item, []).append((cta, tile, n))
+        before = 0
+        for b, n in enumerate(lens):
+            nt = -(-n // TILE)
+            for hb in range(per):
+                mine = by_item.get(b * per + hb, [])
+                if nt == 0:
+                    assert not mine
+                    continue
+                first = before + hb * (nt + COST) + COST
+                i0, i1 = ((first + 1) * G - 1) // T, ((first + nt) * G - 1) // T
+                assert [c for c, _, _ in mine] == list(range(i0, i1 + 1)), (lens, per, nctas)
+                at = 0
+                for _, tile, k in mine:
+                    assert tile == at
+                    at += k
+                assert at == nt
+            before += (nt + COST) * per if nt else 0
