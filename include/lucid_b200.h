@@ -491,8 +491,8 @@ int lucid_copy_pages(int layers, int P, int64_t page_bytes, void* k_pages, int64
 
 /*
  * Token log probabilities of rows of logits, and their gradient.  Row r0 * R1 + r1 of
- * the R0 x R1 rows starts at element r0 s0 + r1 s1; V logits a row, contiguous; dtype
- * 0 bf16, 1 fp16, 2 fp32.
+ * the R0 x R1 rows starts at element r0 s0 + r1 s1; V <= 2^30 logits a row, contiguous;
+ * dtype 0 bf16, 1 fp16, 2 fp32.
  *   logprobs[r] = log softmax(x)[tokens[r]]   (tokens NULL: not computed; token -100:
  *                 0 and no gradient)
  *   entropy[r]  = -sum p log p

@@ -172,8 +172,9 @@ int lucid_copy_pages(int layers, int P, int64_t page_bytes, void* k_pages, int64
   return LUCID_OK;
 }
 
+// V leaves room for the kernels' 32-bit element indexes to pass its end by a batch
 static bool logprob_shape(int64_t R0, int64_t R1, int V, int dtype) {
-  return R0 >= 0 && R1 >= 0 && V > 0 && V <= INT_MAX - 64 && dtype >= 0 && dtype <= 2 &&
+  return R0 >= 0 && R1 >= 0 && V > 0 && V <= 1 << 30 && dtype >= 0 && dtype <= 2 &&
          (R1 == 0 || R0 <= INT_MAX / R1);
 }
 

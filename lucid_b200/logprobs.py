@@ -27,6 +27,8 @@ class TokenLogprobs(NamedTuple):
 def _row_view(logits: torch.Tensor):
     """(logits, R0, R1, s0, s1): the rows as two strided dimensions, without a copy where
     the leading dimensions merge into two."""
+    if logits.numel() == 0:               # contiguous() leaves the strides of an empty tensor alone
+        return logits, 0, 0, 0, 0
     if logits.stride(-1) != 1 and logits.shape[-1] > 1:
         logits = logits.contiguous()
     dims = []
@@ -101,8 +103,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
     """log softmax(logits)[tokens], the entropy -sum p log p, and the ``top`` most likely
     tokens (at most 64; likeliest first, ties to the lowest index) of each row.
 
-    logits [..., V] bf16, fp16 or fp32 on CUDA (any row strides: a view such as
-    logits[:, :-1] is read in place); tokens [...] integers in [0, V), or -100 for rows
+    logits [..., V] bf16, fp16 or fp32 on CUDA, V at most 2^30 (any row strides: a view such
+    as logits[:, :-1] is read in place); tokens [...] integers in [0, V), or -100 for rows
     without one (log probability 0, no gradient through it), or None.  Entries of -inf
     have probability 0; a row without a distribution (all -inf, a NaN or +inf in it)
     gives NaN and top tokens -1.  A token outside the vocabulary is reported by the next

@@ -298,6 +298,7 @@ class PagedCache:
         self._sequences: dict[int, _Sequence] = {}
         self._next = 0
         self._version = 0                     # grows when page lists change under a batch
+        self._steps = 0                       # and this one when a batch's sequences grow
 
     @classmethod
     def for_config(cls, config, num_pages: int, page_size: int = 64, device="cuda") -> "PagedCache":
@@ -362,6 +363,8 @@ class PagedCache:
     def compact(self) -> int:
         """Moves the pages in use to the front of the pool (every page at or past the number
         in use goes to a free one before it) and returns how many moved."""
+        if torch.cuda.is_current_stream_capturing():
+            raise LucidError("PagedCache.compact works on the host: call it outside the capture")
         used = len(self._refs) - len(self._free)
         src = [p for p in range(used, len(self._refs)) if self._refs[p]]
         dst = [p for p in range(used) if not self._refs[p]]
@@ -397,7 +400,7 @@ class PagedBatch:
         for s in self.sequences:
             cache._get(s)
         self._counts: list[int] | None = None   # reserved and not advanced yet
-        self._version = -1
+        self._version = self._steps = -1
         self._table = torch.empty(0, 0, dtype=torch.int32)   # the block table on the host
         self._edits: list[int] = []                          # and the edits it shows
         self._host_lengths: list[int] = []
@@ -418,7 +421,7 @@ class PagedBatch:
     def reserve(self, counts) -> None:
         """Assigns the pages for ``counts`` more tokens of each sequence (one number for
         all, or one each) and copies shared pages that would be written.  Raises LucidError,
-        with nothing changed, when the pool has too few free pages."""
+        with nothing changed, when the pool has too few free pages or the copy fails."""
         if torch.cuda.is_current_stream_capturing():
             raise LucidError("PagedBatch.reserve works on the host: call it before the capture")
         c = self.cache
@@ -437,22 +440,23 @@ class PagedBatch:
             need += max(0, -(-(s.length + n) // ps) - len(s.pages))
         if need > len(c._free):
             raise LucidError(f"the paged cache is full: {need} pages needed, {len(c._free)} of {len(c._refs)} free")
-        src, dst = [], []
-        for s in shared:
-            at = s.length // ps
-            src.append(s.pages[at])
-            dst.append(c._take())
-            c._refs[src[-1]] -= 1
-            s.pages[at] = dst[-1]
+        src, dst = [s.pages[s.length // ps] for s in shared], [c._take() for _ in shared]
+        if src:
+            try:
+                copy_pages(c.key_pages, c.x_pages, src, dst)
+            except BaseException:                # an earlier call's error may surface there
+                c._drop(dst)
+                raise
+        for s, old, new in zip(shared, src, dst):
+            c._refs[old] -= 1
+            s.pages[s.length // ps] = new
             s.edits += 1
         for s, n in zip(seqs, counts):
             if len(s.pages) * ps < s.length + n:
                 s.pages += [c._take() for _ in range(-(-(s.length + n) // ps) - len(s.pages))]
                 s.edits += 1
-        if src:
-            copy_pages(c.key_pages, c.x_pages, src, dst)
-        self._counts, self._version = counts, c._version
         self._upload(seqs, counts)
+        self._counts, self._version, self._steps = counts, c._version, c._steps
 
     def _upload(self, seqs, counts) -> None:
         """Brings the device tensors up to date, touching those that changed."""
@@ -480,6 +484,10 @@ class PagedBatch:
             raise LucidError("reserve() the step's tokens first")
         if self._version != self.cache._version:
             raise LucidError("the cache's pages changed since reserve(): reserve again")
+        if self._steps != self.cache._steps:         # some batch has advanced: one with a sequence of this one?
+            if self.host_lengths != self._host_lengths:
+                raise LucidError("a sequence has grown in another batch since reserve(): reserve again")
+            self._steps = self.cache._steps
 
     def append(self, layer: int, key: torch.Tensor, x: torch.Tensor) -> None:
         """The reserved tokens' rows of one layer, key / x [B,Hkv,N,D] with N at least the
@@ -500,9 +508,12 @@ class PagedBatch:
 
     def advance(self) -> None:
         """Counts the reserved tokens as cached."""
+        if torch.cuda.is_current_stream_capturing():
+            raise LucidError("PagedBatch.advance works on the host: call it after the capture")
         self._check()
         for s, n in zip(self.sequences, self._counts):
             self.cache._sequences[s].length += n
         self.lengths = self.lengths + self.counts
         self._host_lengths = [a + n for a, n in zip(self._host_lengths, self._counts)]
         self._counts = None
+        self.cache._steps += 1

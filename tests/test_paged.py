@@ -106,6 +106,25 @@ def test_token_logprobs_argument_errors(lib):
     assert bwd(V=0) == 1 and bwd(x=odd) == 2 and bwd(d=None) == 2
 
 
+def test_rows_past_the_index_range_are_refused(lib):
+    """An element index runs past a row's end by a batch of vectors, within 32 bits."""
+    for V in ((1 << 30) + 1, (1 << 31) - 65):
+        assert lib.lucid_token_logprobs(1, 1, V, 0, P, 0, V, None, 0, None, P, None, None, None, None, None) == 1
+        assert lib.lucid_token_logprobs_bwd(1, 1, V, 0, P, 0, V, None, P, P, P, P, None) == 1
+
+
+def test_rows_of_logits_as_two_strided_dimensions():
+    from lucid_b200.logprobs import _row_view
+    x = torch.zeros(4, 3, 5, 8)
+    assert _row_view(x)[1:] == (1, 60, 0, 8)
+    assert _row_view(x[:, :, :-1])[1:] == (12, 4, 40, 8)
+    assert _row_view(x[:, :2, :-1])[1:] == (1, 32, 0, 8)                    # three strides: copied
+    assert _row_view(x[0, 0, 0])[1:3] == (1, 1)
+    assert _row_view(x[:1].expand(4, 3, 5, 8))[1:] == (4, 15, 0, 8)
+    for empty in (x[:, :, :0], torch.zeros(0, 3, 2, 8).transpose(0, 2), x[:0]):
+        assert 0 in _row_view(empty)[1:3]                                   # and it returns
+
+
 def test_status_words_name_their_cause():
     assert _lib.decode_status(4 | (16 << 20)).startswith("paged decoding: a page of the block table")
     assert _lib.decode_status(5 | (17 << 20)).startswith("paged append: a length or a new row lies past")
@@ -264,6 +283,58 @@ def test_reserve_again_and_stale_batches(on_cpu):
     cache.free(b)
     with pytest.raises(_lib.LucidError, match="not in the cache"):
         batch.reserve(1)
+
+
+def test_two_batches_with_the_same_sequence(on_cpu):
+    """The one that advances first wins; the other would write over its rows."""
+    cache = _cache()
+    a, b, c = cache.new(3)
+    one, two, other = cache.batch([a, b]), cache.batch([b]), cache.batch([c])
+    k = torch.zeros(2, 1, 1, 4, dtype=torch.bfloat16)
+    for batch in (one, two, other):
+        batch.reserve(1)
+    two.append(0, k[:1], k[:1])
+    two.advance()
+    for call in (lambda: one.append(0, k, k), one.advance):
+        with pytest.raises(_lib.LucidError, match="another batch"):
+            call()
+    other.append(0, k[:1], k[:1])                                 # shares nothing with it
+    other.advance()
+    one.reserve(1)
+    one.advance()
+    assert [cache.length(s) for s in (a, b, c)] == [1, 2, 1]
+
+
+def test_a_failing_page_copy_changes_nothing(on_cpu, monkeypatch):
+    """copy_pages also raises what an earlier call reported."""
+    cache = _cache()
+    a, = cache.new()
+    _write(cache.batch([a]), [2], [[1, 2]])
+    child = cache.fork(a)
+    refs, free, batch = list(cache._refs), cache.free_pages, cache.batch([child])
+
+    def fails(*args):
+        raise _lib.LucidError("reported before")
+    with monkeypatch.context() as m:
+        m.setattr(paged, "copy_pages", fails)
+        with pytest.raises(_lib.LucidError, match="reported before"):
+            batch.reserve(3)
+    assert cache._refs == refs and cache.free_pages == free and cache.pages(a) == cache.pages(child)
+    with pytest.raises(_lib.LucidError, match="reserve"):
+        batch.advance()
+    _write(batch, [1], [[3]])
+    assert _held(cache, child, 0) == [1, 2, 3] and _held(cache, a, 0) == [1, 2]
+
+
+def test_bookkeeping_stays_out_of_captures(on_cpu, monkeypatch):
+    cache = _cache()
+    batch = cache.batch(cache.new())
+    batch.reserve(1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for call in (lambda: batch.reserve(1), batch.advance, cache.compact):
+        with pytest.raises(_lib.LucidError, match="works on the host"):
+            call()
+    assert batch.host_lengths == [0]
 
 
 def test_refusals_of_the_cache(on_cpu):
