@@ -29,6 +29,7 @@ constexpr int kLpGroups = 128;   // groups of threads
 constexpr int kLpHold = 8;       // vectors a thread holds: 32768 bf16 logits in 512 threads
 constexpr int kLpBwdHold = 4;
 constexpr int kLpManyRows = 900;
+constexpr int kLpWarpRows = 3000, kLpWarpBatches = 32;
 constexpr int kLpSmallTop = 24;  // up to here 32 group maxima do
 constexpr float kLpFloor = -200.f;  // 2^-200 is 0 in fp32; keeps 0 * -inf out of w
 
@@ -224,6 +225,134 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 
+// This thread's vectors of the batch at v0 into its own places next[u NT]: cp.async, and
+// what lies over the row's ends with -inf outside.
+// Code size matters here: blocks are at different places of it, and what the
+// instruction cache cannot hold they wait for.  Rare cases are loops, not unrolled.
+template <typename T, int NT>
+__device__ __forceinline__ void lp_fetch(const RowView<T> row, int v0, int tid, uint4* next) {
+  constexpr int VE = RowView<T>::VE;
+  const uint32_t own = (uint32_t)__cvta_generic_to_shared(next);
+  const int e0 = row.first(v0 + tid);
+  const T* from = row.row + e0;
+  bool all = true;
+#pragma unroll
+  for (int u = 0; u < kLpHold; ++u) {
+    const bool in = row.whole(e0 + u * NT * VE);
+    all = all && in;
+    if (in)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(own + u * NT * 16), "l"(from + u * NT * VE) : "memory");
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  if (!all) {
+#pragma unroll 1
+    for (int u = 0; u < kLpHold; ++u)
+      if (!row.whole(e0 + u * NT * VE)) next[u * NT] = row.edge(e0 + u * NT * VE);  // -inf outside
+  }
+}
+
+// (m, l, w) of a thread
+struct Sums {
+  float mx = -INFINITY;
+  Pair l2 = pair(0.f, 0.f), w2 = pair(0.f, 0.f);
+
+  __device__ __forceinline__ void raise(float vm) {  // to a batch with maximum vm
+    if (!(vm <= mx)) {            // larger, or NaN
+      const float mn = max_nan(mx, vm);
+      const float d = fmaxf((mx - mn) * kLog2e, kLpFloor), f = ex2(d);  // nothing yet: f = 0
+      w2 = mul2(pair(f, f), fma2(pair(d, d), l2, w2));
+      l2 = mul2(pair(f, f), l2);
+      mx = mn;
+    }
+  }
+
+  template <typename T, int NT>
+  __device__ __forceinline__ void add(const RowView<T>& row, const uint4 (&raw)[kLpHold], int v0, int tid, float vm) {
+    constexpr int VE = RowView<T>::VE;
+    const Pair nm = pair(-mx, -mx), le = pair(kLog2e, kLog2e);
+    if (VE == 8 && fabsf(mx) < Vec<T>::kNear) {
+      if constexpr (VE == 8) {
+#pragma unroll
+        for (int u = 0; u < kLpHold; ++u)
+          if (v0 + u * NT < row.nvec) {
+            const uint4 x = Vec<T>::bounded(raw[u]);
+#pragma unroll
+            for (int i = 0; i < VE / 2; ++i) {
+              const Pair t2 = mul2(add2(Vec<T>::get(x, i), nm), le);
+              const float2 t = halves(t2);
+              const Pair p = pair(ex2(t.x), ex2(t.y));
+              l2 = add2(l2, p);
+              w2 = fma2(p, t2, w2);
+            }
+          }
+      }
+    } else if (vm != -INFINITY) {  // else nothing to add (and mx may not be finite yet)
+      auto one = [&](const uint4& x) {
+#pragma unroll
+        for (int i = 0; i < VE / 2; ++i) {
+          const float2 t = halves(mul2(add2(Vec<T>::get(x, i), nm), le));
+          const float tx = fmaxf(t.x, kLpFloor), ty = fmaxf(t.y, kLpFloor);
+          const Pair p = pair(ex2(tx), ex2(ty));
+          l2 = add2(l2, p);
+          w2 = fma2(p, pair(tx, ty), w2);
+        }
+      };
+      if constexpr (VE == 4) {
+#pragma unroll
+        for (int u = 0; u < kLpHold; ++u)
+          if (v0 + u * NT < row.nvec) one(raw[u]);
+      } else {                     // a maximum near the type's ends: rare
+#pragma unroll 1
+        for (int v = v0 + tid; v < min(row.nvec, v0 + kLpHold * NT); v += NT) one(row.bits(v));
+      }
+    }
+  }
+
+  __device__ __forceinline__ void join_warp() {  // all lanes get the warp's
+    const float l = halves(l2).x + halves(l2).y, w = halves(w2).x + halves(w2).y;
+    const float M = warp_max_nan(mx);
+    const float d = fmaxf((mx - M) * kLog2e, kLpFloor), f = ex2(d);  // a thread without elements: l = w = 0
+    l2 = pair(warp_sum_f(l * f), 0.f);
+    w2 = pair(warp_sum_f(f * fmaf(d, l, w)), 0.f);
+    mx = M;
+  }
+};
+
+// the warp's values sorted, largest first; the k-th of them
+__device__ __forceinline__ float warp_kth(float v, int lane, int k) {
+#pragma unroll
+  for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+    for (int o = n >> 1; o > 0; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, v, o);
+      v = ((lane & o) == 0) == ((lane & n) == 0) ? fmaxf(v, other) : fminf(v, other);
+    }
+  return __shfl_sync(0xffffffffu, v, k - 1);
+}
+
+// one row's outputs but the alternatives, from its joined sums
+template <typename T>
+__device__ __forceinline__ void lp_write(const LogprobArgs& a, const RowView<T>& row, long long r, bool ok, float M, float ll,
+                                         float ln, float W, float L) {
+  const float nan = __int_as_float(0x7fc00000), H = kLn2 * (ll - W / L);
+  a.entropy[r] = ok ? H : nan;
+  if (a.stats != nullptr) {
+    a.stats[3 * r] = ok ? M : nan;
+    a.stats[3 * r + 1] = ll;
+    a.stats[3 * r + 2] = H;
+  }
+  if (a.tokens != nullptr) {
+    const long long tok = a.tokens[r];
+    float lp = 0.f;
+    if (tok >= 0 && tok < a.V) lp = ok ? (Vec<T>::value(row.row[tok]) - M) - ln : nan;
+    else if (tok != -100) {
+      report(a.status, kStatusToken, kTagLogprobs);
+      lp = nan;
+    }
+    a.logprobs[r] = lp;
+  }
+}
+
 template <int NT, bool TOP>
 struct LpShared {
   static constexpr int kCap = !TOP ? 1 : NT == 128 ? 256 : 512;   // list of elements above T, and of those equal to it
@@ -262,29 +391,8 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
     const unsigned r0 = a.R0 == 1 ? 0 : r / R1;
     return static_cast<const T*>(a.logits) + (long long)r0 * a.s0 + (long long)(r - r0 * R1) * a.s1;
   };
-  const uint32_t own = (uint32_t)__cvta_generic_to_shared(&next[tid]);
-  // Code size matters here: blocks are at different places of it, and what the
-  // instruction cache cannot hold they wait for.  Rare cases are loops, not unrolled.
-  auto fetch = [&](const RowView<T> row, int v0) {  // this thread's vectors of the batch at v0
-    const int e0 = row.first(v0 + tid);
-    const T* from = row.row + e0;
-    bool all = true;
-#pragma unroll
-    for (int u = 0; u < kLpHold; ++u) {
-      const bool in = row.whole(e0 + u * NT * VE);
-      all = all && in;
-      if (in)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(own + u * NT * 16), "l"(from + u * NT * VE) : "memory");
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    if (!all) {
-#pragma unroll 1
-      for (int u = 0; u < kLpHold; ++u)
-        if (!row.whole(e0 + u * NT * VE)) next[u * NT + tid] = row.edge(e0 + u * NT * VE);  // -inf outside
-    }
-  };
   const T* at = row_of(blockIdx.x);
-  fetch(RowView<T>(at, a.V), 0);
+  lp_fetch<T, NT>(RowView<T>(at, a.V), 0, tid, next + tid);
   // Without alternatives a row has one barrier: a warp may be at its next row while others
   // read this row's sums, which the rows therefore keep in turn.
   int turn = 0;
@@ -308,15 +416,7 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
     // after a barrier: the top-th largest of them
     auto select = [&](int which) -> float {
       if (small) {                   // every warp sorts the 32, largest first
-        float v = sh.gmax[which][lane];
-#pragma unroll
-        for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-          for (int o = k >> 1; o > 0; o >>= 1) {
-            const float other = __shfl_xor_sync(0xffffffffu, v, o);
-            v = ((lane & o) == 0) == ((lane & k) == 0) ? fmaxf(v, other) : fminf(v, other);
-          }
-        return __shfl_sync(0xffffffffu, v, a.top - 1);
+        return warp_kth(sh.gmax[which][lane], lane, a.top);
       }
       constexpr int kTeam = NT / kLpGroups;  // NT / 128 threads rank each of 128
       const int me = tid / kTeam;
@@ -363,68 +463,26 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
 
     // ---- one pass: maximum, sum, entropy sum ----
     uint4 raw[kLpHold];
-    float mx = -INFINITY, thr = -INFINITY;
-    Pair l2 = pair(0.f, 0.f), w2 = l2;
+    float thr = -INFINITY;
+    Sums sums;
     for (int v0 = 0; v0 < row.nvec; v0 += kBatch) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
       for (int u = 0; u < kLpHold; ++u) raw[u] = next[u * NT + tid];
       const bool last = v0 + kBatch >= row.nvec;
       if (last && r + gridDim.x < R) at = row_of(r + gridDim.x);
-      if (!last || r + gridDim.x < R) fetch(RowView<T>(at, a.V), last ? 0 : v0 + kBatch);
+      if (!last || r + gridDim.x < R) lp_fetch<T, NT>(RowView<T>(at, a.V), last ? 0 : v0 + kBatch, tid, next + tid);
       uint32_t best = vec_max<T>(raw[0]);
 #pragma unroll
       for (int u = 1; u < kLpHold; ++u) best = Vec<T>::max2(best, vec_max<T>(raw[u]));
       const float vm = Vec<T>::top(best);
-      if (!(vm <= mx)) {            // larger, or NaN
-        const float mn = max_nan(mx, vm);
-        const float d = fmaxf((mx - mn) * kLog2e, kLpFloor), f = ex2(d);  // nothing yet: f = 0
-        w2 = mul2(pair(f, f), fma2(pair(d, d), l2, w2));
-        l2 = mul2(pair(f, f), l2);
-        mx = mn;
-      }
-      const Pair nm = pair(-mx, -mx), le = pair(kLog2e, kLog2e);
-      if (VE == 8 && fabsf(mx) < Vec<T>::kNear) {
-        if constexpr (VE == 8) {
-#pragma unroll
-          for (int u = 0; u < kLpHold; ++u)
-            if (v0 + u * NT < row.nvec) {
-              const uint4 x = Vec<T>::bounded(raw[u]);
-#pragma unroll
-              for (int i = 0; i < VE / 2; ++i) {
-                const Pair t2 = mul2(add2(Vec<T>::get(x, i), nm), le);
-                const float2 t = halves(t2);
-                const Pair p = pair(ex2(t.x), ex2(t.y));
-                l2 = add2(l2, p);
-                w2 = fma2(p, t2, w2);
-              }
-            }
-        }
-      } else if (vm != -INFINITY) {  // else nothing to add (and mx may not be finite yet)
-        auto add = [&](const uint4& x) {
-#pragma unroll
-          for (int i = 0; i < VE / 2; ++i) {
-            const float2 t = halves(mul2(add2(Vec<T>::get(x, i), nm), le));
-            const float tx = fmaxf(t.x, kLpFloor), ty = fmaxf(t.y, kLpFloor);
-            const Pair p = pair(ex2(tx), ex2(ty));
-            l2 = add2(l2, p);
-            w2 = fma2(p, pair(tx, ty), w2);
-          }
-        };
-        if constexpr (VE == 4) {
-#pragma unroll
-          for (int u = 0; u < kLpHold; ++u)
-            if (v0 + u * NT < row.nvec) add(raw[u]);
-        } else {                     // a maximum near the type's ends: rare
-#pragma unroll 1
-          for (int v = v0 + tid; v < min(row.nvec, v0 + kBatch); v += NT) add(row.bits(v));
-        }
-      }
+      sums.raise(vm);
+      sums.add<T, NT>(row, raw, v0, tid, vm);
       // A row of several batches lists its candidates as it goes, by the first batch's
       // threshold, which the final one is not below.
       if (TOP && multi) {      // uniform
         if (v0 == 0) {
-          publish(0, mx);
+          publish(0, sums.mx);
           __syncthreads();
           thr = select(0);
         }
@@ -432,17 +490,12 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
       }
     }
     // ---- join the block: warps by shuffles, the rest by the first warp ----
-    if constexpr (TOP) publish(1, mx);
-    {
-      const float l = halves(l2).x + halves(l2).y, w = halves(w2).x + halves(w2).y;
-      const float wmx = warp_max_nan(mx);
-      const float d = fmaxf((mx - wmx) * kLog2e, kLpFloor), f = ex2(d);  // a thread without elements: l = w = 0
-      const float wl = warp_sum_f(l * f), ww = warp_sum_f(f * fmaf(d, l, w));
-      if (lane == 0) {
-        sh.wm[turn][warp] = wmx;
-        sh.wl[turn][warp] = wl;
-        sh.ww[turn][warp] = ww;
-      }
+    if constexpr (TOP) publish(1, sums.mx);
+    sums.join_warp();
+    if (lane == 0) {
+      sh.wm[turn][warp] = sums.mx;
+      sh.wl[turn][warp] = halves(sums.l2).x;
+      sh.ww[turn][warp] = halves(sums.w2).x;
     }
     __syncthreads();
     if (warp == 0) {
@@ -456,22 +509,7 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
       if (lane == 0) {
         sh.M = ok ? M : nan;
         sh.ln = ln;
-        a.entropy[r] = ok ? kLn2 * (ll - W / L) : nan;
-        if (a.stats != nullptr) {
-          a.stats[3 * (long long)r] = ok ? M : nan;
-          a.stats[3 * (long long)r + 1] = ll;
-          a.stats[3 * (long long)r + 2] = kLn2 * (ll - W / L);
-        }
-        if (a.tokens != nullptr) {
-          const long long tok = a.tokens[r];
-          float lp = 0.f;
-          if (tok >= 0 && tok < a.V) lp = ok ? (Vec<T>::value(row.row[tok]) - M) - ln : nan;
-          else if (tok != -100) {
-            report(a.status, kStatusToken, kTagLogprobs);
-            lp = nan;
-          }
-          a.logprobs[r] = lp;
-        }
+        lp_write<T>(a, row, r, ok, M, ll, ln, W, L);
       }
     }
     if constexpr (TOP) {
@@ -625,6 +663,209 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
   }
 }
 
+// Many rows with up to kLpSmallTop alternatives: a warp (a block of 32 threads) to a row,
+// without any barrier.  The lanes' maxima are the groups; their top-th largest is taken
+// anew whenever the batches seen have doubled.  What is listed meanwhile is a lane's whole
+// batch with its maximum, where that reaches the threshold: one test for 64 elements, and
+// the final threshold drops most of the list (122 of a row of 16 batches with 20
+// alternatives) without a look at its elements.
+constexpr int kLpWarpBlocks = 24;
+constexpr int kLpWarpHits = 320;
+constexpr int kLpWarpCap = 192;  // (kLpSmallTop - 1) vectors, with lanes without one
+struct LpWarpShared {
+  uint4 next[kLpHold * 32];
+  union {
+    float most[kLpWarpHits];     // a listed batch's maximum, then
+    int hit[kLpWarpHits];        // the vectors that reach the final threshold
+  };
+  union {
+    unsigned long long best[kLpWarpCap];  // elements, (value, lowest index first) as one key
+    int hist[256];
+  };
+  int equal[kLpWarpCap];
+  unsigned short from[kLpWarpHits];  // batch and lane
+};
+
+template <typename T>
+__global__ void __launch_bounds__(32, kLpWarpBlocks) logprobs_warp_kernel(const __grid_constant__ LogprobArgs a) {
+  __shared__ __align__(16) LpWarpShared sh;
+  constexpr int VE = RowView<T>::VE, kBatch = kLpHold * 32;
+  const int lane = threadIdx.x;
+  const unsigned below = (1u << lane) - 1u;
+  const unsigned R = (unsigned)(a.R0 * a.R1), R1 = (unsigned)a.R1;
+  auto row_of = [&](unsigned r) {
+    const unsigned r0 = a.R0 == 1 ? 0 : r / R1;
+    return static_cast<const T*>(a.logits) + (long long)r0 * a.s0 + (long long)(r - r0 * R1) * a.s1;
+  };
+  const T* at = row_of(blockIdx.x);
+  lp_fetch<T, 32>(RowView<T>(at, a.V), 0, lane, sh.next + lane);
+  for (unsigned r = blockIdx.x; r < R; r += gridDim.x) {
+    const RowView<T> row(at, a.V);
+    float thr = -INFINITY;
+    int nh = 0;                        // uniform, as the other counts below
+    bool fresh = false;
+    Sums sums;
+    for (int v0 = 0, batch = 0; v0 < row.nvec; v0 += kBatch) {
+      uint4 raw[kLpHold];
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+      for (int u = 0; u < kLpHold; ++u) raw[u] = sh.next[u * 32 + lane];
+      const bool last = v0 + kBatch >= row.nvec;
+      if (last && r + gridDim.x < R) at = row_of(r + gridDim.x);
+      if (!last || r + gridDim.x < R) lp_fetch<T, 32>(RowView<T>(at, a.V), last ? 0 : v0 + kBatch, lane, sh.next + lane);
+      uint32_t best = vec_max<T>(raw[0]);
+#pragma unroll
+      for (int u = 1; u < kLpHold; ++u) best = Vec<T>::max2(best, vec_max<T>(raw[u]));
+      const float vm = Vec<T>::top(best);
+      sums.raise(vm);
+      const int id = batch++ * 32 + lane;
+      fresh = (batch & (batch - 1)) == 0;
+      if (fresh) thr = warp_kth(sums.mx, lane, a.top);
+      const unsigned some = __ballot_sync(0xffffffffu, vm >= thr);
+      const int n = nh + __popc(some & below);
+      if (vm >= thr && n < kLpWarpHits) {
+        sh.from[n] = (unsigned short)id;
+        sh.most[n] = vm;
+      }
+      nh += __popc(some);
+      sums.add<T, 32>(row, raw, v0, lane, vm);
+    }
+    const float mine = sums.mx;
+    sums.join_warp();
+    const float M = sums.mx, L = halves(sums.l2).x, ll = log2f(L), ln = logf(L);
+    const bool ok = fabsf(M) < INFINITY;  // else no distribution: all -inf, a NaN or +inf
+    if (lane == 0) lp_write<T>(a, row, r, ok, M, ll, ln, halves(sums.w2).x, L);
+    if (!ok) {
+      for (int i = lane; i < a.top; i += 32) {
+        a.top_lp[(long long)r * a.top + i] = __int_as_float(0x7fc00000);
+        a.top_tok[(long long)r * a.top + i] = -1;
+      }
+      continue;
+    }
+    // ---- the listed batches that reach the final threshold ----
+    if (!fresh) thr = warp_kth(mine, lane, a.top);
+    const bool over = nh > kLpWarpHits;  // too many: every vector is looked at
+    __syncwarp();
+    if (!over) {
+      const int listed = nh;
+      nh = 0;
+#pragma unroll 1
+      for (int i = lane; i - lane < listed; i += 32) {
+        const bool in = i < listed && sh.most[i] >= thr;
+        const int id = i < listed ? sh.from[i] : 0;
+        const unsigned some = __ballot_sync(0xffffffffu, in);
+        __syncwarp();
+        if (in) sh.from[nh + __popc(some & below)] = (unsigned short)id;  // at or before i: read already
+        nh += __popc(some);
+      }
+      __syncwarp();
+    }
+    // ---- their vectors that do ----
+    const uint32_t t2 = Vec<T>::twice(thr);
+    const int looks = over ? row.nvec : nh * kLpHold;
+    int nv = 0;
+    auto vector = [&](int i) {
+      if (over) return i;
+      const int id = sh.from[i / kLpHold];
+      return (id >> 5) * kBatch + i % kLpHold * 32 + (id & 31);
+    };
+#pragma unroll 1
+    for (int i = lane; i - lane < looks; i += 32 * 4) {
+      uint4 x[4];
+      int v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] = i + 32 * k < looks ? vector(i + 32 * k) : row.nvec;
+        x[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (v[k] < row.nvec) x[k] = row.bits(v[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool hit = v[k] < row.nvec && Vec<T>::reaches(vec_max<T>(x[k]), t2);
+        const unsigned some = __ballot_sync(0xffffffffu, hit);
+        const int n = nv + __popc(some & below);
+        if (hit && n < kLpWarpHits) sh.hit[n] = v[k];
+        nv += __popc(some);
+      }
+    }
+    __syncwarp();
+    // ---- and their elements: (value, index) in sh.best ----
+    auto key_of = [](float x, int e) { return (unsigned long long)order_key(x) << 32 | (0xffffffffu - (uint32_t)e); };
+    int na = 0, nb = 0;
+    if (nv <= kLpWarpHits) {
+#pragma unroll 1
+      for (int i = lane; i - lane < nv * VE; i += 32) {
+        const int e = row.first(i < nv * VE ? sh.hit[i / VE] : 0) + i % VE;
+        const bool in = i < nv * VE && e >= 0 && e < a.V;
+        const float x = in ? Vec<T>::value(row.row[e]) : -INFINITY;
+        const unsigned some = __ballot_sync(0xffffffffu, in && x >= thr);
+        const int n = na + __popc(some & below);
+        if (in && x >= thr && n < kLpWarpCap) sh.best[n] = key_of(x, e);
+        na += __popc(some);
+      }
+    }
+    if (nv > kLpWarpHits || na > kLpWarpCap) {  // by scans in order, those equal to the threshold apart
+      auto scan = [&]() {
+        na = nb = 0;
+        __syncwarp();
+#pragma unroll 1
+        for (int e = lane; e - lane < a.V; e += 32) {
+          const float x = e < a.V ? Vec<T>::value(row.row[e]) : -INFINITY;
+          const bool above = e < a.V && x > thr, equal = e < a.V && x == thr;
+          const unsigned sa = __ballot_sync(0xffffffffu, above), se = __ballot_sync(0xffffffffu, equal);
+          const int pa = na + __popc(sa & below), pe = nb + __popc(se & below);
+          if (above && pa < kLpWarpCap) sh.best[pa] = key_of(x, e);
+          if (equal && pe < kLpWarpCap) sh.equal[pe] = e;  // the lowest indices
+          na += __popc(sa);
+          nb += __popc(se);
+        }
+      };
+      scan();
+      if (na > kLpWarpCap) {  // make the threshold the exact top-th largest value
+        uint32_t prefix = 0;
+        int remain = a.top;
+        for (int byte = 3; byte >= 0; --byte) {
+          __syncwarp();
+          for (int i = lane; i < 256; i += 32) sh.hist[i] = 0;
+          __syncwarp();
+#pragma unroll 1
+          for (int e = lane; e < a.V; e += 32) {
+            const uint32_t key = order_key(Vec<T>::value(row.row[e]));
+            if (byte == 3 || (key >> (8 * byte + 8)) == prefix) atomicAdd(&sh.hist[(key >> (8 * byte)) & 255], 1);
+          }
+          __syncwarp();
+          int d = 255;
+          while (d > 0 && sh.hist[d] < remain) remain -= sh.hist[d--];
+          prefix = (prefix << 8) | (uint32_t)d;
+        }
+        thr = key_value(prefix);
+        scan();
+      }
+      na = min(na, kLpWarpCap);
+      nb = min(nb, kLpWarpCap);
+    }
+    __syncwarp();
+    // ---- ranks, as above ----
+    for (int c = lane; c < na + nb; c += 32) {
+      const bool above = c < na;
+      const unsigned long long key = above ? sh.best[c] : 0;
+      const int e = above ? (int)(0xffffffffu - (uint32_t)key) : sh.equal[c - na];
+      int rank = 0;
+      if (above) {
+        for (int q = 0; q < na; ++q) rank += sh.best[q] > key;
+      } else {
+        rank = na;
+        for (int q = 0; q < nb; ++q) rank += sh.equal[q] < e;
+      }
+      if (rank < a.top) {
+        a.top_lp[(long long)r * a.top + rank] = ((above ? key_value((uint32_t)(key >> 32)) : thr) - M) - ln;
+        a.top_tok[(long long)r * a.top + rank] = e;
+      }
+    }
+    __syncwarp();                      // the lists are free for the next row
+  }
+}
+
 // d x_i = g_lp (1[i = tok] - p_i) - g_ent p_i (log p_i + H).  Rows with both factors 0
 // (a masked token, say) are written as zeros without being read.
 template <typename T>
@@ -719,6 +960,24 @@ static cudaError_t launch_fwd(const LogprobArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
+template <typename T>
+static cudaError_t launch_warp(const LogprobArgs& a, cudaStream_t st) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices];
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < kDevices) sms = known[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    if (dev < kDevices) known[dev].store(sms, std::memory_order_relaxed);
+  }
+  const unsigned grid = (unsigned)std::min<long long>(a.R0 * a.R1, (long long)sms * kLpWarpBlocks);
+  logprobs_warp_kernel<T><<<grid, 32, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
 // Many rows, or short ones: 128 threads a row, 7 or 8 rows to an SM, whose joins hide
 // behind one another (8190 rows of 32000 bf16: 98 us, with 512 threads 125; with 20
 // alternatives 174 and 230).  Few rows: 512 threads a row, for the latency (300 rows, 20
@@ -731,6 +990,8 @@ static cudaError_t launch_fwd_t(const LogprobArgs& a, cudaStream_t st) {
   constexpr int kShort = kLpHold * 128 * RowView<T>::VE;  // a batch of 128 threads
   const bool narrow = a.V <= kShort || (a.R0 * a.R1 >= kLpManyRows &&
                                         (a.top == 0 || (a.top <= kLpSmallTop && a.V <= 4 * kShort)));
+  if (a.top > 0 && a.top <= kLpSmallTop && a.R0 * a.R1 >= kLpWarpRows && a.V <= kLpWarpBatches * kLpHold * 32 * RowView<T>::VE)
+    return launch_warp<T>(a, st);
   if (a.top > 0) return narrow ? launch_fwd<T, 128, true>(a, st) : launch_fwd<T, 512, true>(a, st);
   return narrow ? launch_fwd<T, 128, false>(a, st) : launch_fwd<T, 512, false>(a, st);
 }

@@ -4,6 +4,7 @@ Tolerances.  A row's sum is V / 512 terms in turn in a thread, then a tree: with
 V / 512 + 24 roundings and exp2's 2 ulp, l and w are within n 2^-23 of themselves, so
     |logprob - ref| <= n 2^-23 + |ref| 2^-22            (the log, the difference)
     |entropy - ref| <= 2 n 2^-23 (1 + ln V)             (log2 l and w / l are at most ln V)
+Where many rows get a warp each, a thread adds V / 64 terms of half a step, n = V / 128 + 24.
 p is within (n + 2 |log p| + 4) 2^-23 of itself; the gradient adds half a step of its type
 (finfo.eps / 2, or half the smallest subnormal)."""
 import math
@@ -19,8 +20,8 @@ pytestmark = pytest.mark.gpu
 BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
-def slack(V):
-    return (V / 512 + 24) * 2.0 ** -23
+def slack(V, wide=512):
+    return (V / wide + 24) * 2.0 ** -23
 
 
 def reference(x, tokens):
@@ -36,25 +37,31 @@ def ranked(x, k):
     return torch.sort(x.double(), dim=-1, descending=True, stable=True).indices[..., :k]
 
 
-def check(x, tokens, top):
+def check(x, tokens, top, wide=512):
     V = x.shape[-1]
+    err = slack(V, wide)
     got = lb.token_logprobs(x, tokens, top=top)
     lp, chosen, h = reference(x, tokens)
     assert got.logprobs.shape == got.entropy.shape == x.shape[:-1] and got.top_tokens.shape == (*x.shape[:-1], top)
+    live = (x == x).all(-1) & ~(x == math.inf).any(-1) & (x > -math.inf).any(-1)     # else without a distribution
+    assert got.entropy[~live].isnan().all() and got.top_logprobs[~live].isnan().all() and (got.top_tokens[~live] == -1).all()
+    assert (got.logprobs[~live].isnan() == (tokens[~live] >= 0)).all()
     assert got.logprobs.dtype == got.entropy.dtype == got.top_logprobs.dtype == F32 and got.top_tokens.dtype == torch.int64
+    whole, got = got, lb.TokenLogprobs(*(part[live] for part in got))
+    x, lp, chosen, h = x[live], lp[live], chosen[live], h[live]
     inf = chosen < -torch.finfo(F32).max                         # -6e38 has no fp32 value but -inf
     assert (got.logprobs[inf] == -math.inf).all()
-    assert ((got.logprobs - chosen).abs()[~inf] <= slack(V) + chosen.abs()[~inf] * 2.0 ** -22).all(), (got.logprobs - chosen).abs().max()
-    assert ((got.entropy - h).abs() <= 2 * slack(V) * (1 + math.log(V))).all(), (got.entropy - h).abs().max()
+    assert ((got.logprobs - chosen).abs()[~inf] <= err + chosen.abs()[~inf] * 2.0 ** -22).all(), (got.logprobs - chosen).abs().max()
+    assert ((got.entropy - h).abs() <= 2 * err * (1 + math.log(V))).all(), (got.entropy - h).abs().max()
     if top:
         want = ranked(x, top)
         assert torch.equal(got.top_tokens, want)
         ref = lp.gather(-1, want)
         fin = ref >= -torch.finfo(F32).max
-        assert ((got.top_logprobs - ref).abs()[fin] <= slack(V) + ref.abs()[fin] * 2.0 ** -22).all()
+        assert ((got.top_logprobs - ref).abs()[fin] <= err + ref.abs()[fin] * 2.0 ** -22).all()
         assert (got.top_logprobs[~fin] == -math.inf).all()
     _lib.check_status()
-    return got
+    return whole
 
 
 def rows(dev, shape, dtype, seed=0, spread=3.0):
@@ -84,6 +91,73 @@ def test_many_rows_and_long_rows(cuda_device, dtype, R, V, top):
     by the first one's threshold."""
     x = rows(cuda_device, (R, V), dtype, seed=R)
     check(x, some_tokens(x), top)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("R,V,top", [(3000, 9001, 20), (3557, 31000, 24), (7111, 2049, 1), (3000, 40, 24), (3000, 185, 24),
+                                     (3001, 32768, 5), (3001, 5, 5)])
+def test_a_warp_a_row(cuda_device, dtype, R, V, top):
+    """Many rows with few alternatives; as many rows as warps, and some more."""
+    x = rows(cuda_device, (R, V), dtype, seed=R)
+    check(x, some_tokens(x), top, wide=128)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+def test_a_warp_a_row_of_any_kind(cuda_device, dtype):
+    R, V = 3001, 12003
+    low = torch.finfo(dtype).min
+    x = rows(cuda_device, (R, V), dtype, seed=8)
+    x[0] = 0                                                     # all equal
+    x[1, 8000:] = 30                                             # thousands best
+    x[2, 7::50] = 30
+    x[3, :], x[3, 100:103] = 1, 3                                # three above many ties
+    x[4] = x[4].float().round().to(dtype)
+    x[5, ::2], x[5, 1::2] = -0.0, 0.0
+    x[6] = torch.sort(x[6]).values
+    x[7] = torch.sort(-x[7].abs(), descending=True).values       # keys of negative numbers
+    x[8] = torch.sort(x[8]).values.view(3, V // 3).t().reshape(-1)
+    x[9, : V // 2] = -math.inf                                   # a start that says nothing
+    x[10, : V - 40] = low
+    x[11, 1:] = -math.inf                                        # one left, three left, fewer than asked for
+    x[12, :], x[12, [5, 2000, 12002]] = low, torch.tensor([1.0, 2.0, 1.0], dtype=dtype, device=cuda_device)
+    x[13, 3:] = low
+    x[14, ::1700] = 50                                           # next to each other in no lane
+    x[15] = low
+    x[16], x[16, 256 * 8:256 * 9] = -40, x[17, 256 * 8:256 * 9]  # all of the large ones in a few vectors
+    t = some_tokens(x)
+    t[11] = 0
+    check(x, t, 20, wide=128)
+    check(x[:, 1:-1], t.clamp(max=V - 3), 24, wide=128)          # odd row starts
+    broken = x.clone()
+    broken[20], broken[21, 17], broken[22, V - 1], broken[3000, 600] = -math.inf, math.nan, math.inf, math.nan
+    got = lb.token_logprobs(broken, t, top=20)
+    bad = [20, 21, 22, 3000]
+    assert got.entropy[bad].isnan().all() and got.logprobs[bad].isnan().all()
+    assert got.top_logprobs[bad].isnan().all() and (got.top_tokens[bad] == -1).all()
+    keep = torch.ones(R, dtype=torch.bool, device=cuda_device)
+    keep[bad] = False
+    same = lb.token_logprobs(x, t, top=20)
+    for a, b in zip(got, same):
+        assert torch.equal(a[keep], b[keep])                     # the others do not notice, bit for bit
+
+
+def test_a_warp_a_row_with_its_gradient(cuda_device):
+    """The row statistics that the gradient needs, next to alternatives, in strided rows."""
+    x = rows(cuda_device, (2, 1502, 3001), F32, seed=5).requires_grad_(True)
+    t = some_tokens(x[:, :-1])
+    got = lb.token_logprobs(x[:, :-1], t, top=4)
+    gl, ge = rows(cuda_device, got.entropy.shape, F32, seed=6), rows(cuda_device, got.entropy.shape, F32, seed=7)
+    d, = torch.autograd.grad((got.logprobs, got.entropy), x, (gl, ge))
+    lp, _, h = reference(x.detach()[:, :-1], t)
+    p, real = lp.exp(), (t >= 0)[..., None]
+    one = torch.zeros_like(p).scatter_(-1, t.clamp(min=0)[..., None], 1.0) * real
+    gl, ge = gl.double()[..., None] * real, ge.double()[..., None]
+    want = gl * (one - p) - ge * p * (lp + h[..., None])
+    mag = (gl.abs() + ge.abs() * (lp.abs() + h[..., None] + 1)) * p     # as in test_gradient_matches_formula, V / 128 terms
+    tol = 2.0 ** -24 * want.abs() + mag * (3001 / 128 + 28 + 2 * lp.abs()) * 2.0 ** -23 * (1 + math.log(3001)) \
+        + gl.abs() * one * 2.0 ** -23 + torch.finfo(F32).smallest_normal
+    assert not d[:, -1].any()
+    assert ((d[:, :-1] - want).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
