@@ -29,7 +29,8 @@ constexpr int kLpGroups = 128;   // groups of threads
 constexpr int kLpHold = 8;       // vectors a thread holds: 32768 bf16 logits in 512 threads
 constexpr int kLpBwdHold = 4;
 constexpr int kLpManyRows = 900;
-constexpr int kLpWarpRows = 3000, kLpWarpBatches = 32;
+constexpr int kLpWarpHold = 5;   // of a warp that has a row to itself
+constexpr int kLpWarpBatches = 128;
 constexpr int kLpSmallTop = 24;  // up to here 32 group maxima do
 constexpr float kLpFloor = -200.f;  // 2^-200 is 0 in fp32; keeps 0 * -inf out of w
 
@@ -229,7 +230,7 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // what lies over the row's ends with -inf outside.
 // Code size matters here: blocks are at different places of it, and what the
 // instruction cache cannot hold they wait for.  Rare cases are loops, not unrolled.
-template <typename T, int NT>
+template <typename T, int NT, int HOLD>
 __device__ __forceinline__ void lp_fetch(const RowView<T> row, int v0, int tid, uint4* next) {
   constexpr int VE = RowView<T>::VE;
   const uint32_t own = (uint32_t)__cvta_generic_to_shared(next);
@@ -237,7 +238,7 @@ __device__ __forceinline__ void lp_fetch(const RowView<T> row, int v0, int tid, 
   const T* from = row.row + e0;
   bool all = true;
 #pragma unroll
-  for (int u = 0; u < kLpHold; ++u) {
+  for (int u = 0; u < HOLD; ++u) {
     const bool in = row.whole(e0 + u * NT * VE);
     all = all && in;
     if (in)
@@ -246,7 +247,7 @@ __device__ __forceinline__ void lp_fetch(const RowView<T> row, int v0, int tid, 
   asm volatile("cp.async.commit_group;" ::: "memory");
   if (!all) {
 #pragma unroll 1
-    for (int u = 0; u < kLpHold; ++u)
+    for (int u = 0; u < HOLD; ++u)
       if (!row.whole(e0 + u * NT * VE)) next[u * NT] = row.edge(e0 + u * NT * VE);  // -inf outside
   }
 }
@@ -266,14 +267,14 @@ struct Sums {
     }
   }
 
-  template <typename T, int NT>
-  __device__ __forceinline__ void add(const RowView<T>& row, const uint4 (&raw)[kLpHold], int v0, int tid, float vm) {
+  template <typename T, int NT, int HOLD>
+  __device__ __forceinline__ void add(const RowView<T>& row, const uint4 (&raw)[HOLD], int v0, int tid, float vm) {
     constexpr int VE = RowView<T>::VE;
     const Pair nm = pair(-mx, -mx), le = pair(kLog2e, kLog2e);
     if (VE == 8 && fabsf(mx) < Vec<T>::kNear) {
       if constexpr (VE == 8) {
 #pragma unroll
-        for (int u = 0; u < kLpHold; ++u)
+        for (int u = 0; u < HOLD; ++u)
           if (v0 + u * NT < row.nvec) {
             const uint4 x = Vec<T>::bounded(raw[u]);
 #pragma unroll
@@ -299,11 +300,11 @@ struct Sums {
       };
       if constexpr (VE == 4) {
 #pragma unroll
-        for (int u = 0; u < kLpHold; ++u)
+        for (int u = 0; u < HOLD; ++u)
           if (v0 + u * NT < row.nvec) one(raw[u]);
       } else {                     // a maximum near the type's ends: rare
 #pragma unroll 1
-        for (int v = v0 + tid; v < min(row.nvec, v0 + kLpHold * NT); v += NT) one(row.bits(v));
+        for (int v = v0 + tid; v < min(row.nvec, v0 + HOLD * NT); v += NT) one(row.bits(v));
       }
     }
   }
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
     return static_cast<const T*>(a.logits) + (long long)r0 * a.s0 + (long long)(r - r0 * R1) * a.s1;
   };
   const T* at = row_of(blockIdx.x);
-  lp_fetch<T, NT>(RowView<T>(at, a.V), 0, tid, next + tid);
+  lp_fetch<T, NT, kLpHold>(RowView<T>(at, a.V), 0, tid, next + tid);
   // Without alternatives a row has one barrier: a warp may be at its next row while others
   // read this row's sums, which the rows therefore keep in turn.
   int turn = 0;
@@ -471,13 +472,13 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
       for (int u = 0; u < kLpHold; ++u) raw[u] = next[u * NT + tid];
       const bool last = v0 + kBatch >= row.nvec;
       if (last && r + gridDim.x < R) at = row_of(r + gridDim.x);
-      if (!last || r + gridDim.x < R) lp_fetch<T, NT>(RowView<T>(at, a.V), last ? 0 : v0 + kBatch, tid, next + tid);
+      if (!last || r + gridDim.x < R) lp_fetch<T, NT, kLpHold>(RowView<T>(at, a.V), last ? 0 : v0 + kBatch, tid, next + tid);
       uint32_t best = vec_max<T>(raw[0]);
 #pragma unroll
       for (int u = 1; u < kLpHold; ++u) best = Vec<T>::max2(best, vec_max<T>(raw[u]));
       const float vm = Vec<T>::top(best);
       sums.raise(vm);
-      sums.add<T, NT>(row, raw, v0, tid, vm);
+      sums.add<T, NT, kLpHold>(row, raw, v0, tid, vm);
       // A row of several batches lists its candidates as it goes, by the first batch's
       // threshold, which the final one is not below.
       if (TOP && multi) {      // uniform
@@ -666,14 +667,18 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
 // Many rows with up to kLpSmallTop alternatives: a warp (a block of 32 threads) to a row,
 // without any barrier.  The lanes' maxima are the groups; their top-th largest is taken
 // anew whenever the batches seen have doubled.  What is listed meanwhile is a lane's whole
-// batch with its maximum, where that reaches the threshold: one test for 64 elements, and
-// the final threshold drops most of the list (122 of a row of 16 batches with 20
+// batch with its maximum, where that reaches the threshold: one test for 40 elements, and
+// the final threshold drops most of the list (about 140 of a row of 25 batches, with 20
 // alternatives) without a look at its elements.
-constexpr int kLpWarpBlocks = 24;
+// 8190 rows of 32000 bf16, 20 best: 119 us with 28 warps of 5 vectors a thread to an SM, 125
+// with 24 of 8 or 28 of 4.  What bounds it: issue slots are busy 63 % of the time, DRAM moves
+// 4.4 TB/s; 2.1 rows a warp leave the last round a fifth full, and the warps' latencies in
+// the lists (shuffles, 1.1; fixed, 2.1 of 8.9 cycles an instruction) are not all hidden.
+constexpr int kLpWarpBlocks = 28;
 constexpr int kLpWarpHits = 320;
 constexpr int kLpWarpCap = 192;  // (kLpSmallTop - 1) vectors, with lanes without one
 struct LpWarpShared {
-  uint4 next[kLpHold * 32];
+  uint4 next[kLpWarpHold * 32];
   union {
     float most[kLpWarpHits];     // a listed batch's maximum, then
     int hit[kLpWarpHits];        // the vectors that reach the final threshold
@@ -689,7 +694,7 @@ struct LpWarpShared {
 template <typename T>
 __global__ void __launch_bounds__(32, kLpWarpBlocks) logprobs_warp_kernel(const __grid_constant__ LogprobArgs a) {
   __shared__ __align__(16) LpWarpShared sh;
-  constexpr int VE = RowView<T>::VE, kBatch = kLpHold * 32;
+  constexpr int VE = RowView<T>::VE, kBatch = kLpWarpHold * 32;
   const int lane = threadIdx.x;
   const unsigned below = (1u << lane) - 1u;
   const unsigned R = (unsigned)(a.R0 * a.R1), R1 = (unsigned)a.R1;
@@ -698,7 +703,7 @@ __global__ void __launch_bounds__(32, kLpWarpBlocks) logprobs_warp_kernel(const 
     return static_cast<const T*>(a.logits) + (long long)r0 * a.s0 + (long long)(r - r0 * R1) * a.s1;
   };
   const T* at = row_of(blockIdx.x);
-  lp_fetch<T, 32>(RowView<T>(at, a.V), 0, lane, sh.next + lane);
+  lp_fetch<T, 32, kLpWarpHold>(RowView<T>(at, a.V), 0, lane, sh.next + lane);
   for (unsigned r = blockIdx.x; r < R; r += gridDim.x) {
     const RowView<T> row(at, a.V);
     float thr = -INFINITY;
@@ -706,16 +711,16 @@ __global__ void __launch_bounds__(32, kLpWarpBlocks) logprobs_warp_kernel(const 
     bool fresh = false;
     Sums sums;
     for (int v0 = 0, batch = 0; v0 < row.nvec; v0 += kBatch) {
-      uint4 raw[kLpHold];
+      uint4 raw[kLpWarpHold];
       asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-      for (int u = 0; u < kLpHold; ++u) raw[u] = sh.next[u * 32 + lane];
+      for (int u = 0; u < kLpWarpHold; ++u) raw[u] = sh.next[u * 32 + lane];
       const bool last = v0 + kBatch >= row.nvec;
       if (last && r + gridDim.x < R) at = row_of(r + gridDim.x);
-      if (!last || r + gridDim.x < R) lp_fetch<T, 32>(RowView<T>(at, a.V), last ? 0 : v0 + kBatch, lane, sh.next + lane);
+      if (!last || r + gridDim.x < R) lp_fetch<T, 32, kLpWarpHold>(RowView<T>(at, a.V), last ? 0 : v0 + kBatch, lane, sh.next + lane);
       uint32_t best = vec_max<T>(raw[0]);
 #pragma unroll
-      for (int u = 1; u < kLpHold; ++u) best = Vec<T>::max2(best, vec_max<T>(raw[u]));
+      for (int u = 1; u < kLpWarpHold; ++u) best = Vec<T>::max2(best, vec_max<T>(raw[u]));
       const float vm = Vec<T>::top(best);
       sums.raise(vm);
       const int id = batch++ * 32 + lane;
@@ -728,7 +733,7 @@ __global__ void __launch_bounds__(32, kLpWarpBlocks) logprobs_warp_kernel(const 
         sh.most[n] = vm;
       }
       nh += __popc(some);
-      sums.add<T, 32>(row, raw, v0, lane, vm);
+      sums.add<T, 32, kLpWarpHold>(row, raw, v0, lane, vm);
     }
     const float mine = sums.mx;
     sums.join_warp();
@@ -762,12 +767,12 @@ __global__ void __launch_bounds__(32, kLpWarpBlocks) logprobs_warp_kernel(const 
     }
     // ---- their vectors that do ----
     const uint32_t t2 = Vec<T>::twice(thr);
-    const int looks = over ? row.nvec : nh * kLpHold;
+    const int looks = over ? row.nvec : nh * kLpWarpHold;
     int nv = 0;
     auto vector = [&](int i) {
       if (over) return i;
-      const int id = sh.from[i / kLpHold];
-      return (id >> 5) * kBatch + i % kLpHold * 32 + (id & 31);
+      const int id = sh.from[i / kLpWarpHold];
+      return (id >> 5) * kBatch + i % kLpWarpHold * 32 + (id & 31);
     };
 #pragma unroll 1
     for (int i = lane; i - lane < looks; i += 32 * 4) {
@@ -978,22 +983,34 @@ static cudaError_t launch_warp(const LogprobArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// Many rows, or short ones: 128 threads a row, 7 or 8 rows to an SM, whose joins hide
-// behind one another (8190 rows of 32000 bf16: 98 us, with 512 threads 125; with 20
-// alternatives 174 and 230).  Few rows: 512 threads a row, for the latency (300 rows, 20
-// alternatives: 23 and 17 us; 900 rows: equal); and for more alternatives than the 32 groups
-// serve (50 of 8190 rows: 283 and 260 us), or in rows of more than four short batches, whose
-// first one sets too low a threshold for them (1665 x 65060 fp32, 20
-// best: 286 and 100 us).
+// Without alternatives.  Many rows, or short ones: 128 threads a row, 8 rows to an SM, whose
+// joins hide behind one another (8190 rows of 32000 bf16: 98 us, with 512 threads 125).  Few
+// rows: 512 threads a row, for the latency (900 rows: equal).
+//
+// With up to 24 alternatives a warp a row, once there are rows enough to hide that a warp
+// needs 10 us and 4 more per 1000 vectors for its row.  20 best, bf16, us with a warp / 128 /
+// 512 threads:
+//   8190 x 32000   119 / 172 / 232      1200 x 32000    33 /  38 / 39      600 x 32000   29 / 25 / 25
+//   4100 x 128000  200 / 633 / 271      1200 x 128000  101 / 263 / 87      600 x 16000   21 / 15 / 25
+//   9000 x 2000     31 /  82 / 290       600 x 2000     10 /  10 / 27      150 x 2000     9 /  8 / 12
+// so from 900 rows and one more for every 16 vectors of a row, or 300 where a row is two
+// batches; but to 128 batches a row, whose list the doublings still fit (2500 x 160000: 183 /
+// 605 / 211; 4200 x 200000, which it does not always: 478 / 1232 / 438).  Below that 128 threads
+// where the rows are at least 150 for each of their batches, of which four at most (the
+// first one sets the threshold for the lists: 900 x 65000: 68 and with 512 threads 49), else 512.
+// More alternatives than the 32 groups serve: 512 threads (50 best of 8190 x 32000: 283 with 128
+// threads and 260), but for a row of one batch (900 x 500: 86 with 512, 17 with 128).
 template <typename T>
 static cudaError_t launch_fwd_t(const LogprobArgs& a, cudaStream_t st) {
-  constexpr int kShort = kLpHold * 128 * RowView<T>::VE;  // a batch of 128 threads
-  const bool narrow = a.V <= kShort || (a.R0 * a.R1 >= kLpManyRows &&
-                                        (a.top == 0 || (a.top <= kLpSmallTop && a.V <= 4 * kShort)));
-  if (a.top > 0 && a.top <= kLpSmallTop && a.R0 * a.R1 >= kLpWarpRows && a.V <= kLpWarpBatches * kLpHold * 32 * RowView<T>::VE)
+  constexpr int VE = RowView<T>::VE, kShort = kLpHold * 128 * VE;  // a batch of 128 threads
+  const long long rows = a.R0 * a.R1;
+  if (a.top == 0)
+    return a.V <= kShort || rows >= kLpManyRows ? launch_fwd<T, 128, false>(a, st) : launch_fwd<T, 512, false>(a, st);
+  if (a.top <= kLpSmallTop && a.V <= kLpWarpBatches * kLpWarpHold * 32 * VE &&
+      rows >= (a.V <= 2 * kLpWarpHold * 32 * VE ? 300 : kLpManyRows + a.V / VE / 16))
     return launch_warp<T>(a, st);
-  if (a.top > 0) return narrow ? launch_fwd<T, 128, true>(a, st) : launch_fwd<T, 512, true>(a, st);
-  return narrow ? launch_fwd<T, 128, false>(a, st) : launch_fwd<T, 512, false>(a, st);
+  const bool narrow = a.V <= kShort || (a.top <= kLpSmallTop && a.V <= 4 * kShort && rows * kShort >= 150LL * a.V);
+  return narrow ? launch_fwd<T, 128, true>(a, st) : launch_fwd<T, 512, true>(a, st);
 }
 
 cudaError_t launch_logprobs_fwd(const LogprobArgs& a, int dtype, cudaStream_t st) {

@@ -95,7 +95,8 @@ def test_many_rows_and_long_rows(cuda_device, dtype, R, V, top):
 
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 @pytest.mark.parametrize("R,V,top", [(3000, 9001, 20), (3557, 31000, 24), (7111, 2049, 1), (3000, 40, 24), (3000, 185, 24),
-                                     (3001, 32768, 5), (3001, 5, 5)])
+                                     (3001, 32768, 5), (3001, 5, 5), (300, 2560, 24), (1300, 50000, 24),
+                                     (2000, 130000, 20)])
 def test_a_warp_a_row(cuda_device, dtype, R, V, top):
     """Many rows with few alternatives; as many rows as warps, and some more."""
     x = rows(cuda_device, (R, V), dtype, seed=R)
