@@ -672,8 +672,8 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
 // alternatives) without a look at its elements.
 // 8190 rows of 32000 bf16, 20 best: 119 us with 28 warps of 5 vectors a thread to an SM, 125
 // with 24 of 8 or 28 of 4.  What bounds it: issue slots are busy 63 % of the time, DRAM moves
-// 4.4 TB/s; 2.1 rows a warp leave the last round a fifth full, and the warps' latencies in
-// the lists (shuffles, 1.1; fixed, 2.1 of 8.9 cycles an instruction) are not all hidden.
+// 4.4 TB/s; of the 8.9 cycles that a warp takes for an instruction 2.1 are fixed latency, 1.1
+// loads, 2.0 shuffles and shared memory, 1.7 other warps' turns.
 constexpr int kLpWarpBlocks = 28;
 constexpr int kLpWarpHits = 320;
 constexpr int kLpWarpCap = 192;  // (kLpSmallTop - 1) vectors, with lanes without one
