@@ -21,7 +21,7 @@ LIB = os.path.join(HERE, "liblucid_b200.so")
 
 SOURCES = ["lucid_prep.cu", "lucid_fwd.cu", "lucid_bwd.cu", "capi.cu", "path_block.cu", "path_kernels.cu",
            "path_capi.cu", "lucid_decode.cu", "decode_capi.cu", "paged_decode.cu", "paged_pages.cu", "logprobs.cu", "serve_capi.cu"]
-HEADERS = ["sm100.cuh", "lucid_common.cuh", "tmap.h", "path_common.cuh", "profile.h", "serve_common.cuh"]
+HEADERS = ["sm100.cuh", "lucid_common.cuh", "tmap.h", "path_common.cuh", "profile.h", "serve_common.cuh", "paged_flat.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -26,6 +26,7 @@
 // has 64 or more and would hand its scores back through tensor memory for the softmax.
 // HBM bounds the pass (4 x 32765 tokens, 32 heads of 128: 2.15 GB in 327 us, 6.5 TB/s), the
 // tensor pipe is active 16 % of it.
+#include "paged_flat.h"
 #include "serve_common.cuh"
 
 #include <algorithm>
@@ -210,7 +211,7 @@ template <bool R8, int CE, int NK, int NX, int MODE>
 struct PdShape {
   static constexpr int kCols = NX * 8 * CE;                 // columns covered
   static constexpr int kRowBytes = MODE == kFlat ? 0 : kCols <= 64 ? 128 : 256;
-  static constexpr int kPool = MODE == kFlat ? 16 * 2 * ((NK * 16 < kCols ? NK * 16 : kCols) - 4) : 16 * kRowBytes;  // bytes of a pool in a stage, at most
+  static constexpr int kPool = MODE == kFlat ? 32 * flat_most_d(NK) : 16 * kRowBytes;  // bytes of a pool in a stage, at most
   static constexpr int kCtas = kCols <= 64 || MODE != kRows && (R8 || kCols <= 96) ? 3 : 2;
   static constexpr int kStages = kCtas == 2 || kPool <= 2560 ? 3 : 2;
   // reads of the columns past D may run up to 192 bytes past a flat run
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
   constexpr int KS = NK * CE / 4;  // 16-element k steps
   using Shape = PdShape<R8, CE, NK, NX, MODE>;
   constexpr int CB = CE * 2, RB = Shape::kRowBytes, POOL = Shape::kPool, STAGE = 2 * POOL, STAGES = Shape::kStages;
-  constexpr int NU = MODE == kFull ? RB / CB / 2 : MODE == kRows ? (NK * 4 + 1) / 2 : (POOL / 16 + 31) / 32;  // copies per lane and pool
+  constexpr int NU = MODE == kFull ? RB / CB / 2 : MODE == kRows ? (NK * 4 + 1) / 2 : flat_copies(NK);  // copies per lane and pool
   extern __shared__ __align__(16) unsigned char ring[];  // [warp][stage][pool]: 16 tokens
   __shared__ float red[2][R8 ? 8 : 16][132];  // a warp pair's accumulator rows
   __shared__ float red_ml[kPdWarps][16][2];
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
         if (lim >= 16) {
 #pragma unroll
           for (int u = 0; u < NU; ++u)
-            if (u < NU - 1 || 16 * (32 * u + lane) < 32 * a.D) {
+            if (flat_copied(NK, a.D, u, lane)) {
               copy_async<16>(to + 512 * u, kp + 256 * u, 16);
               copy_async<16>(to + POOL + 512 * u, xp + 256 * u, 16);
             }
@@ -959,9 +960,11 @@ static cudaError_t launch_pd_d(PagedDecodeArgs& a, cudaStream_t st) {
     return launch_pd<STEP, R8, 8, 4, 2, kRows>(a, st);
   }
   if (base16 && a.k.sn == a.D && a.x.sn == a.D && a.ps % 16 == 0) {  // D is an odd multiple of 4 here
-    if (a.D < 64) return launch_pd<STEP, R8, 4, 4, 2, kFlat>(a, st);
-    if (a.D < 80) return launch_pd<STEP, R8, 4, 5, 3, kFlat>(a, st);
-    return launch_pd<STEP, R8, 4, 8, 4, kFlat>(a, st);
+    switch (flat_chunks(a.D)) {
+      case 4: return launch_pd<STEP, R8, 4, 4, 2, kFlat>(a, st);
+      case 5: return launch_pd<STEP, R8, 4, 5, 3, kFlat>(a, st);
+      default: return launch_pd<STEP, R8, 4, 8, 4, kFlat>(a, st);
+    }
   }
   if (a.D <= 64) return launch_pd<STEP, R8, 4, 4, 2, kRows>(a, st);
   if (a.D <= 80) return launch_pd<STEP, R8, 4, 5, 3, kRows>(a, st);
