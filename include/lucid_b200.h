@@ -448,7 +448,7 @@ int lucid_cp_solve_bwd(int B, int H, int N, int D, float scale, int blk_lo, int 
  *   also writes k_new and x_new into row n of the sequence's pages.
  * lucid_paged_decode_attn: the attention alone, over the n cached tokens (none: zeros).
  * Both split the cached tokens of the whole batch evenly over the GPU whatever the
- * lengths; sums are fp32, results are the same from run to run.
+ * lengths; weights and sums are fp32, results are the same from run to run.
  */
 size_t lucid_paged_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int step);
 int lucid_paged_decode_step(int B, int Hq, int Hkv, int D, int P, int ps, int M, float scale, float eps,

@@ -9,7 +9,10 @@
 // 16-row operand, so both sums come out of one pass over the cached rows:
 //   S = A K^T (mma m16n8k16: exact bf16 products, fp32 sums), the scores scaled
 //   afterwards in fp32 (softmax rows by s, the update row by s rstd_new rstd_t), and
-//   acc += P X with P split into bf16 hi + lo, so that P keeps 16 bits.
+//   acc += P X with P split into three bf16 parts, which hold all 24 bits of an fp32
+//   weight: the products are exact, the sums fp32.  (Two parts, 16 bits, are 0 to 3 % faster
+//   at 8 query heads per kv head, 30.8 and 29.9 us a call for 24 ragged sequences, and
+//   slower at one.)
 // sum(k_t^2) is the diagonal of K K^T, computed by the same instructions: the B fragment
 // of a key tile is also its A fragment, and with at most 8 query rows it rides in the
 // rows of A that S leaves empty.
@@ -223,7 +226,7 @@ struct PdShape {
 // once.  Page numbers are looked up one tile before their copies are issued.
 //
 // STEP: an update row behind the query rows.  R8: at most 8 rows, so rows 8-15 of the
-// P operand carry the low halves of P and one mma does both.  A row's elements are cut
+// P operand carry the second parts of P and one mma does both.  A row's elements are cut
 // into chunks of CE (16 bytes where every row is 16-byte aligned, else 8): lane j of a
 // quad holds the key chunks 4 i + j (i < NK), lane group g the value chunks
 // 8 c + g (c < NX); the same permutation of the inner index on both operands, and of
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
         rk[2] = __shfl_sync(0xffffffffu, v1, 9 * j);
         rk[3] = __shfl_sync(0xffffffffu, v1, 9 * j + 4);
       }
-      uint32_t phi[4], plo[4];
+      uint32_t phi[4], pmi[4], plo[4];
       float al[2] = {1.f, 1.f};
 #pragma unroll
       for (int hf = 0; hf < (R8 ? 1 : 2); ++hf) {
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           // the reference point moves only when a score passes it by kPdSlack: until then
-          // the weights stay below 2^kPdSlack, whose digits fp32 and bf16 pairs hold alike
+          // the weights stay below 2^kPdSlack, which costs an fp32 sum no digits
           if (!is_upd && mx > m[hf] + kPdSlack) {
             al[hf] = ex2(m[hf] - mx);        // 0 while nothing has been seen
             m[hf] = mx;
@@ -518,8 +521,12 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
         phi[2 * hf] = pack_bf16(p[0], p[1]);
         phi[2 * hf + 1] = pack_bf16(p[2], p[3]);
         const float2 h0 = unpack_bf16(phi[2 * hf]), h1 = unpack_bf16(phi[2 * hf + 1]);
-        plo[2 * hf] = pack_bf16(p[0] - h0.x, p[1] - h0.y);
-        plo[2 * hf + 1] = pack_bf16(p[2] - h1.x, p[3] - h1.y);
+        p[0] -= h0.x; p[1] -= h0.y; p[2] -= h1.x; p[3] -= h1.y;  // exact
+        pmi[2 * hf] = pack_bf16(p[0], p[1]);
+        pmi[2 * hf + 1] = pack_bf16(p[2], p[3]);
+        const float2 m0 = unpack_bf16(pmi[2 * hf]), m1 = unpack_bf16(pmi[2 * hf + 1]);
+        plo[2 * hf] = pack_bf16(p[0] - m0.x, p[1] - m0.y);
+        plo[2 * hf + 1] = pack_bf16(p[2] - m1.x, p[3] - m1.y);
       }
       if constexpr (R8) al[1] = al[0];
       if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
@@ -533,9 +540,11 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
       }
       auto weigh = [&](float (&d)[4], uint32_t b0, uint32_t b1) {
         if constexpr (R8) {
-          mma16816(d, phi[0], plo[0], phi[1], plo[1], b0, b1);
+          mma16816(d, phi[0], pmi[0], phi[1], pmi[1], b0, b1);
+          mma16816(d, plo[0], 0u, plo[1], 0u, b0, b1);
         } else {
           mma16816(d, phi[0], phi[2], phi[1], phi[3], b0, b1);
+          mma16816(d, pmi[0], pmi[2], pmi[1], pmi[3], b0, b1);
           mma16816(d, plo[0], plo[2], plo[1], plo[3], b0, b1);
         }
       };

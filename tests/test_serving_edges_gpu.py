@@ -5,7 +5,7 @@ import torch
 
 import lucid_b200 as lb
 from lucid_b200 import _lib
-from test_paged_gpu import check_attention, check_step, make, run_attention, run_step
+from test_paged_gpu import check, check_attention, check_step, make, ref_attention, run_attention, run_step
 
 pytestmark = pytest.mark.gpu
 
@@ -19,4 +19,35 @@ def test_dense_rows_on_8_byte_boundaries(cuda_device, D, Hq):
     assert s["kp"].is_contiguous() and s["table"].max() == s["kp"].shape[0] - 1
     check_step(s, *run_step(s, append=False))
     check_attention(s, run_attention(s))
+    _lib.check_status()
+
+
+@pytest.mark.parametrize("gq", [1, 16])
+def test_weights_keep_the_bits_of_fp32(cuda_device, gq):
+    """Sums that cancel: two tokens of score 0 hold p b as two bf16 parts, against one of
+    weight p = exp(-t / 32) and value b, so what is left shows p's last bits.  The score is exact
+    but for log2 e's rounding and its own, 2^-23 for |z| < 1; exp2 adds 2^-22, and at most six fp32
+    sums on the way half a step of the sum of |p x| or, truncated, a whole one: 9 2^-23 in all,
+    12 allowed.  A weight of 16 bits is off by up to 2^-18, 32 2^-23."""
+    H, D = 32, 64
+    s = make(cuda_device, [3], H * gq, H, D, 16, seed=5)
+    s["scale"] = 1 / 32
+    t = torch.linspace(1, 22, H, device=cuda_device).bfloat16().double()
+    p = torch.exp(-t / 32)[:, None]
+    page = int(s["table"][0, 0])
+    b = s["xp"][page, :, 1].double()
+    s["kp"][page, :, :3] = 0
+    s["kp"][page, :, 1, 0] = -t.bfloat16()
+    high = (p * b).bfloat16()
+    s["xp"][page, :, 0], s["xp"][page, :, 2] = -high, -(p * b - high.double()).bfloat16()
+    s["q"].zero_()
+    s["q"][..., 0] = 1
+    s["k"].zero_()                                   # the step's own token: weight 1, value v
+    s["v"].zero_()                                   # less e^-32 of the others, next to nothing
+    ref, mag, _ = ref_attention(s, 0)
+    assert (ref.abs() < 2.0 ** -16 * mag).all()
+    check(run_attention(s)[0, 0], ref, 12 * 2.0 ** -23 * mag)
+    o, xn = run_step(s, append=False)
+    ref, mag, _ = ref_attention(s, 0, (s["k"][0], xn[0]))
+    check(o[0, 0], ref, 12 * 2.0 ** -23 * mag)
     _lib.check_status()
