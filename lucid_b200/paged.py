@@ -390,7 +390,10 @@ class PagedBatch:
 
     One model step is ``reserve(counts)``, then ``append`` or ``step`` in every layer, then
     ``advance()``; LucidForCausalLM.forward does all three.  ``block_table``, ``lengths``
-    and ``counts`` are the device tensors the operators read."""
+    and ``counts`` are the device tensors the operators read; they are written in place, so
+    a captured ``append`` or ``step`` follows them.  Replay it where the eager call would
+    be, after ``reserve`` (a replay checks nothing) and before ``advance``, and keep the batch as long
+    as the graph.  A batch whose table a graph reads cannot outgrow it: ``reserve`` refuses."""
 
     def __init__(self, cache: PagedCache, sequences):
         self.cache = cache
@@ -406,6 +409,7 @@ class PagedBatch:
         self._host_lengths: list[int] = []
         self._host_counts: list[int] = []
         self.block_table = self.lengths = self.counts = None
+        self._captured = False                               # a graph reads these three
 
     def __len__(self) -> int:
         return len(self.sequences)
@@ -438,6 +442,9 @@ class PagedBatch:
                     shared.append(s)
                     need += 1
             need += max(0, -(-(s.length + n) // ps) - len(s.pages))
+        if self._captured and max(-(-(s.length + n) // ps) for s, n in zip(seqs, counts)) > self.block_table.shape[1]:
+            raise LucidError(f"a sequence outgrows the {self.block_table.shape[1]} pages of the block table that a captured "
+                             "graph reads: make a new batch of the sequences and capture again")
         if need > len(c._free):
             raise LucidError(f"the paged cache is full: {need} pages needed, {len(c._free)} of {len(c._refs)} free")
         src, dst = [s.pages[s.length // ps] for s in shared], [c._take() for _ in shared]
@@ -460,24 +467,29 @@ class PagedBatch:
 
     def _upload(self, seqs, counts) -> None:
         """Brings the device tensors up to date, touching those that changed."""
-        dev = self.cache.key_pages.device
         edits = [s.edits for s in seqs]
         if edits != self._edits or self.block_table is None:
             width = max(1, max(len(s.pages) for s in seqs))
             if width > self._table.shape[1]:                 # with room to grow: a page at a time is usual
-                self._table = torch.full((len(seqs), width + width // 2 + 8), -1, dtype=torch.int32)
-                self._edits = []
+                table = torch.full((len(seqs), width + width // 2 + 8), -1, dtype=torch.int32)
+                self.block_table = torch.empty_like(table, device=self.cache.key_pages.device)
+                self._table, self._edits = table, []
             for i, s in enumerate(seqs):
                 if not self._edits or self._edits[i] != edits[i]:
                     self._table[i, :len(s.pages)] = torch.tensor(s.pages, dtype=torch.int32)
-            self.block_table, self._edits = self._table.to(dev, copy=True), edits
+            self.block_table.copy_(self._table)
+            self._edits = edits
         lengths = [s.length for s in seqs]
-        if lengths != self._host_lengths or self.lengths is None:
-            self.lengths = torch.tensor(lengths, dtype=torch.int32).to(dev)
+        if lengths != self._host_lengths:
+            self.lengths = self._fill(self.lengths, lengths)
             self._host_lengths = lengths
-        if counts != self._host_counts or self.counts is None:
-            self.counts = torch.tensor(counts, dtype=torch.int32).to(dev)
+        if counts != self._host_counts:
+            self.counts = self._fill(self.counts, counts)
             self._host_counts = counts
+
+    def _fill(self, t: torch.Tensor | None, values) -> torch.Tensor:
+        host = torch.tensor(values, dtype=torch.int32)
+        return host.to(self.cache.key_pages.device, copy=True) if t is None else t.copy_(host)
 
     def _check(self) -> None:
         if self._counts is None:
@@ -488,6 +500,8 @@ class PagedBatch:
             if self.host_lengths != self._host_lengths:
                 raise LucidError("a sequence has grown in another batch since reserve(): reserve again")
             self._steps = self.cache._steps
+        if torch.cuda.is_current_stream_capturing():
+            self._captured = True
 
     def append(self, layer: int, key: torch.Tensor, x: torch.Tensor) -> None:
         """The reserved tokens' rows of one layer, key / x [B,Hkv,N,D] with N at least the
@@ -513,7 +527,7 @@ class PagedBatch:
         self._check()
         for s, n in zip(self.sequences, self._counts):
             self.cache._sequences[s].length += n
-        self.lengths = self.lengths + self.counts
+        self.lengths.add_(self.counts)
         self._host_lengths = [a + n for a, n in zip(self._host_lengths, self._counts)]
         self._counts = None
         self.cache._steps += 1

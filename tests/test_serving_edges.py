@@ -1,0 +1,52 @@
+"""The serving operators' host side at the edges of what it takes, without a GPU."""
+import pytest
+import torch
+
+import lucid_b200 as lb
+from lucid_b200 import _lib
+from test_paged import _cache, _held, _write, on_cpu  # noqa: F401
+
+
+def test_a_batch_keeps_its_device_tensors(on_cpu):
+    """A captured step reads the tensors' addresses: the bookkeeping writes into them."""
+    cache = _cache(pages=40)
+    batch = cache.batch(cache.new(2))
+    _write(batch, [3, 5], [[1, 2, 3], [4, 5, 6, 7, 8]])
+    kept = [batch.block_table, batch.lengths, batch.counts]
+    other = cache.batch(cache.new())
+    for step in range(12):
+        if step == 4:
+            cache.free(cache.fork(batch.sequences[0]))
+        if step == 8:
+            _write(other, [1], [[0]])
+            other = cache.batch(cache.new())
+        _write(batch, [1, step % 2], [[step], [step][:step % 2]])
+        assert all(a is b for a, b in zip(kept, (batch.block_table, batch.lengths, batch.counts)))
+        assert batch.lengths.tolist() == batch.host_lengths and batch.counts.tolist() == [1, step % 2]
+        for row, s in zip(batch.block_table.tolist(), batch.sequences):
+            assert row[:len(cache.pages(s))] == cache.pages(s)
+    assert _held(cache, batch.sequences[0], 0) == [1, 2, 3, *range(12)]
+
+
+def test_a_captured_batch_refuses_to_outgrow_its_table(on_cpu, monkeypatch):
+    """With nothing changed; a new batch of the sequences goes on."""
+    cache = _cache(pages=60)
+    batch = cache.batch(cache.new(2))
+    k = torch.zeros(2, 1, 1, 4, dtype=torch.bfloat16)
+    batch.reserve(1)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    batch.append(0, k, k)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    batch.advance()
+    room = batch.block_table.shape[1]
+    child = cache.fork(batch.sequences[0])
+    batch.reserve(room * 4 - 1)
+    kept, free, refs = batch.block_table, cache.free_pages, list(cache._refs)
+    with pytest.raises(_lib.LucidError, match="capture again"):
+        batch.reserve([1, room * 4])
+    assert batch.block_table is kept and cache.free_pages == free and cache._refs == refs
+    assert cache.pages(child) and batch.host_lengths == [1, 1]
+    batch = cache.batch(batch.sequences)
+    batch.reserve([1, room * 4])
+    batch.advance()
+    assert batch.host_lengths == [2, room * 4 + 1]

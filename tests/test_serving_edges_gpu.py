@@ -51,3 +51,57 @@ def test_weights_keep_the_bits_of_fp32(cuda_device, gq):
     ref, mag, _ = ref_attention(s, 0, (s["k"][0], xn[0]))
     check(o[0, 0], ref, 12 * 2.0 ** -23 * mag)
     _lib.check_status()
+
+
+def test_a_captured_batch_step_follows_the_bookkeeping(cuda_device):
+    """reserve, replay, advance, with forks, frees, moved pages and another batch's steps in
+    between: the same bits as a twin cache's eager steps, and no page but the reserved rows
+    changes."""
+    H, D, ps = 2, 68, 16
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    rn = lambda *shape: torch.randn(*shape, generator=g, device=cuda_device).bfloat16()
+    caches = [lb.PagedCache(2, H, D, 60, ps, device=cuda_device) for _ in range(2)]
+    batches = [c.batch(c.new(3)) for c in caches]
+    prompt = [rn(3, H, 40, D) for _ in range(2)]
+    for c, b in zip(caches, batches):
+        c.key_pages.zero_()
+        c.x_pages.zero_()
+        b.reserve([40, 15, 31])
+        for layer in range(2):
+            b.append(layer, *prompt)
+        b.advance()
+    q, k, v = rn(3, 4, 1, D), rn(3, H, 1, D), rn(3, H, 1, D)
+    scale = D ** -0.5
+    batches[0].reserve(1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [batches[0].step(layer, q, k, v, scale) for layer in range(2)]
+    for step in range(40):
+        for t in (q, k, v):
+            t.copy_(rn(*t.shape))
+        for c, b in zip(caches, batches):
+            if step == 3:
+                c.fork(b.sequences[1])
+            if step == 9:
+                c.free(3)
+            if step == 12:
+                spare = c.batch(c.new(2))
+                spare.reserve(30)
+                for layer in range(2):
+                    spare.append(layer, prompt[0][:2], prompt[1][:2])
+                spare.advance()
+            if step == 20:
+                c.free(4)
+                c.compact()
+            b.reserve(1)
+        graph.replay()
+        batches[0].advance()
+        want = [batches[1].step(layer, q, k, v, scale) for layer in range(2)]
+        batches[1].advance()
+        for (o, x), (o2, x2) in zip(out, want):
+            assert torch.equal(o, o2) and torch.equal(x, x2)
+        for t in ("key_pages", "x_pages"):
+            assert torch.equal(getattr(caches[0], t), getattr(caches[1], t)), step
+    assert batches[0].lengths.tolist() == batches[0].host_lengths == [80, 55, 71]
+    _lib.check_status()
