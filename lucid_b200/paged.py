@@ -465,6 +465,7 @@ class PagedBatch:
         self._upload(seqs, counts)
         self._counts, self._version, self._steps = counts, c._version, c._steps
 
+    @torch.inference_mode(False)   # a tensor made in inference mode could not be written outside it
     def _upload(self, seqs, counts) -> None:
         """Brings the device tensors up to date, touching those that changed."""
         edits = [s.edits for s in seqs]

@@ -50,3 +50,16 @@ def test_a_captured_batch_refuses_to_outgrow_its_table(on_cpu, monkeypatch):
     batch.reserve([1, room * 4])
     batch.advance()
     assert batch.host_lengths == [2, room * 4 + 1]
+
+
+def test_bookkeeping_in_and_out_of_inference_mode(on_cpu):
+    """Tensors made in inference mode could not be written outside it."""
+    cache = _cache(pages=40)
+    a = cache.new(2)
+    batch = cache.batch(a)
+    with torch.inference_mode():
+        _write(batch, [3, 5], [[1, 2, 3], [4, 5, 6, 7, 8]])
+    _write(batch, [6, 1], [[4, 5, 6, 7, 8, 9], [9]])
+    with torch.inference_mode():
+        _write(batch, [1, 1], [[10], [10]])
+    assert _held(cache, a[0], 1) == [2, 3, 4, 5, 6, 7, 8, 9, 10, 11] and batch.lengths.tolist() == [10, 7]
