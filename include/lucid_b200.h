@@ -446,6 +446,7 @@ int lucid_cp_solve_bwd(int B, int H, int N, int D, float scale, int blk_lo, int 
  *     o     = softmax over the n cached tokens and the new one of s q . k, times x
  *   q, o [B, Hq, D], k_new, v_new, x_new [B, Hkv, D] with strides (sb, sh).  append != 0
  *   also writes k_new and x_new into row n of the sequence's pages.
+ *   Without query heads (Hq = 0) or sequences nothing is computed and nothing written.
  * lucid_paged_decode_attn: the attention alone, over the n cached tokens (none: zeros).
  * Both split the cached tokens of the whole batch evenly over the GPU whatever the
  * lengths; weights and sums are fp32, results are the same from run to run.

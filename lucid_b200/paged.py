@@ -142,6 +142,8 @@ def paged_decode_step(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     dev, index, kp, ks, xp, xs = _pools(key_pages, x_pages)
     P, Hkv, ps, D = key_pages.shape
     B, Hq = _one_token(query)
+    if Hq == 0:
+        raise ValueError("query: a step needs at least one query head")
     query, qp, qs = _rows(query, "query", (B, Hq, 1, D), dev)
     key, kn, kns = _rows(key, "key", (B, Hkv, 1, D), dev)
     value, vn, vns = _rows(value, "value", (B, Hkv, 1, D), dev)

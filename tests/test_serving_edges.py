@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import lucid_b200 as lb
-from lucid_b200 import _lib
+from lucid_b200 import _lib, paged
 from test_paged import _cache, _held, _write, on_cpu  # noqa: F401
 
 
@@ -63,3 +63,15 @@ def test_bookkeeping_in_and_out_of_inference_mode(on_cpu):
     with torch.inference_mode():
         _write(batch, [1, 1], [[10], [10]])
     assert _held(cache, a[0], 1) == [2, 3, 4, 5, 6, 7, 8, 9, 10, 11] and batch.lengths.tolist() == [10, 7]
+
+
+def test_without_query_heads_there_is_no_step(monkeypatch):
+    """The new token's key would be neither solved nor cached."""
+    monkeypatch.setattr(_lib, "_lib", object())
+    monkeypatch.setattr(paged, "_pools", lambda k, x: (k.device, 0, 0, k.stride(), 0, x.stride()))
+    t = torch.zeros(2, 0, 1, 64, dtype=torch.bfloat16)
+    kv = torch.zeros(2, 2, 1, 64, dtype=torch.bfloat16)
+    pool = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    n = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="query"):
+        lb.paged_decode_step(t, kv, kv, pool, pool, n[:, None], n, 0.1)
