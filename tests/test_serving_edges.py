@@ -75,3 +75,25 @@ def test_without_query_heads_there_is_no_step(monkeypatch):
     n = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="query"):
         lb.paged_decode_step(t, kv, kv, pool, pool, n[:, None], n, 0.1)
+
+
+def test_the_entry_script_defines_what_it_runs():
+    """python __graft_entry__.py smoke: everything that smoke() calls is there when the
+    block at the script's end calls it."""
+    import ast
+    import os
+
+    from conftest import ROOT
+    with open(os.path.join(ROOT, "__graft_entry__.py")) as f:
+        body = ast.parse(f.read()).body
+    main = [i for i, n in enumerate(body) if isinstance(n, ast.If) and "__main__" in ast.unparse(n.test)]
+    defined = [n.name for n in body[:main[0]] if isinstance(n, ast.FunctionDef)]
+    everywhere = {n.name: n for n in body if isinstance(n, ast.FunctionDef)}
+    assert "smoke" in defined and len(main) == 1
+    reached, todo = set(), ["smoke", "build"]
+    while todo:
+        name = todo.pop()
+        if name not in reached:
+            reached.add(name)
+            todo += [n.id for n in ast.walk(everywhere[name]) if isinstance(n, ast.Name) and n.id in everywhere]
+    assert reached <= set(defined)
