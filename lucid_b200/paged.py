@@ -37,13 +37,16 @@ __all__ = ["paged_decode_step", "paged_decode_attention", "paged_append", "copy_
 
 _NO_GUARD = contextlib.nullcontext()
 _BF16, _INT32 = torch.bfloat16, torch.int32
-_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream(i).cuda_stream without building a Stream
-_current_device = torch._C._cuda_getDevice
+
+
+def _raw_stream(index: int) -> int:
+    """current_stream(index).cuda_stream without building a Stream."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _on(index: int):
     """Context in which device ``index``, which holds a tensor, is the current one."""
-    return _NO_GUARD if _current_device() == index else torch.cuda.device(index)
+    return _NO_GUARD if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
 @functools.lru_cache(maxsize=1024)

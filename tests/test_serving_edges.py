@@ -97,3 +97,31 @@ def test_the_entry_script_defines_what_it_runs():
             reached.add(name)
             todo += [n.id for n in ast.walk(everywhere[name]) if isinstance(n, ast.Name) and n.id in everywhere]
     assert reached <= set(defined)
+
+
+def _runs(code):
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    got = subprocess.run([sys.executable, "-c", code + "\nprint('fine')"], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and got.stdout.strip().endswith("fine"), got.stderr[-2000:]
+
+
+def test_the_package_imports_on_a_torch_without_cuda():
+    """Its C module lacks these names."""
+    _runs("""
+import torch
+for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+import lucid_b200 as lb
+t = torch.zeros(4, 1, 4, 4, dtype=torch.bfloat16)
+for call in (lambda: lb.copy_pages(t, t, [0], [1]), lambda: lb.token_logprobs(torch.zeros(2, 5), None)):
+    try:
+        call()
+    except RuntimeError as e:
+        assert "no CPU fallback" in str(e), e
+    else:
+        raise AssertionError
+""")
