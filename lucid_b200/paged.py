@@ -49,6 +49,13 @@ def _on(index: int):
     return _NO_GUARD if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
+def _capturing() -> bool:
+    try:
+        return torch.cuda.is_current_stream_capturing()
+    except RuntimeError:             # no usable CUDA: a cache on the CPU keeps its books
+        return False
+
+
 @functools.lru_cache(maxsize=1024)
 def _workspace_words(index: int, B: int, Hq: int, Hkv: int, D: int, step: int) -> int:
     """Decoding workspace on device ``index`` (the current one), in 4-byte words."""
@@ -368,7 +375,7 @@ class PagedCache:
     def compact(self) -> int:
         """Moves the pages in use to the front of the pool (every page at or past the number
         in use goes to a free one before it) and returns how many moved."""
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             raise LucidError("PagedCache.compact works on the host: call it outside the capture")
         used = len(self._refs) - len(self._free)
         src = [p for p in range(used, len(self._refs)) if self._refs[p]]
@@ -431,7 +438,7 @@ class PagedBatch:
         """Assigns the pages for ``counts`` more tokens of each sequence (one number for
         all, or one each) and copies shared pages that would be written.  Raises LucidError,
         with nothing changed, when the pool has too few free pages or the copy fails."""
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             raise LucidError("PagedBatch.reserve works on the host: call it before the capture")
         c = self.cache
         seqs = [c._get(s) for s in self.sequences]
@@ -506,7 +513,7 @@ class PagedBatch:
             if self.host_lengths != self._host_lengths:
                 raise LucidError("a sequence has grown in another batch since reserve(): reserve again")
             self._steps = self.cache._steps
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             self._captured = True
 
     def append(self, layer: int, key: torch.Tensor, x: torch.Tensor) -> None:
@@ -528,7 +535,7 @@ class PagedBatch:
 
     def advance(self) -> None:
         """Counts the reserved tokens as cached."""
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             raise LucidError("PagedBatch.advance works on the host: call it after the capture")
         self._check()
         for s, n in zip(self.sequences, self._counts):

@@ -125,3 +125,20 @@ for call in (lambda: lb.copy_pages(t, t, [0], [1]), lambda: lb.token_logprobs(to
     else:
         raise AssertionError
 """)
+
+
+def test_the_cache_keeps_its_books_without_a_gpu():
+    """Asking for the capture of a stream raises where CUDA cannot be used."""
+    _runs("""
+import torch
+def none():
+    raise RuntimeError("no CUDA here")
+torch.cuda.is_current_stream_capturing = none
+import lucid_b200 as lb
+cache = lb.PagedCache(1, 1, 4, 12, 4, device="cpu")
+batch = cache.batch(cache.new(2))
+batch.reserve([3, 5])
+batch.advance()
+cache.free(batch.sequences[0])
+assert cache.free_pages == 10 and cache.length(batch.sequences[1]) == 5
+""")
