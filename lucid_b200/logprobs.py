@@ -5,6 +5,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from .paged import _on, _raw_stream
@@ -109,9 +110,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
     have probability 0; a row without a distribution (all -inf, a NaN or +inf in it)
     gives NaN and top tokens -1.  A token outside the vocabulary is reported by the next
     call or ``check_status()``.  Differentiable once in logits through ``logprobs`` and
-    ``entropy``; the arithmetic is fp32, the gradient has the logits' type.  To capture the
-    backward into a CUDA graph use torch.autograd.grad: ``backward()`` on a leaf that an
-    eager graph also holds makes torch wait for another stream, which a capture cannot."""
+    ``entropy``, in reverse mode; the arithmetic is fp32, the gradient has the logits' type.
+    To capture the backward into a CUDA graph use torch.autograd.grad: ``backward()`` on a
+    leaf that an eager graph also holds makes torch wait for another stream, which a capture
+    cannot."""
+    if unpack_dual(logits).tangent is not None:
+        raise NotImplementedError("token_logprobs: no forward mode, only the gradient of logprobs and entropy")
     if not logits.is_cuda:
         raise RuntimeError("logits: LUCID B200 kernels need CUDA tensors (no CPU fallback)")
     if logits.dtype not in _DTYPES:

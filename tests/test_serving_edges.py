@@ -142,3 +142,19 @@ batch.advance()
 cache.free(batch.sequences[0])
 assert cache.free_pages == 10 and cache.length(batch.sequences[1]) == 5
 """)
+
+
+def test_token_logprobs_refuse_forward_mode():
+    """The tangent of the logits would be dropped."""
+    from torch.autograd import forward_ad
+    x = torch.randn(2, 5, requires_grad=False)
+    with forward_ad.dual_level():
+        for logits in (forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(x.clone().requires_grad_(), x)[:, :4]):
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                lb.token_logprobs(logits, None)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
+                lb.token_logprobs(logits, None)
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            lb.token_logprobs(x, None)
+    with pytest.raises(NotImplementedError, match="forward mode"):
+        torch.func.jvp(lambda z: lb.token_logprobs(z, None).entropy, (x,), (x,))
