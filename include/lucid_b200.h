@@ -505,6 +505,7 @@ int lucid_copy_pages(int layers, int P, int64_t page_bytes, void* k_pages, int64
  * lucid_token_logprobs_bwd: dlogits [R][V] (contiguous, the logits' dtype) =
  *   g_logprobs (1[token] - p) - g_entropy p (log p + H); either factor may be NULL (zero).
  *   Rows with both factors zero are written as zeros without being read.
+ *   A token outside the vocabulary (but -100) makes its row NaN unless g_logprobs is 0 there.
  */
 #define LUCID_MAX_TOP 64
 int lucid_token_logprobs(int64_t R0, int64_t R1, int V, int dtype, const void* logits, int64_t s0, int64_t s1,

@@ -878,8 +878,10 @@ __global__ void __launch_bounds__(kLpThreads, 3) logprobs_bwd_kernel(const __gri
   constexpr int VE = RowView<T>::VE;
   const long long r = blockIdx.x;
   const long long tk = a.tokens != nullptr ? a.tokens[r] : -100;
-  const int tok = tk >= 0 && tk < a.V ? (int)tk : INT_MIN;   // anything else has no element
-  const float gl = a.g_lp != nullptr && tk >= 0 ? a.g_lp[r] : 0.f;
+  const bool given = tk >= 0 && tk < a.V;
+  const int tok = given ? (int)tk : INT_MIN;                 // anything else has no element
+  float gl = a.g_lp != nullptr && tk != -100 ? a.g_lp[r] : 0.f;
+  if (!given && gl != 0.f) gl = __int_as_float(0x7fc00000);  // like the log probability
   const float ge = a.g_ent != nullptr ? a.g_ent[r] : 0.f;
   const T* in = static_cast<const T*>(a.logits) + (r / a.R1) * a.s0 + (r % a.R1) * a.s1;
   T* out = static_cast<T*>(a.dlogits) + r * a.V;

@@ -105,3 +105,23 @@ def test_a_captured_batch_step_follows_the_bookkeeping(cuda_device):
             assert torch.equal(getattr(caches[0], t), getattr(caches[1], t)), step
     assert batches[0].lengths.tolist() == batches[0].host_lengths == [80, 55, 71]
     _lib.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_gradient_of_tokens_outside_the_vocabulary(cuda_device, dtype):
+    """NaN like their log probability, whichever side they are on; without a factor for it, and
+    for -100, the entropy's alone."""
+    x = torch.randn(8, 50, generator=torch.Generator(device=cuda_device).manual_seed(1), device=cuda_device).to(dtype)
+    t = torch.tensor([1, 50, -1, 2 ** 40, -99, -100, 60, -7], device=cuda_device)
+    gl = torch.tensor([1., 2., -1., .5, 3., 1., 0., 0.], device=cuda_device)
+    for ge in (torch.zeros(8, device=cuda_device), torch.linspace(-1, 1, 8, device=cuda_device)):
+        x.requires_grad_(True)
+        got = lb.token_logprobs(x, t)
+        with pytest.raises(_lib.LucidError, match="a token lies outside the vocabulary"):
+            _lib.check_status()
+        d, = torch.autograd.grad([got.logprobs, got.entropy], x, [gl, ge])
+        assert d[1:5].isnan().all() and torch.isfinite(d[[0, 5, 6, 7]]).all()
+        alone = lb.token_logprobs(x, None)
+        want, = torch.autograd.grad(alone.entropy, x, ge)
+        assert torch.equal(d[5:], want[5:])
+    _lib.check_status()
