@@ -1,10 +1,13 @@
 """The serving operators at the edges of what they take, on the GPU.  Tolerances as in
 test_paged_gpu.py and test_logprobs_gpu.py."""
+import math
+
 import pytest
 import torch
 
 import lucid_b200 as lb
 from lucid_b200 import _lib
+from test_logprobs_gpu import rows
 from test_paged_gpu import check, check_attention, check_step, make, ref_attention, run_attention, run_step
 
 pytestmark = pytest.mark.gpu
@@ -125,3 +128,48 @@ def test_the_gradient_of_tokens_outside_the_vocabulary(cuda_device, dtype):
         want, = torch.autograd.grad(alone.entropy, x, ge)
         assert torch.equal(d[5:], want[5:])
     _lib.check_status()
+
+
+def test_append_tells_a_page_from_a_length(cuda_device):
+    """One cause each: a page missing inside the table, rows past a table of valid pages."""
+    for table, count, match in (([0, -1, 2], 20, "a page of the block table"), ([0, 9, 2], 20, "a page of the block table"),
+                                ([0, 1, 2], 49, "past the block table")):
+        kp = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device=cuda_device)
+        xp = torch.zeros_like(kp)
+        k = torch.ones(1, 2, 60, 64, dtype=torch.bfloat16, device=cuda_device)
+        n, c = (torch.tensor([v], dtype=torch.int32, device=cuda_device) for v in (0, count))
+        lb.paged_append(k, k, kp, xp, torch.tensor([table], dtype=torch.int32, device=cuda_device), n, c)
+        with pytest.raises(_lib.LucidError, match=match):
+            _lib.check_status()
+        written = [0, 1, 2] if count == 49 else [0]
+        assert torch.equal(kp, xp) and [p for p in range(4) if kp[p].any()] == written and (kp[written] == 1).all()
+    _lib.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("R,V", [(3, 5), (4, 1000), (2, 32001)])
+def test_the_gradient_of_the_entropy_without_tokens(cuda_device, dtype, R, V):
+    """Tolerance of the gradient as in test_logprobs_gpu.py, g_lp 0."""
+    x = rows(cuda_device, (R, V), dtype, seed=V)
+    x[0, V // 2] = -math.inf
+    x.requires_grad_(True)
+    ge = torch.randn(R, generator=torch.Generator(device=cuda_device).manual_seed(3), device=cuda_device)
+    got = lb.token_logprobs(x, None)
+    assert got.logprobs is None
+    d, = torch.autograd.grad(got.entropy, x, ge)
+    lp = torch.log_softmax(x.detach().double(), -1)
+    p, lpf = lp.exp(), torch.where(lp > -math.inf, lp, 0.0)
+    h = -(p * lpf).sum(-1, keepdim=True)
+    want = -ge[:, None] * p * (lpf + h)
+    mag = ge.abs()[:, None] * (lpf.abs() + h + 1) * p
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + mag * (V / 512 + 28 + 2 * lpf.abs()) * 2.0 ** -23 * (1 + math.log(V)) \
+        + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    assert d.dtype == dtype and ((d.double() - want).abs() <= tol).all()
+    _lib.check_status()
+
+
+def test_forward_mode_is_refused_on_the_gpu(cuda_device):
+    from torch.autograd import forward_ad
+    x = torch.randn(2, 5, device=cuda_device)
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+        lb.token_logprobs(forward_ad.make_dual(x, x), None)
