@@ -324,6 +324,8 @@ class PagedCache:
 
     def new(self, count: int = 1) -> list[int]:
         """``count`` empty sequences; a sequence is known by its number."""
+        if count < 0:
+            raise ValueError(f"new: a count of {count} sequences")
         made = list(range(self._next, self._next + count))
         self._next += count
         for i in made:

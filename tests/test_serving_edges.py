@@ -158,3 +158,14 @@ def test_token_logprobs_refuse_forward_mode():
             lb.token_logprobs(x, None)
     with pytest.raises(NotImplementedError, match="forward mode"):
         torch.func.jvp(lambda z: lb.token_logprobs(z, None).entropy, (x,), (x,))
+
+
+def test_a_negative_count_of_new_sequences(on_cpu):
+    """It would hand out the numbers of living sequences again."""
+    cache = _cache()
+    a, b = cache.new(2)
+    _write(cache.batch([b]), [2], [[1, 2]])
+    for bad in (-1, -2):
+        with pytest.raises(ValueError, match="count"):
+            cache.new(bad)
+    assert cache.new(0) == [] and cache.new() == [b + 1] and _held(cache, b, 0) == [1, 2]
