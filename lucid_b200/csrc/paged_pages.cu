@@ -75,8 +75,8 @@ cudaError_t launch_paged_append(const PagedAppendArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// One block per 16 KB segment of one (pair, layer, tensor); four vectors in flight per
-// thread.
+// One block per segment of one (pair, layer, tensor), 16 KB of it, or 8 KB where vectors are
+// 8 bytes; four vectors in flight per thread.
 constexpr int kCopyThreads = 256, kCopyUnroll = 4;
 
 template <typename V>

@@ -56,7 +56,7 @@ int decode(bool step, int B, int Hq, int Hkv, int D, int P, int ps, int M, float
     return LUCID_ERR_ALIGN;
   if (!ptr_ok(workspace, 16) || workspace_bytes < decode_bytes(B, Hq, Hkv, D, step)) return LUCID_ERR_WORKSPACE;
   PagedDecodeArgs a{};
-  a.B = B; a.H = Hkv; a.Hq = Hq; a.D = D; a.P = P; a.ps = ps; a.M = M;
+  a.B = B; a.H = Hkv; a.D = D; a.P = P; a.ps = ps; a.M = M;
   a.ps_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (ps == 1 << s) a.ps_shift = s;

@@ -30,7 +30,7 @@ struct PoolView {
 
 // Paged decoding of one new token per sequence (csrc/paged_decode.cu).
 struct PagedDecodeArgs {
-  int B, H, Hq, D;             // sequences, kv heads, query heads, head dimension
+  int B, H, D;                 // sequences, kv heads, head dimension
   int P, ps, M;                // pool pages, page size, block table width
   int ps_shift;                // log2 of the page size, -1 if it is no power of two
   int gq, nblk, rows, nctas;   // query heads per kv head, row blocks of them, rows per block, CTAs (set by the launch)
@@ -43,7 +43,7 @@ struct PagedDecodeArgs {
   const int* lengths;
   bf16* xo; long long xo_sb, xo_sh;         // solved new values (step only)
   bf16* o;  long long o_sb, o_sh;
-  float* part;                              // [nctas + B H nblk][rows][D + 4]
+  float* part;                              // [nctas + B H nblk][rows, and one in the step][D + 4]
   int* status;
   int append;                               // step: write (kn, xo) into the pages
 };
