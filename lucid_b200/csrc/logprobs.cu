@@ -670,9 +670,9 @@ __global__ void __launch_bounds__(NT, lp_blocks(NT, TOP)) logprobs_fwd_kernel(co
 // batch with its maximum, where that reaches the threshold: one test for 40 elements, and
 // the final threshold drops most of the list (about 140 of a row of 25 batches, with 20
 // alternatives) without a look at its elements.
-// 8190 rows of 32000 bf16, 20 best: 119 us with 28 warps of 5 vectors a thread to an SM, 125
-// with 24 of 8 or 28 of 4.  What bounds it: issue slots are busy 63 % of the time, DRAM moves
-// 4.4 TB/s; of the 8.9 cycles that a warp takes for an instruction 2.1 are fixed latency, 1.1
+// 8190 rows of 32000 bf16, 20 best: 120 us with 28 warps of 5 vectors a thread to an SM, 125
+// with 24 of 8 or 28 of 4.  What bounds it: issue slots are busy 63 % of the time; 4.4 TB/s of
+// logits, 4.9 with the second look at the listed batches; of the 8.9 cycles that a warp takes for an instruction 2.1 are fixed latency, 1.1
 // loads, 2.0 shuffles and shared memory, 1.7 other warps' turns.
 constexpr int kLpWarpBlocks = 28;
 constexpr int kLpWarpHits = 320;
@@ -992,16 +992,19 @@ static cudaError_t launch_warp(const LogprobArgs& a, cudaStream_t st) {
 // With up to 24 alternatives a warp a row, once there are rows enough to hide that a warp
 // needs 10 us and 4 more per 1000 vectors for its row.  20 best, bf16, us with a warp / 128 /
 // 512 threads:
-//   8190 x 32000   119 / 172 / 232      1200 x 32000    33 /  38 / 39      600 x 32000   29 / 25 / 25
-//   4100 x 128000  200 / 633 / 271      1200 x 128000  101 / 263 / 87      600 x 16000   21 / 15 / 25
+//   8190 x 32000   120 / 173 / 230      1200 x 32000    33 /  38 / 39      600 x 32000   29 / 25 / 25
+//   4100 x 128000  200 / 640 / 270      1200 x 128000  101 / 263 / 87      600 x 16000   21 / 15 / 25
 //   9000 x 2000     31 /  82 / 290       600 x 2000     10 /  10 / 27      150 x 2000     9 /  8 / 12
+// fp32, where a row has twice the vectors, crosses at the same counts of them:
+//   1800 x 32000    56 /  84 /  64      1200 x 32000    47 /  69 / 45       900 x 2000    12 / 14 / 27
+//   2600 x 65000   119 / 411 / 133      1800 x 65000    95 / 336 / 94       600 x 2000    11 /  8 / 21
 // so from 900 rows and one more for every 16 vectors of a row, or 300 where a row is two
 // batches; but to 128 batches a row, whose list the doublings still fit (2500 x 160000: 183 /
 // 605 / 211; 4200 x 200000, which it does not always: 478 / 1232 / 438).  Below that 128 threads
 // where the rows are at least 150 for each of their batches, of which four at most (the
 // first one sets the threshold for the lists: 900 x 65000: 68 and with 512 threads 49), else 512.
-// More alternatives than the 32 groups serve: 512 threads (50 best of 8190 x 32000: 283 with 128
-// threads and 260), but for a row of one batch (900 x 500: 86 with 512, 17 with 128).
+// More alternatives than the 32 groups serve: 512 threads (50 best of 8190 x 32000: 305 with 128
+// threads and 261), but for a row of one batch (900 x 500: 86 with 512, 17 with 128).
 template <typename T>
 static cudaError_t launch_fwd_t(const LogprobArgs& a, cudaStream_t st) {
   constexpr int VE = RowView<T>::VE, kShort = kLpHold * 128 * VE;  // a batch of 128 threads

@@ -10,9 +10,12 @@
 //   S = A K^T (mma m16n8k16: exact bf16 products, fp32 sums), the scores scaled
 //   afterwards in fp32 (softmax rows by s, the update row by s rstd_new rstd_t), and
 //   acc += P X with P split into three bf16 parts, which hold all 24 bits of an fp32
-//   weight: the products are exact, the sums fp32.  (Two parts, 16 bits, are 0 to 3 % faster
-//   at 8 query heads per kv head, 30.8 and 29.9 us a call for 24 ragged sequences, and
-//   slower at one.)
+//   weight, so the products are exact.  A tile's are summed from zero by the MMAs, then added
+//   to the row's sums: an MMA cuts its result off instead of rounding it, which over the
+//   148 tiles of a CTA at 4 x 32765 tokens left 70 of 32768 results on the other side of a bf16
+//   rounding than the exact ones, now 2.  (Two parts, 16 bits: 46.  Time on one GPU, 24
+//   ragged sequences with 8 query heads per kv head / 4 x 32765 tokens with one: 31.3 / 338 us
+//   a pass with the sums left to the MMAs, 32.5 / 341 as it is, 31.2 / 335 with two parts.)
 // sum(k_t^2) is the diagonal of K K^T, computed by the same instructions: the B fragment
 // of a key tile is also its A fragment, and with at most 8 query rows it rides in the
 // rows of A that S leaves empty.
@@ -27,8 +30,8 @@
 //
 // The products are mma.sync's: a kv head brings 1 to 16 rows a step, where a tcgen05 tile
 // has 64 or more and would hand its scores back through tensor memory for the softmax.
-// HBM bounds the pass (4 x 32765 tokens, 32 heads of 128: 2.15 GB in 327 us, 6.5 TB/s), the
-// tensor pipe is active 16 % of it.
+// HBM bounds the pass (4 x 32765 tokens, 32 heads of 128: 2.15 GB in 324 to 340 us a call on
+// different GPUs, 6.3 to 6.6 TB/s); over 4 x 8189 tokens the tensor pipe is active 30 % of it.
 #include "paged_flat.h"
 #include "serve_common.cuh"
 
@@ -47,6 +50,20 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// the same from zero
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// two rounded sums in one instruction
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+  asm("{\n.reg .b64 s, t;\nmov.b64 s, {%0, %1};\nmov.b64 t, {%2, %3};\nadd.rn.f32x2 s, s, t;\nmov.b64 {%0, %1}, s;\n}"
+      : "+f"(x), "+f"(y) : "f"(a), "f"(b));
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -87,7 +104,8 @@ __device__ __forceinline__ int pd_tiles(int n) { return (int)(((unsigned)n + kPd
 // An item counts as its tiles and kPdItemCost more in front of them, about what its
 // queries' loads and its merge of the warps cost: batches with many short sequences would
 // otherwise give some CTAs a dozen items and others none.  24 sequences of 4 to 6007 tokens
-// (4 kv heads of 68): 34.8 us without, 28.9, 23.1 and 23.8 us with 1, 2 and 4.
+// (4 kv heads of 68): 35.8 us without, 28.7, 24.6 and 25.7 us with 1, 2 and 4; the attention of
+// 48 sequences of 0 to 8150 tokens (4 of 128): 52.6, 48.7, 48.1 and 48.3 us.
 __device__ __forceinline__ int pd_units(int n) { return n > 0 ? pd_tiles(n) + kPdItemCost : 0; }
 
 // units of the whole batch (every lane returns the sum)
@@ -207,9 +225,10 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
 enum : int { kRows = 0, kFull = 1, kFlat = 2 };
 
 // Three CTAs of four warps per SM where the registers allow (at most 168 a thread): the
-// tile loop is a chain of short dependent steps, and D = 128 over 4 x 32K tokens took
-// 388 us with two CTAs and three stages, 336 us with three and two.  16 rows at D > 96,
-// and the addresses of odd rows at D > 64, need more registers.
+// tile loop is a chain of short dependent steps.  24 ragged sequences at D = 68 take 28.1 us
+// with two CTAs and 24.6 with three; at D = 128, with three stages for two CTAs and two for
+// three, 4 x 32K tokens take 334 us either way, 48 ragged sequences 46.8 and 48.1.  16 rows at
+// D > 96, and the addresses of odd rows at D > 64, need more registers.
 template <bool R8, int CE, int NK, int NX, int MODE>
 struct PdShape {
   static constexpr int kCols = NX * 8 * CE;                 // columns covered
@@ -538,15 +557,18 @@ __global__ void __launch_bounds__(kPdThreads, PdShape<R8, CE, NK, NX, MODE>::kCt
           acc[i][3] *= al[1];
         }
       }
-      auto weigh = [&](float (&d)[4], uint32_t b0, uint32_t b1) {
+      auto weigh = [&](float (&sum)[4], uint32_t b0, uint32_t b1) {
+        float d[4];                          // the smallest parts first
         if constexpr (R8) {
+          mma16816_zero(d, plo[0], 0u, plo[1], 0u, b0, b1);
           mma16816(d, phi[0], pmi[0], phi[1], pmi[1], b0, b1);
-          mma16816(d, plo[0], 0u, plo[1], 0u, b0, b1);
         } else {
-          mma16816(d, phi[0], phi[2], phi[1], phi[3], b0, b1);
+          mma16816_zero(d, plo[0], plo[2], plo[1], plo[3], b0, b1);
           mma16816(d, pmi[0], pmi[2], pmi[1], pmi[3], b0, b1);
-          mma16816(d, plo[0], plo[2], plo[1], plo[3], b0, b1);
+          mma16816(d, phi[0], phi[2], phi[1], phi[3], b0, b1);
         }
+        add2(sum[0], sum[1], d[0], d[1]);
+        add2(sum[2], sum[3], d[2], d[3]);
       };
       if constexpr (CE == 8) {               // columns in order: tile i holds 8 i .. 8 i + 7
 #pragma unroll

@@ -173,3 +173,44 @@ def test_forward_mode_is_refused_on_the_gpu(cuda_device):
     x = torch.randn(2, 5, device=cuda_device)
     with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
         lb.token_logprobs(forward_ad.make_dual(x, x), None)
+
+
+@pytest.mark.parametrize("gq", [1, 9])
+def test_long_sums_are_rounded_not_cut(cuda_device, gq):
+    """A long sequence's first half holds N values b with weight p = exp(-t / 32), with a token
+    of score 0 and value 0 in every 16, so that every warp weighs by the same maximum; the
+    second half's tokens have score 0, values that take N p b away again and few bits, so
+    their sums are exact.  Every CTA adds up about 128 tiles a row.  What is left, relative to the
+    sum of |p x|, of which the first half is one half, in units of 2^-23:
+      p: exp2 2, its argument 1; a tile's own products and sums, cut at three places, 3; so 3 in all
+      sums rounded to nearest: each at most half a unit of the sum so far, 128 of them 32, so
+      16 in all, without direction: next to nothing in the mean over heads and columns
+    Sums cut off at fp32's last digit lose half a unit at each of 384 places, 33 in the mean."""
+    H, D, ps, n = 32, 16, 64, 128 * 444 // 32 * 64
+    kp = torch.zeros(n // ps, H, ps, D, dtype=torch.bfloat16, device=cuda_device)
+    xp = torch.zeros_like(kp)
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    t = torch.linspace(1, 22, H, device=cuda_device).bfloat16().double()[:, None]
+    b = (1 + torch.rand(H, D, generator=g, device=cuda_device)).bfloat16().double()
+    half = n // ps // 2
+    held = torch.arange(ps, device=cuda_device) % 16 != 0
+    kp[:half, :, held, 0] = -t.bfloat16()
+    xp[:half, :, held] = b.bfloat16()[:, None]
+    total = half * int(held.sum()) * torch.exp(-t / 32) * b
+    second = half * ps - 3
+    rest, each = total.clone(), (total / second).bfloat16()
+    xp[half:] = -each[:, None]
+    rest -= second * each.double()
+    for i in range(3):                               # the last three tokens take the rest
+        part = rest.bfloat16()
+        xp[-1, :, ps - 1 - i] = -part
+        rest -= part.double()
+    assert (rest.abs() < 2.0 ** -24 * total).all()
+    weight = half * int(held.sum()) * torch.exp(-t / 32) + half * 4 + half * ps
+    q = torch.zeros(1, H * gq, 1, D, dtype=torch.bfloat16, device=cuda_device)
+    q[..., 0] = 1
+    table = torch.arange(n // ps, dtype=torch.int32, device=cuda_device)[None]
+    o = lb.paged_decode_attention(q, kp, xp, table, torch.tensor([n], dtype=torch.int32, device=cuda_device), 1 / 32)
+    off = (o.view(H, gq, D).double() - (rest / weight)[:, None]) * weight[:, None] / (2 * total)[:, None] * 2.0 ** 23
+    assert off.abs().max() <= 3 + 16 + 1 and off.mean().abs() <= 3 + 1, (off.abs().max(), off.mean())
+    _lib.check_status()
