@@ -261,6 +261,8 @@ class _StatusWatch:
     def wait_all(self) -> None:
         if self.words:
             import torch
+            if torch.cuda.is_current_stream_capturing():
+                raise LucidError("check_status waits for the GPU: call it outside the capture")
             for index in list(self.words):
                 torch.cuda.synchronize(index)
         self._take(True)

@@ -169,3 +169,24 @@ def test_a_negative_count_of_new_sequences(on_cpu):
         with pytest.raises(ValueError, match="count"):
             cache.new(bad)
     assert cache.new(0) == [] and cache.new() == [b + 1] and _held(cache, b, 0) == [1, 2]
+
+
+def test_check_status_refuses_a_capture(monkeypatch):
+    """It waits for the devices whose words it reads, which would spoil the capture."""
+    import ctypes
+    word = ctypes.c_int32(0)
+    watch = _lib._StatusWatch()
+    waited = []
+    monkeypatch.setattr(torch.cuda, "synchronize", waited.append)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    watch.wait_all()                                  # no words: nothing to wait for
+    watch.words[0] = (None, word, 0)
+    with pytest.raises(_lib.LucidError, match="outside the capture"):
+        watch.wait_all()
+    assert not waited
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    word.value = 4 | 16 << 20
+    with pytest.raises(_lib.LucidError, match="paged decoding"):
+        watch.wait_all()
+    watch.wait_all()
+    assert waited == [0, 0]
