@@ -30,8 +30,8 @@
 //
 // The products are mma.sync's: a kv head brings 1 to 16 rows a step, where a tcgen05 tile
 // has 64 or more and would hand its scores back through tensor memory for the softmax.
-// HBM bounds the pass (4 x 32765 tokens, 32 heads of 128: 2.15 GB in 324 to 340 us a call on
-// different GPUs, 6.3 to 6.6 TB/s); over 4 x 8189 tokens the tensor pipe is active 30 % of it.
+// HBM bounds the pass (4 x 32765 tokens, 32 heads of 128: 2.15 GB in 333 to 339 us a call,
+// 6.3 to 6.5 TB/s); over 4 x 8189 tokens the tensor pipe is active 30 % of it.
 #include "paged_flat.h"
 #include "serve_common.cuh"
 
@@ -104,8 +104,8 @@ __device__ __forceinline__ int pd_tiles(int n) { return (int)(((unsigned)n + kPd
 // An item counts as its tiles and kPdItemCost more in front of them, about what its
 // queries' loads and its merge of the warps cost: batches with many short sequences would
 // otherwise give some CTAs a dozen items and others none.  24 sequences of 4 to 6007 tokens
-// (4 kv heads of 68): 35.8 us without, 28.7, 24.6 and 25.7 us with 1, 2 and 4; the attention of
-// 48 sequences of 0 to 8150 tokens (4 of 128): 52.6, 48.7, 48.1 and 48.3 us.
+// (4 kv heads of 68): 37.7 us without, 30.2, 25.6 and 26.6 us with 1, 2 and 4; the attention of
+// 48 sequences of 0 to 8150 tokens (4 of 128): 52.8, 48.1, 47.5 and 48.2 us.
 __device__ __forceinline__ int pd_units(int n) { return n > 0 ? pd_tiles(n) + kPdItemCost : 0; }
 
 // units of the whole batch (every lane returns the sum)
@@ -225,10 +225,10 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
 enum : int { kRows = 0, kFull = 1, kFlat = 2 };
 
 // Three CTAs of four warps per SM where the registers allow (at most 168 a thread): the
-// tile loop is a chain of short dependent steps.  24 ragged sequences at D = 68 take 28.1 us
-// with two CTAs and 24.6 with three; at D = 128, with three stages for two CTAs and two for
-// three, 4 x 32K tokens take 334 us either way, 48 ragged sequences 46.8 and 48.1.  16 rows at
-// D > 96, and the addresses of odd rows at D > 64, need more registers.
+// tile loop is a chain of short dependent steps.  24 ragged sequences at D = 68 take 28.3 us
+// with two CTAs and 25.6 with three; at D = 128, with three stages for two CTAs and two for
+// three, 24 ragged sequences with 16 heads on 8 take 51.5 and 47.6, 4 x 32K tokens with 32 heads
+// 326 and 338 in a short run, 355 and 339 under the power cap.  16 rows at D > 96, and the addresses of odd rows at D > 64, need more registers.
 template <bool R8, int CE, int NK, int NX, int MODE>
 struct PdShape {
   static constexpr int kCols = NX * 8 * CE;                 // columns covered

@@ -11,7 +11,8 @@ A pool is [P, Hkv, page_size, D] bf16 (any strides with a unit innermost one); t
 table [B, M] int32 names the pages of each sequence in order and ``lengths`` [B] int32 the
 tokens cached so far; both live on the pool's device.  A negative length marks an unused
 place of the batch: zeros come out and nothing is written.  Only the rows below a
-sequence's length are ever read, so pages need no clearing.  What only the device can
+sequence's length are ever read, so pages need no clearing; an infinity or NaN among them
+makes its sequence's results NaN.  What only the device can
 see (a page outside the pool, a length past the block table) is not followed but
 reported: the next call of this package or ``check_status()`` raises LucidError.
 
@@ -406,8 +407,9 @@ class PagedBatch:
     ``advance()``; LucidForCausalLM.forward does all three.  ``block_table``, ``lengths``
     and ``counts`` are the device tensors the operators read; they are written in place, so
     a captured ``append`` or ``step`` follows them.  Replay it where the eager call would
-    be, after ``reserve`` (a replay checks nothing) and before ``advance``, and keep the batch as long
-    as the graph.  A batch whose table a graph reads cannot outgrow it: ``reserve`` refuses."""
+    be, after ``reserve`` (a replay checks nothing) and before ``advance`` on one stream, and
+    keep the batch as long as the graph.  A batch whose table a graph reads does not outgrow
+    it: ``reserve`` refuses."""
 
     def __init__(self, cache: PagedCache, sequences):
         self.cache = cache
