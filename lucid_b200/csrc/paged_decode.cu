@@ -30,8 +30,8 @@
 //
 // The products are mma.sync's: a kv head brings 1 to 16 rows a step, where a tcgen05 tile
 // has 64 or more and would hand its scores back through tensor memory for the softmax.
-// HBM bounds the pass (4 x 32765 tokens, 32 heads of 128: 2.15 GB in 333 to 339 us a call,
-// 6.3 to 6.5 TB/s); over 4 x 8189 tokens the tensor pipe is active 30 % of it.
+// HBM bounds the pass (4 x 32765 tokens, 32 heads of 128: 2.15 GB in 333 to 349 us a call
+// in runs of different length, 6.2 to 6.5 TB/s); over 4 x 8189 tokens the tensor pipe is active 30 % of it.
 #include "paged_flat.h"
 #include "serve_common.cuh"
 
