@@ -11,10 +11,10 @@ A pool is [P, Hkv, page_size, D] bf16 (any strides with a unit innermost one); t
 table [B, M] int32 names the pages of each sequence in order and ``lengths`` [B] int32 the
 tokens cached so far; both live on the pool's device.  A negative length marks an unused
 place of the batch: zeros come out and nothing is written.  Only the rows below a
-sequence's length are ever read, so pages need no clearing; an infinity or NaN among them
-makes its sequence's results NaN.  What only the device can
-see (a page outside the pool, a length past the block table) is not followed but
-reported: the next call of this package or ``check_status()`` raises LucidError.
+sequence's length are ever read, so pages need no clearing; an infinity or NaN among
+them can make its sequence's results NaN.  What only the device can see (a page outside the
+pool, a length past the block table) is not followed but reported: the next call of this
+package or ``check_status()`` raises LucidError.
 
 These operators are inference only; their outputs carry no gradient.  They can be captured
 into CUDA graphs; the workspace of a captured call belongs to its graph.  A sequence's
@@ -458,7 +458,8 @@ class PagedBatch:
                     shared.append(s)
                     need += 1
             need += max(0, -(-(s.length + n) // ps) - len(s.pages))
-        if self._captured and max(-(-(s.length + n) // ps) for s, n in zip(seqs, counts)) > self.block_table.shape[1]:
+        if self._captured and self.block_table.shape[1] < max(max(len(s.pages), -(-(s.length + n) // ps))
+                                                              for s, n in zip(seqs, counts)):
             raise LucidError(f"a sequence outgrows the {self.block_table.shape[1]} pages of the block table that a captured "
                              "graph reads: make a new batch of the sequences and capture again")
         if need > len(c._free):

@@ -190,3 +190,20 @@ def test_check_status_refuses_a_capture(monkeypatch):
         watch.wait_all()
     watch.wait_all()
     assert waited == [0, 0]
+
+
+def test_another_batch_grows_a_captured_batchs_sequence(on_cpu, monkeypatch):
+    """Its reserved pages alone are more than the captured table holds."""
+    cache = _cache(pages=60)
+    batch = cache.batch(cache.new())
+    k = torch.zeros(1, 1, 1, 4, dtype=torch.bfloat16)
+    batch.reserve(1)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        batch.append(0, k, k)
+    batch.advance()
+    kept, other = batch.block_table, cache.batch(batch.sequences)
+    other.reserve(4 * kept.shape[1] + 4)
+    with pytest.raises(_lib.LucidError, match="capture again"):
+        batch.reserve(1)
+    assert batch.block_table is kept
