@@ -185,7 +185,7 @@ def test_long_sums_are_rounded_not_cut(cuda_device, gq):
       p: exp2 2, its argument 1; a tile's own products and sums, cut at three places, 3; so 3 in all
       sums rounded to nearest: each at most half a unit of the sum so far, 128 of them 32, so
       16 in all, without direction: next to nothing in the mean over heads and columns
-    Sums cut off at fp32's last digit lose half a unit at each of 384 places, 33 in the mean."""
+    Sums cut off at fp32's last digit, at 384 places, left 15 in the mean and up to 105."""
     H, D, ps, n = 32, 16, 64, 128 * 444 // 32 * 64
     kp = torch.zeros(n // ps, H, ps, D, dtype=torch.bfloat16, device=cuda_device)
     xp = torch.zeros_like(kp)
